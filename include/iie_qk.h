@@ -216,6 +216,44 @@ int iie_attn_decode_batch_rows_dev(const int64_t *q_dev, const int64_t *k_dev, c
                                    int32_t *vcache_dev, long long q_ld, long long kv_ld, long long pos, long long n_seqs, long long seq_stride,
                                    long long window, const int64_t *cos_dev, const int64_t *sin_dev, int rope, int n_heads, int n_kv,
                                    int head_dim, long long cache_rows, int fa, long long inv_sqrt, int64_t *out_dev, void *stream);
+/* ---- paged key/value cache (no counterpart in the reference, whose caches are contiguous: north-mini-code/src/nmc/cohere2.py:306-322) ----
+ * kpages_dev / vpages_dev int32 [n_pages][n_kv][page_rows][head_dim]: the rows of the contiguous caches (keys after rotation) in pages;
+ * table_dev [n_seqs][table_ld]: physical page of every logical page of a sequence, position t being row t % page_rows of logical page
+ * t / page_rows.  Sequences may share pages that none of them appends to.  cos_dev / sin_dev [rope_rows][head_dim / 2]; rope as above.
+ * Positions, lengths and page numbers are read on the device: what lies outside the pool, the table or the rotation rows raises bit 4 of the
+ * flag word and is left out.  All entries: 0 ok, 1 bad argument or CUDA failure; asynchronous on `stream`; they allocate nothing and share
+ * no scratch, so calls on different streams may overlap and captured calls stay valid as long as the caller's buffers.
+ *
+ * Append: `tokens` rows of keys and values [n_kv * head_dim], int64 (narrow = 0) or int32 (1), k_ld / v_ld apart.  Sequence i takes rows
+ * rows_dev[i] .. rows_dev[i + 1] - 1 (rows_dev NULL: row i, one each) as its positions start_dev[i], start_dev[i] + 1, ...; a negative start
+ * leaves the sequence out, rows behind the last sequence's are not read.  No two sequences append to the same page.  bounds_dev (nullable)
+ * [n_pages][n_kv][2][head_dim] receives, for every page that was met, the largest and the smallest value of each key dimension over its rows
+ * up to the last one written.  A value beyond int32 raises bit 2. */
+int iie_paged_append_dev(const void *k_dev, const void *v_dev, int narrow, long long k_ld, long long v_ld, long long tokens, int32_t *kpages_dev,
+                         int32_t *vpages_dev, long long n_pages, long long page_rows, const int *table_dev, long long table_ld,
+                         const int *start_dev, const int *rows_dev, long long n_seqs, const int64_t *cos_dev, const int64_t *sin_dev,
+                         long long rope_rows, int rope, int n_kv, int head_dim, int fa, int32_t *bounds_dev, void *stream);
+/* Attention of one new token per sequence: q_dev rows [n_heads * head_dim], q_ld apart, before rotation, the token of sequence i at position
+ * lengths_dev[i] - 1, its key and value already in the cache; lengths_dev[i] = 0: no sequence, its output row is zero.  max_length bounds the
+ * lengths.  window > 0: the last `window` keys.  selected_dev (nullable) [n_seqs][n_kv][n_selected]: only the rows of these logical pages
+ * count, every entry as it stands, negative ones not at all.  Arithmetic of iie_attn_decode_dev over the keys that count.  work_dev: at
+ * least iie_paged_attn_bytes (-1: bad argument) bytes, 16-byte aligned.  out_dev [n_seqs][n_heads * head_dim]. */
+long long iie_paged_attn_bytes(long long n_seqs, long long max_length, long long window, int n_selected, long long page_rows, int n_heads,
+                               int n_kv, int head_dim);
+int iie_paged_attn_dev(const int64_t *q_dev, long long q_ld, const int32_t *kpages_dev, const int32_t *vpages_dev, long long n_pages,
+                       long long page_rows, const int *table_dev, long long table_ld, const int *lengths_dev, long long n_seqs,
+                       long long max_length, const int *selected_dev, int n_selected, long long window, const int64_t *cos_dev,
+                       const int64_t *sin_dev, long long rope_rows, int rope, int n_heads, int n_kv, int head_dim, int fa,
+                       long long inv_sqrt, void *work_dev, long long work_bytes, int64_t *out_dev, void *stream);
+/* The pages a token attends to: per sequence and KV head the first keep_first and last keep_last visible pages, then those of the highest
+ * score, the lowest page among equals, n_select in all (at most 2^31 - 1); selected_dev [n_seqs][n_kv][n_select] ascending, -1 behind them.  The score of a page
+ * is an upper bound of its keys' products with the token: the largest, over the query heads of the KV head, of
+ * sum_i max(q_i largest_i, q_i smallest_i), modulo 2^64, with the rotated query and the page's bounds_dev.  score_dev: scratch of
+ * n_seqs * n_kv * table_ld values. */
+int iie_paged_select_dev(const int64_t *q_dev, long long q_ld, const int32_t *bounds_dev, long long n_pages, long long page_rows,
+                         const int *table_dev, long long table_ld, const int *lengths_dev, long long n_seqs, int n_select, int keep_first,
+                         int keep_last, long long window, const int64_t *cos_dev, const int64_t *sin_dev, long long rope_rows, int rope,
+                         int n_heads, int n_kv, int head_dim, int fa, int64_t *score_dev, int *selected_dev, void *stream);
 /* The attention half of a decoder block for ONE token, accumulated into the residual row:
  *   x_dev [d_model] += (attention(q, cache) Wo^T), with [q | k | v] = h Wqkv^T,
  * where h is the normalised row whose digit planes the LAST single-token iie_moe_block_dev / iie_moe_forward_dev

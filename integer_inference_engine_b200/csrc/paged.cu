@@ -1,0 +1,437 @@
+// Paged key/value cache: append with rotation, ranking of pages by a bound of their scores, and the attention of one new token per
+// sequence in its general form (any head dimension, page size and number of query heads).  Arithmetic of the attention: attn.cu.
+//
+// The general form keeps scores and exponentials in memory and takes five launches: it carries the shapes that have no other.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "paged.h"
+
+namespace iie {
+
+namespace {
+
+// ---- append -------------------------------------------------------------------------------------------------------------------
+// A CTA takes the new rows of one (page, KV head): a thread keeps a pair of dimensions and walks the rows, so that the page's bounds
+// need no atomics.  They are formed again from the page's rows, old ones read back: a function of what the cache holds, whatever was
+// appended and given up before.
+constexpr int PA_THREADS = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedAppendArgs a) {
+    pdl_enter();
+    __shared__ int s_seq, s_first, s_count;
+    __shared__ long long s_page, s_row;
+    __shared__ int s_scan[PA_THREADS / 32];
+    __shared__ int s_lim[4][PA_THREADS];
+    const int tid = threadIdx.x, kv = blockIdx.y, P = a.P;
+    if (tid == 0) s_seq = -1;
+    __syncthreads();
+    // the unit-th page that new rows reach: its sequence, first new row and count
+    if (!a.rows) {
+        if (tid == 0) {
+            const int b = blockIdx.x, at = a.start[b];
+            if (at >= 0) { s_seq = b; s_page = at / P; s_first = at % P; s_count = 1; s_row = b; }
+        }
+    } else {
+        int before = 0;                                            // units of the sequences in front
+        for (int b0 = 0; b0 < a.B; b0 += PA_THREADS) {
+            const int b = b0 + tid;
+            long long at = -1, from = 0, n = 0;
+            if (b < a.B) {
+                at = a.start[b]; from = a.rows[b]; n = (long long)a.rows[b + 1] - from;
+                if (n < 0 || from < 0 || from + n > a.T) { if (blockIdx.x == 0 && kv == 0) atomicOr(a.flags, 16); n = 0; }
+                if (at < 0) n = 0;
+            }
+            const int units = n > 0 ? (int)((at + n - 1) / P - at / P + 1) : 0;
+            int upto = units;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if ((tid & 31) >= d) upto += o; }
+            if ((tid & 31) == 31) s_scan[tid >> 5] = upto;
+            __syncthreads();
+            int base = before, all = 0;
+            for (int w = 0; w < PA_THREADS / 32; w++) { if (w < (tid >> 5)) base += s_scan[w]; all += s_scan[w]; }
+            const int mine = (int)blockIdx.x - (base + upto - units);
+            if (mine >= 0 && mine < units) {
+                const long long p0 = (at / P + mine) * P, lo = max(at, p0), hi = min(at + n, p0 + P);
+                s_seq = b; s_page = p0 / P; s_first = (int)(lo - p0); s_count = (int)(hi - lo); s_row = from + (lo - at);
+            }
+            before += all;
+            __syncthreads();
+            if (s_seq >= 0 || before > (int)blockIdx.x) break;
+        }
+    }
+    __syncthreads();
+    if (s_seq < 0) return;
+    const long long logical = s_page;
+    int page = -1;
+    if (logical < a.table_ld && !(a.rope && logical * P + s_first + s_count > a.rope_rows)) page = a.table[(long long)s_seq * a.table_ld + logical];
+    if (page < 0 || page >= a.n_pages) { if (tid == 0) atomicOr(a.flags, 16); return; }
+    const int half = a.hd / 2, first = s_first, count = s_count;
+    const long long cell = ((long long)page * a.Hkv + kv) * P * a.hd;
+    int32_t *kp = a.kpages + cell, *vp = a.vpages + cell;
+    const T *k = static_cast<const T *>(a.k) + s_row * a.k_ld + (long long)kv * a.hd, *v = static_cast<const T *>(a.v) + s_row * a.v_ld + (long long)kv * a.hd;
+    bool bad = false;
+    const int width = min(half, PA_THREADS), groups = PA_THREADS / width, i_own = tid % width, g = tid / width;
+    for (int i0 = 0; i0 < half; i0 += width) {
+        const int i = i0 + i_own, d0 = a.rope == 2 ? i : 2 * i, d1 = a.rope == 2 ? i + half : 2 * i + 1;
+        int mx0 = INT32_MIN, mn0 = INT32_MAX, mx1 = INT32_MIN, mn1 = INT32_MAX;
+        if (g < groups && i < half) {
+            if (a.bounds)
+                for (int r = g; r < first; r += groups) {
+                    const int x0 = kp[(long long)r * a.hd + d0], x1 = kp[(long long)r * a.hd + d1];
+                    mx0 = max(mx0, x0); mn0 = min(mn0, x0); mx1 = max(mx1, x1); mn1 = min(mn1, x1);
+                }
+            for (int r = g; r < count; r += groups) {
+                int64_t x0 = k[r * a.k_ld + d0], x1 = k[r * a.k_ld + d1];
+                const int64_t y0 = v[r * a.v_ld + d0], y1 = v[r * a.v_ld + d1];
+                paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, logical * P + first + r, i, x0, x1);
+                bad = bad || x0 != (int32_t)x0 || x1 != (int32_t)x1 || y0 != (int32_t)y0 || y1 != (int32_t)y1;
+                const long long to = (long long)(first + r) * a.hd;
+                kp[to + d0] = (int32_t)x0; kp[to + d1] = (int32_t)x1; vp[to + d0] = (int32_t)y0; vp[to + d1] = (int32_t)y1;
+                mx0 = max(mx0, (int32_t)x0); mn0 = min(mn0, (int32_t)x0); mx1 = max(mx1, (int32_t)x1); mn1 = min(mn1, (int32_t)x1);
+            }
+        }
+        if (a.bounds) {
+            __syncthreads();
+            s_lim[0][tid] = mx0; s_lim[1][tid] = mn0; s_lim[2][tid] = mx1; s_lim[3][tid] = mn1;
+            __syncthreads();
+            if (g == 0 && i < half) {
+                for (int o = 1; o < groups; o++) {
+                    const int t = o * width + tid;
+                    mx0 = max(mx0, s_lim[0][t]); mn0 = min(mn0, s_lim[1][t]); mx1 = max(mx1, s_lim[2][t]); mn1 = min(mn1, s_lim[3][t]);
+                }
+                int32_t *to = a.bounds + ((long long)page * a.Hkv + kv) * 2 * a.hd;
+                to[d0] = mx0; to[d1] = mx1; to[a.hd + d0] = mn0; to[a.hd + d1] = mn1;
+            }
+        }
+    }
+    if (bad) atomicOr(a.flags, 4);
+}
+
+// ---- attention, general form ------------------------------------------------------------------------------------------------------
+constexpr int PG_HEADS = 8, PG_KEYS = 64;
+
+struct GeneralWork {
+    long long *score;              // [B][H][slots]: scores, then exponentials
+    long long *top;                // [B][H]
+    unsigned long long *z;         // [B][H]
+    long long *acc;                // [B][H][hd]
+};
+__host__ __device__ inline GeneralWork general_work(const PagedAttnArgs &a) {
+    GeneralWork w;
+    const long long rows = (long long)a.B * a.H;
+    w.score = static_cast<long long *>(a.work);
+    w.top = w.score + rows * a.max_slots;
+    w.z = reinterpret_cast<unsigned long long *>(w.top + rows);
+    w.acc = reinterpret_cast<long long *>(w.z + rows);
+    return w;
+}
+// Row of slot j: key j of the visible ones, or row j of the selected pages; false where there is none.
+__device__ __forceinline__ bool general_row(const PagedAttnArgs &a, const PagedSpan &s, int b, int kv, long long j, long long &row, bool &bad) {
+    long long logical, r;
+    if (a.sel) {
+        if (j >= (long long)a.n_sel * a.P) return false;
+        logical = a.sel[((long long)b * a.Hkv + kv) * a.n_sel + j / a.P];
+        r = j % a.P;
+        if (logical < 0) return false;
+        if (logical >= a.table_ld) { bad = true; return false; }
+        const long long pos = logical * a.P + r;
+        if (pos < s.lo || pos >= s.len) return false;
+    } else {
+        const long long pos = s.lo + j;
+        if (pos >= s.len) return false;
+        logical = pos / a.P; r = pos % a.P;
+    }
+    const int page = a.table[(long long)b * a.table_ld + logical];
+    if (page < 0 || page >= a.n_pages) { bad = true; return false; }
+    row = ((long long)page * a.Hkv + kv) * a.P + r;
+    return true;
+}
+
+__global__ void paged_general_init_kernel(const PagedAttnArgs a) {
+    pdl_enter();
+    const GeneralWork w = general_work(a);
+    const long long rows = (long long)a.B * a.H, n = rows * a.hd;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
+        w.acc[i] = 0;
+        if (i < rows) { w.top[i] = INT64_MIN; w.z[i] = 0; }
+    }
+}
+
+// scores of 64 slots for up to eight query heads of a KV head: a warp per key, lanes over the dimensions
+__global__ void __launch_bounds__(256) paged_general_scores_kernel(const PagedAttnArgs a) {
+    pdl_enter();
+    extern __shared__ __align__(16) int64_t pg_q[];                // [8][hd]
+    const GeneralWork w = general_work(a);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = a.H / a.Hkv, groups = (rep + PG_HEADS - 1) / PG_HEADS;
+    const int b = blockIdx.z, kv = blockIdx.y / groups, h0 = (blockIdx.y % groups) * PG_HEADS, heads = min(PG_HEADS, rep - h0), half = a.hd / 2;
+    PagedSpan s;
+    if (!paged_span(a, b, s)) { if (tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.flags, 16); return; }
+    const long long j0 = (long long)blockIdx.x * PG_KEYS;
+    if (s.len == 0 || (!a.sel && s.lo + j0 >= s.len)) return;
+    for (int idx = tid; idx < heads * half; idx += blockDim.x) {
+        const int h = idx / half, i = idx % half, d0 = a.rope == 2 ? i : 2 * i, d1 = a.rope == 2 ? i + half : 2 * i + 1;
+        const int64_t *src = a.q + b * a.q_ld + (long long)(kv * rep + h0 + h) * a.hd;
+        int64_t x0 = src[d0], x1 = src[d1];
+        paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, s.len - 1, i, x0, x1);
+        pg_q[h * a.hd + d0] = x0; pg_q[h * a.hd + d1] = x1;
+    }
+    __syncthreads();
+    long long best[PG_HEADS];
+#pragma unroll
+    for (int h = 0; h < PG_HEADS; h++) best[h] = INT64_MIN;
+    bool bad = false;
+    for (long long j = j0 + warp; j < min(j0 + PG_KEYS, a.max_slots); j += 8) {
+        long long row = 0;
+        const bool seen = general_row(a, s, b, kv, j, row, bad);
+#pragma unroll
+        for (int h = 0; h < PG_HEADS; h++) {
+            if (h >= heads) break;
+            uint64_t dot = 0;
+            if (seen) for (int d = lane; d < a.hd; d += 32) dot += (uint64_t)pg_q[h * a.hd + d] * (uint64_t)(int64_t)a.kpages[row * a.hd + d];
+#pragma unroll
+            for (int m = 16; m > 0; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
+            const long long sc = (long long)((uint64_t)((int64_t)dot >> a.fa) * (uint64_t)a.inv_sqrt) >> a.fa;
+            if (lane == 0) w.score[((long long)b * a.H + kv * rep + h0 + h) * a.max_slots + j] = seen ? sc : INT64_MIN;
+            if (seen) best[h] = max(best[h], sc);
+        }
+    }
+    if (lane == 0)
+#pragma unroll
+        for (int h = 0; h < PG_HEADS; h++)
+            if (h < heads && best[h] != INT64_MIN) atomicMax(w.top + (long long)b * a.H + kv * rep + h0 + h, best[h]);
+    if (bad && lane == 0) atomicOr(a.flags, 16);
+}
+
+__global__ void __launch_bounds__(256) paged_general_exp_kernel(const PagedAttnArgs a) {
+    pdl_enter();
+    const GeneralWork w = general_work(a);
+    const long long row = (long long)blockIdx.z * a.H + blockIdx.y, top = w.top[row];
+    if (top == INT64_MIN) return;                                   // no key
+    PagedSpan s;
+    paged_span(a, blockIdx.z, s);
+    const long long n = a.sel ? a.max_slots : min(a.max_slots, (long long)(s.len - s.lo));
+    unsigned long long z = 0;
+    for (long long j = (long long)blockIdx.x * 1024 + threadIdx.x; j < min(n, (long long)(blockIdx.x + 1) * 1024); j += 256) {
+        const long long sc = w.score[row * a.max_slots + j];
+        long long e = 0;
+        if (sc != INT64_MIN) {
+            const uint64_t below = min((uint64_t)top - (uint64_t)sc, (uint64_t)a.clip);
+            e = exp2_neg_fixed((int64_t)(below * (uint64_t)a.log2e) >> a.fa, a.fa);
+        }
+        w.score[row * a.max_slots + j] = e;
+        z += (unsigned long long)e;
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) z += __shfl_xor_sync(0xffffffffu, z, m);
+    if ((threadIdx.x & 31) == 0 && z) atomicAdd(w.z + row, z);
+}
+
+// sum of p v over 128 slots: 32 dimensions x 8 groups of slots per CTA and turn
+__global__ void __launch_bounds__(256) paged_general_values_kernel(const PagedAttnArgs a) {
+    pdl_enter();
+    __shared__ long long s_p[PG_HEADS][128];
+    __shared__ long long s_row[128];
+    const GeneralWork w = general_work(a);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = a.H / a.Hkv, groups = (rep + PG_HEADS - 1) / PG_HEADS;
+    const int b = blockIdx.z, kv = blockIdx.y / groups, h0 = (blockIdx.y % groups) * PG_HEADS, heads = min(PG_HEADS, rep - h0);
+    PagedSpan s;
+    if (!paged_span(a, b, s)) return;
+    const long long j0 = (long long)blockIdx.x * 128;
+    if (s.len == 0 || (!a.sel && s.lo + j0 >= s.len)) return;
+    bool bad = false;
+    for (int i = tid; i < 128; i += 256) {
+        long long row = -1;
+        if (j0 + i >= a.max_slots || !general_row(a, s, b, kv, j0 + i, row, bad)) row = -1;
+        s_row[i] = row;
+    }
+    __syncthreads();
+    for (int i = tid; i < heads * 128; i += 256) {
+        const int h = i >> 7, j = i & 127;
+        const long long head = (long long)b * a.H + kv * rep + h0 + h;
+        const unsigned long long z = w.z[head];
+        s_p[h][j] = s_row[j] >= 0 && z ? (long long)(((unsigned long long)w.score[head * a.max_slots + j0 + j] << a.fa) / z) : 0;
+    }
+    __syncthreads();
+    for (int d = lane; d < a.hd; d += 32) {
+        long long sum[PG_HEADS];
+#pragma unroll
+        for (int h = 0; h < PG_HEADS; h++) sum[h] = 0;
+        for (int j = warp * 16; j < warp * 16 + 16; j++) {
+            if (s_row[j] < 0) continue;
+            const long long v = a.vpages[s_row[j] * a.hd + d];
+#pragma unroll
+            for (int h = 0; h < PG_HEADS; h++) if (h < heads) sum[h] += s_p[h][j] * v;
+        }
+#pragma unroll
+        for (int h = 0; h < PG_HEADS; h++)
+            if (h < heads && sum[h]) atomicAdd(reinterpret_cast<unsigned long long *>(w.acc + ((long long)b * a.H + kv * rep + h0 + h) * a.hd + d), (unsigned long long)sum[h]);
+    }
+}
+
+__global__ void paged_general_out_kernel(const PagedAttnArgs a) {
+    pdl_enter();
+    const GeneralWork w = general_work(a);
+    const long long n = (long long)a.B * a.H * a.hd;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) a.out[i] = w.acc[i] >> a.fa;
+}
+
+// ---- ranking of pages -----------------------------------------------------------------------------------------------------------
+// score(page) = max over the heads of a KV head of sum_i max(q_i mx_i, q_i mn_i), an upper bound of q . k over the page's keys
+__global__ void __launch_bounds__(256) paged_rank_kernel(const PagedSelectArgs a) {
+    pdl_enter();
+    extern __shared__ __align__(16) int64_t pg_q[];                // [rep][hd]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = a.H / a.Hkv, b = blockIdx.z, kv = blockIdx.y, half = a.hd / 2;
+    PagedSpan s;
+    if (!paged_span(a, b, s)) { if (tid == 0 && blockIdx.x == 0 && kv == 0) atomicOr(a.flags, 16); return; }
+    const int first = s.lo / a.P, last = (s.len + a.P - 1) / a.P;      // pages first .. last - 1
+    const int page0 = first + blockIdx.x * 32;
+    if (page0 >= last) return;
+    for (int idx = tid; idx < rep * half; idx += blockDim.x) {
+        const int h = idx / half, i = idx % half, d0 = a.rope == 2 ? i : 2 * i, d1 = a.rope == 2 ? i + half : 2 * i + 1;
+        const int64_t *src = a.q + b * a.q_ld + (long long)(kv * rep + h) * a.hd;
+        int64_t x0 = src[d0], x1 = src[d1];
+        paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, s.len - 1, i, x0, x1);
+        pg_q[h * a.hd + d0] = x0; pg_q[h * a.hd + d1] = x1;
+    }
+    __syncthreads();
+    bool bad = false;
+    for (int at = page0 + warp; at < min(page0 + 32, last); at += 8) {
+        const int page = a.table[(long long)b * a.table_ld + at];
+        long long best = INT64_MIN;
+        if (page < 0 || page >= a.n_pages) bad = true;
+        else {
+            const int32_t *mx = a.bounds + ((long long)page * a.Hkv + kv) * 2 * a.hd, *mn = mx + a.hd;
+            for (int h = 0; h < rep; h++) {
+                uint64_t sum = 0;
+                for (int d = lane; d < a.hd; d += 32) {
+                    const int64_t q = pg_q[h * a.hd + d];
+                    sum += (uint64_t)q * (uint64_t)(int64_t)(q > 0 ? mx[d] : mn[d]);
+                }
+#pragma unroll
+                for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+                best = max(best, (long long)sum);
+            }
+        }
+        if (lane == 0) a.score[((long long)b * a.Hkv + kv) * a.table_ld + at - first] = best;
+    }
+    if (bad && lane == 0) atomicOr(a.flags, 16);
+}
+
+// The n_sel best pages of one (sequence, KV head): radix selection of the n_sel-th largest 64-bit score, then the pages above it and the first
+// ones equal to it, in order.
+constexpr int PS_THREADS = 1024;
+__global__ void __launch_bounds__(PS_THREADS) paged_pick_kernel(const PagedSelectArgs a) {
+    pdl_enter();
+    __shared__ int s_hist[256], s_scan[2][32], s_digit, s_left;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = blockIdx.x, b = blockIdx.y;
+    int *out = a.out + ((long long)b * a.Hkv + kv) * a.n_sel;
+    PagedSpan s;
+    const bool ok = paged_span(a, b, s);
+    const int first = s.lo / a.P, n = ok && s.len > 0 ? (s.len - 1) / a.P - first + 1 : 0, take = min(n, a.n_sel);
+    for (int i = take + tid; i < a.n_sel; i += PS_THREADS) out[i] = -1;
+    if (n <= a.n_sel) {
+        for (int i = tid; i < n; i += PS_THREADS) out[i] = first + i;
+        return;
+    }
+    const long long *score = a.score + ((long long)b * a.Hkv + kv) * a.table_ld;
+    auto key = [&](int i) -> uint64_t {                            // ascending as unsigned; pages that always count come out on top
+        if (i < a.keep_first || i >= n - a.keep_last) return ~0ULL;
+        return min((uint64_t)score[i] ^ (1ULL << 63), ~0ULL - 1);
+    };
+    uint64_t limit = 0;
+    int left = take;                                               // of the pages that share the digits found so far
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        if (tid < 256) s_hist[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += PS_THREADS) {
+            const uint64_t u = key(i);
+            if (shift == 56 || (u >> (shift + 8)) == (limit >> (shift + 8))) atomicAdd(&s_hist[(u >> shift) & 255], 1);
+        }
+        __syncthreads();
+        if (warp == 0) {                                           // the digit in which the left-th largest lies: lane l has digits 255 - 8l ..
+            int mine = 0;
+            for (int d = 0; d < 8; d++) mine += s_hist[255 - 8 * lane - d];
+            int upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
+            int above = upto - mine;
+            if (above < left && upto >= left)
+                for (int d = 0; d < 8; d++) {
+                    const int c = s_hist[255 - 8 * lane - d];
+                    if (above + c >= left) { s_digit = 255 - 8 * lane - d; s_left = left - above; break; }
+                    above += c;
+                }
+        }
+        __syncthreads();
+        limit |= (uint64_t)s_digit << shift;
+        left = s_left;
+        __syncthreads();
+    }
+    int done = 0, equal_done = 0;                                  // pages written, pages equal to the limit met
+    for (int i0 = 0; i0 < n; i0 += PS_THREADS) {
+        const int i = i0 + tid;
+        const uint64_t u = i < n ? key(i) : 0;
+        const bool eq = i < n && u == limit;
+        const unsigned eqs = __ballot_sync(0xffffffffu, eq);
+        if (lane == 0) s_scan[0][warp] = __popc(eqs);
+        __syncthreads();
+        int eq_before = equal_done + __popc(eqs & ((1u << lane) - 1)), eq_all = 0;
+        for (int w2 = 0; w2 < PS_THREADS / 32; w2++) { if (w2 < warp) eq_before += s_scan[0][w2]; eq_all += s_scan[0][w2]; }
+        const bool in = i < n && (u > limit || (eq && eq_before < left));
+        const unsigned ins = __ballot_sync(0xffffffffu, in);
+        if (lane == 0) s_scan[1][warp] = __popc(ins);
+        __syncthreads();
+        int at = done + __popc(ins & ((1u << lane) - 1)), in_all = 0;
+        for (int w2 = 0; w2 < PS_THREADS / 32; w2++) { if (w2 < warp) at += s_scan[1][w2]; in_all += s_scan[1][w2]; }
+        if (in) out[at] = first + i;
+        done += in_all; equal_done += eq_all;
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t s) {
+    if (a.B == 0 || a.T == 0) return cudaSuccess;
+    // pages that T rows of B sequences reach: a sequence's first and last page beside those its rows fill
+    const long long units = a.rows ? std::min(a.T, a.T / a.P + 2 * (long long)a.B) : a.B;
+    if (units > INT32_MAX) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)units, (unsigned)a.Hkv);
+    const cudaError_t e = a.narrow ? launch_behind(paged_append_kernel<int32_t>, grid, PA_THREADS, 0, s, a) : launch_behind(paged_append_kernel<int64_t>, grid, PA_THREADS, 0, s, a);
+    note_launch();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+size_t paged_attn_bytes(const PagedAttnArgs &a) { return (size_t)a.B * a.H * ((size_t)a.max_slots + 2 + a.hd) * 8; }
+
+cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s) {
+    const int rep = a.H / a.Hkv, pairs = a.Hkv * ((rep + PG_HEADS - 1) / PG_HEADS);
+    const unsigned flat = (unsigned)std::min<long long>(1184, ((long long)a.B * a.H * a.hd + 255) / 256);
+    const long long slots = a.max_slots;
+    launch_behind(paged_general_init_kernel, flat, 256, 0, s, a);
+    if (slots > 0) {
+        launch_behind(paged_general_scores_kernel, dim3((unsigned)((slots + PG_KEYS - 1) / PG_KEYS), pairs, a.B), 256, (size_t)PG_HEADS * a.hd * 8, s, a);
+        launch_behind(paged_general_exp_kernel, dim3((unsigned)((slots + 1023) / 1024), a.H, a.B), 256, 0, s, a);
+        launch_behind(paged_general_values_kernel, dim3((unsigned)((slots + 127) / 128), pairs, a.B), 256, 0, s, a);
+    }
+    const cudaError_t e = launch_behind(paged_general_out_kernel, flat, 256, 0, s, a);
+    note_launch(5);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
+    const size_t smem = (size_t)(a.H / a.Hkv) * a.hd * 8;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(paged_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    launch_behind(paged_rank_kernel, dim3((unsigned)((a.table_ld + 31) / 32), a.Hkv, a.B), 256, smem, s, a);
+    const cudaError_t e = launch_behind(paged_pick_kernel, dim3(a.Hkv, a.B), PS_THREADS, 0, s, a);
+    note_launch(2);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace iie

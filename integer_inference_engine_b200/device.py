@@ -175,6 +175,170 @@ def attention_decode_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc
     return out
 
 
+def _same_device(**tensors) -> None:
+    """Every tensor given lies on the current device, where the kernels run."""
+    here = torch.device("cuda", torch.cuda.current_device())
+    for name, t in tensors.items():
+        if t is not None and t.device != here:
+            raise ValueError(f"{name} lies on {t.device}, the current device is {here}")
+
+
+def _paged_pool(kpages: torch.Tensor, vpages: torch.Tensor) -> tuple:
+    if kpages.dim() != 4 or kpages.shape != vpages.shape or kpages.dtype != torch.int32 or vpages.dtype != torch.int32:
+        raise ValueError("kpages and vpages must be int32 [pages, n_kv, page rows, head_dim] of one shape")
+    if not (kpages.is_contiguous() and vpages.is_contiguous()) or kpages.numel() == 0:
+        raise ValueError("kpages and vpages must be contiguous and not empty")
+    return tuple(int(n) for n in kpages.shape)
+
+
+def _paged_table(table: torch.Tensor, per_seq: dict) -> tuple:
+    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.shape[1] == 0:
+        raise ValueError("table must be a contiguous int32 [sequences, pages of a sequence]")
+    for name, t in per_seq.items():
+        if t.dtype != torch.int32 or t.shape != (table.shape[0],) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector with an entry per row of table")
+    return int(table.shape[0]), int(table.shape[1])
+
+
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether a matrix is rows of adjacent values that do not overlap (any distance apart)."""
+    return (t.shape[0] == 0 or t.stride(1) == 1) and (t.shape[0] < 2 or t.stride(0) >= t.shape[1])
+
+
+def _paged_rope(rope: int, cos, sin, head_dim: int) -> tuple:
+    """Pointers of the rotation tables and their rows."""
+    if rope not in (0, 1, 2):
+        raise ValueError("rope is 0 (none), 1 (pairs 2i, 2i + 1) or 2 (pairs i, i + head_dim / 2)")
+    if rope == 0:
+        return None, None, 0
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t is None or t.dtype != torch.int64 or t.dim() != 2 or t.shape[1] != head_dim // 2 or not t.is_contiguous() or t.shape != cos.shape:
+            raise ValueError(f"{name} must be a contiguous int64 [positions, head_dim / 2]")
+    return cos.data_ptr(), sin.data_ptr(), int(cos.shape[0])
+
+
+def _paged_query(q: torch.Tensor, n_seqs: int, n_kv: int, head_dim: int) -> int:
+    """Query heads of q [sequences, heads * head_dim]."""
+    if q.dtype != torch.int64 or q.dim() != 2 or q.shape[0] != n_seqs or q.shape[1] == 0 or q.shape[1] % (n_kv * head_dim) or not _rows_apart(q):
+        raise ValueError("q must be int64 [sequences, heads * head_dim], heads a multiple of the KV heads, columns adjacent")
+    return int(q.shape[1]) // head_dim
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
+                 rows: torch.Tensor | None = None, fa: int = 16, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, rope: int = 0,
+                 bounds: torch.Tensor | None = None) -> None:
+    """New keys and values into a paged cache, the keys rotated at their positions on the way.
+
+    ``kpages`` / ``vpages`` int32 [pages, n_kv, page rows, head_dim] hold the rows of all sequences; ``table`` int32 [B, pages of a
+    sequence] has the physical page of every logical page (position ``t`` is row ``t % page rows`` of logical page ``t // page rows``).
+    ``k`` / ``v`` [T, n_kv * head_dim], int64 or int32, before rotation; rows may be column slices of one matrix.  Sequence ``i`` takes rows
+    ``rows[i] .. rows[i + 1] - 1`` (``rows`` int32 [B + 1]; None: row ``i``, one each) as positions ``start[i]``, ``start[i] + 1``, ...
+    (int32 [B]); a negative start leaves it out, rows behind the last sequence's are not read.  No two sequences append to one page.
+    ``bounds`` int32 [pages, n_kv, 2, head_dim] receives the largest and smallest value of every key dimension over the rows of each page
+    met, up to the last one written: what :func:`paged_select` ranks pages by.  A value beyond int32 raises bit 2, a position or page
+    outside the cache (it is left out) bit 4 of :func:`read_flags`."""
+    n_pages, n_kv, page_rows, head_dim = _paged_pool(kpages, vpages)
+    B, per_seq = _paged_table(table, {"start": start})
+    if k.dtype not in (torch.int64, torch.int32) or v.dtype != k.dtype or k.dim() != 2 or k.shape != v.shape or k.shape[1] != n_kv * head_dim:
+        raise ValueError("k and v must be int64 or int32 [rows, n_kv * head_dim] of one shape")
+    if not (_rows_apart(k) and _rows_apart(v)):
+        raise ValueError("the columns of k and v must be adjacent and their rows must not overlap")
+    if rows is None and k.shape[0] < B:
+        raise ValueError("without rows, k and v need a row per sequence")
+    if rows is not None and (rows.dtype != torch.int32 or rows.shape != (B + 1,) or not rows.is_contiguous()):
+        raise ValueError("rows must be a contiguous int32 vector with one entry more than table has rows")
+    if bounds is not None and (bounds.dtype != torch.int32 or bounds.shape != (n_pages, n_kv, 2, head_dim) or not bounds.is_contiguous()):
+        raise ValueError("bounds must be a contiguous int32 [pages, n_kv, 2, head_dim]")
+    cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
+    lib = qk_cuda._lib()
+    _same_device(k=k, v=v, kpages=kpages, vpages=vpages, table=table, start=start, rows=rows, bounds=bounds, cos=cos, sin=sin)
+    with _CUDA_LOCK:
+        rc = lib.iie_paged_append_dev(k.data_ptr(), v.data_ptr(), int(k.dtype == torch.int32), max(k.stride(0), k.shape[1]), max(v.stride(0), v.shape[1]), k.shape[0],
+                                      kpages.data_ptr(), vpages.data_ptr(), n_pages, page_rows, table.data_ptr(), per_seq, start.data_ptr(),
+                                      rows.data_ptr() if rows is not None else None, B, cos_p, sin_p, rope_rows, int(rope), n_kv, head_dim, int(fa),
+                                      bounds.data_ptr() if bounds is not None else None, _stream_ptr())
+    if rc != 0:
+        raise CudaContextError(f"paged append failed with status {rc}")
+
+
+def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, fa: int = 16,
+                    window: int = 0, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, rope: int = 0, inv_sqrt: int | None = None,
+                    pages: torch.Tensor | None = None, max_length: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """GQA attention of one new token per sequence over a paged cache (layout: :func:`paged_append`, which comes first: the token's own key
+    and value are in the cache).  ``q`` [B, heads * head_dim] int64 before rotation (rows may be column slices); ``lengths`` int32 [B]: keys of
+    each sequence, its token being at position ``lengths - 1``; 0 for a slot without a sequence, whose output is zero.  ``window`` > 0
+    keeps the last ``window`` keys.  ``pages`` int32 [B, n_kv, n] (from :func:`paged_select`): only the rows of these logical pages count, each
+    entry as it stands, negative ones not at all.  ``max_length`` bounds the lengths where the caller knows better than the table's
+    width (scratch and launch go by it; a longer sequence is left out with bit 4 of :func:`read_flags`).  Returns [B, heads * head_dim]
+    int64, the bytes :func:`attention_decode` gives over the same keys."""
+    n_pages, n_kv, page_rows, head_dim = _paged_pool(kpages, vpages)
+    B, per_seq = _paged_table(table, {"lengths": lengths})
+    n_heads = _paged_query(q, B, n_kv, head_dim)
+    if pages is not None and (pages.dtype != torch.int32 or pages.dim() != 3 or pages.shape[:2] != (B, n_kv) or pages.shape[2] == 0 or not pages.is_contiguous()):
+        raise ValueError("pages must be a contiguous int32 [sequences, n_kv, n] with n > 0")
+    if max_length is None:
+        max_length = per_seq * page_rows
+    if not 0 <= max_length <= per_seq * page_rows:
+        raise ValueError("max_length must lie within the table's pages")
+    if window < 0:
+        raise ValueError("window must not be negative (0: every key)")
+    if inv_sqrt is None:
+        inv_sqrt = int(round((1.0 / head_dim ** 0.5) * (1 << fa)))
+    if out is None:
+        out = torch.empty((B, n_heads * head_dim), dtype=torch.int64, device=q.device)
+    elif out.dtype != torch.int64 or out.shape != (B, n_heads * head_dim) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous int64 [sequences, heads * head_dim]")
+    cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
+    lib = qk_cuda._lib()
+    _same_device(q=q, kpages=kpages, vpages=vpages, table=table, lengths=lengths, pages=pages, out=out, cos=cos, sin=sin)
+    picked = 0 if pages is None else int(pages.shape[2])
+    need = lib.iie_paged_attn_bytes(B, max_length, int(window), picked, page_rows, n_heads, n_kv, head_dim)
+    if need < 0:
+        raise ValueError("a shape that paged attention does not take")
+    work = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)      # the stream's own: calls on other streams have theirs
+    with _CUDA_LOCK:
+        rc = lib.iie_paged_attn_dev(q.data_ptr(), max(q.stride(0), q.shape[1]), kpages.data_ptr(), vpages.data_ptr(), n_pages, page_rows, table.data_ptr(), per_seq, lengths.data_ptr(), B,
+                                    int(max_length), pages.data_ptr() if pages is not None else None, picked, int(window), cos_p, sin_p, rope_rows, int(rope),
+                                    n_heads, n_kv, head_dim, int(fa), int(inv_sqrt), work.data_ptr(), need, out.data_ptr(), _stream_ptr())
+    if rc != 0:
+        raise CudaContextError(f"paged attention failed with status {rc}")
+    return out
+
+
+def paged_select(q: torch.Tensor, bounds: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, page_rows: int, n_select: int, keep_first: int = 1,
+                 keep_last: int = 1, fa: int = 16, window: int = 0, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, rope: int = 0,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """The ``n_select`` logical pages of every sequence and KV head that the new token attends to: the first ``keep_first`` and last
+    ``keep_last`` visible ones, then those whose keys can score highest, judged by the page's ``bounds`` (:func:`paged_append`): the largest, over
+    the query heads of the KV head, of ``sum_i max(q_i largest_i, q_i smallest_i)``, modulo 2**64; the lowest page among equals.
+    ``q``, ``table``, ``lengths``, ``window`` and the rotation as for :func:`paged_attention`.  Returns int32 [B, n_kv, n_select], ascending, -1 behind
+    the last: its ``pages``."""
+    if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.dtype != torch.int32 or not bounds.is_contiguous() or bounds.numel() == 0:
+        raise ValueError("bounds must be a contiguous int32 [pages, n_kv, 2, head_dim]")
+    n_pages, n_kv, _, head_dim = (int(n) for n in bounds.shape)
+    B, per_seq = _paged_table(table, {"lengths": lengths})
+    n_heads = _paged_query(q, B, n_kv, head_dim)
+    if page_rows <= 0 or n_select <= 0 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > n_select:
+        raise ValueError("page_rows and n_select must be positive, keep_first + keep_last at most n_select")
+    if window < 0:
+        raise ValueError("window must not be negative (0: every key)")
+    if out is None:
+        out = torch.empty((B, n_kv, n_select), dtype=torch.int32, device=q.device)
+    elif out.dtype != torch.int32 or out.shape != (B, n_kv, n_select) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous int32 [sequences, n_kv, n_select]")
+    cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
+    lib = qk_cuda._lib()
+    _same_device(q=q, bounds=bounds, table=table, lengths=lengths, out=out, cos=cos, sin=sin)
+    score = torch.empty((B, n_kv, per_seq), dtype=torch.int64, device=q.device)
+    with _CUDA_LOCK:
+        rc = lib.iie_paged_select_dev(q.data_ptr(), max(q.stride(0), q.shape[1]), bounds.data_ptr(), n_pages, int(page_rows), table.data_ptr(), per_seq, lengths.data_ptr(), B, int(n_select),
+                                      int(keep_first), int(keep_last), int(window), cos_p, sin_p, rope_rows, int(rope), n_heads, n_kv, head_dim, int(fa),
+                                      score.data_ptr(), out.data_ptr(), _stream_ptr())
+    if rc != 0:
+        raise CudaContextError(f"page selection failed with status {rc}")
+    return out
+
+
 def attention_block(wqkv: int, wo: int, x: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor, pos: int, n_heads: int,
                     n_kv: int, head_dim: int, fa: int = 16, fw: int = 24, window: int = 0, cos: torch.Tensor | None = None,
                     sin: torch.Tensor | None = None, rope: int = 0, inv_sqrt: int | None = None,
