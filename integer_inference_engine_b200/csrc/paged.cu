@@ -405,9 +405,13 @@ cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t s) {
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-size_t paged_attn_bytes(const PagedAttnArgs &a) { return (size_t)a.B * a.H * ((size_t)a.max_slots + 2 + a.hd) * 8; }
+size_t paged_attn_bytes(const PagedAttnArgs &a) {
+    if (paged_tc_ok(a)) return paged_tc_bytes(a);
+    return (size_t)a.B * a.H * ((size_t)a.max_slots + 2 + a.hd) * 8;
+}
 
 cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s) {
+    if (paged_tc_ok(a)) return launch_paged_tc(a, s);
     const int rep = a.H / a.Hkv, pairs = a.Hkv * ((rep + PG_HEADS - 1) / PG_HEADS);
     const unsigned flat = (unsigned)std::min<long long>(1184, ((long long)a.B * a.H * a.hd + 255) / 256);
     const long long slots = a.max_slots;

@@ -45,12 +45,16 @@ struct PagedAttnArgs {
     int rope, H, Hkv, hd, fa, B;
     long long inv_sqrt, log2e, clip;
     long long max_slots;           // keys of a sequence at most: visible ones, or rows of the selected pages
-    void *work;                    // paged_attn_bytes
+    void *work;                    // paged_attn_bytes, 16-byte aligned
     int64_t *out;                  // [B][H * hd]
     int *flags;
 };
 size_t paged_attn_bytes(const PagedAttnArgs &a);
 cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s);
+// the form on tcgen05 (paged_tc.cu): whether a shape is its own, its scratch, its launches
+bool paged_tc_ok(const PagedAttnArgs &a);
+size_t paged_tc_bytes(const PagedAttnArgs &a);
+cudaError_t launch_paged_tc(const PagedAttnArgs &a, cudaStream_t s);
 
 struct PagedSelectArgs {
     const int64_t *q;

@@ -21,6 +21,7 @@ bool shape_ok(int n_heads, int n_kv, int hd, int fa, int rope, const void *cos, 
     return n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 && n_heads <= 65535 && hd >= 2 && hd <= PAGED_MAX_HEAD && (hd & 1) == 0 && fa >= 1 && fa <= 29 &&
            rope >= 0 && rope <= 2 && (rope == 0 || (cos && sin && rope_rows > 0));
 }
+// (rows of a table, and of a pool and its KV heads, are numbered in 31 bits)
 bool pool_ok(long long n_pages, long long P, long long n_seqs, long long table_ld) {
     return n_pages > 0 && n_pages <= INT32_MAX && P > 0 && P <= INT32_MAX && n_seqs >= 0 && n_seqs <= 65535 && table_ld > 0 && table_ld <= INT32_MAX / P;
 }
@@ -29,8 +30,9 @@ long long slots_of(long long max_length, long long window, long long n_sel, long
     if (n_sel > 0) return n_sel * P;
     return window > 0 ? std::min(window, max_length) : max_length;
 }
-PagedAttnArgs attn_shape(long long n_seqs, long long max_length, long long window, int n_sel, long long P, int n_heads, int n_kv, int hd) {
+PagedAttnArgs attn_shape(long long n_seqs, long long max_length, long long window, int n_sel, long long P, int n_heads, int n_kv, int hd, int fa) {
     PagedAttnArgs a = {};
+    a.fa = fa;
     a.B = (int)n_seqs; a.H = n_heads; a.Hkv = n_kv; a.hd = hd; a.P = (int)P; a.n_sel = n_sel; a.window = window;
     a.max_len = max_length; a.max_slots = slots_of(max_length, window, n_sel, P);
     return a;
@@ -62,10 +64,10 @@ extern "C" int iie_paged_append_dev(const void *k_dev, const void *v_dev, int na
     return 0;
 }
 
-extern "C" long long iie_paged_attn_bytes(long long n_seqs, long long max_length, long long window, int n_selected, long long page_rows, int n_heads, int n_kv, int head_dim) {
-    if (!pool_ok(1, page_rows, n_seqs, 1) || !shape_ok(n_heads, n_kv, head_dim, 16, 0, nullptr, nullptr, 0) || n_selected < 0 || max_length < 0 || max_length > INT32_MAX ||
+extern "C" long long iie_paged_attn_bytes(long long n_seqs, long long max_length, long long window, int n_selected, long long page_rows, int n_heads, int n_kv, int head_dim, int fa) {
+    if (!pool_ok(1, page_rows, n_seqs, 1) || !shape_ok(n_heads, n_kv, head_dim, fa, 0, nullptr, nullptr, 0) || n_selected < 0 || max_length < 0 || max_length > INT32_MAX ||
         (long long)n_selected * page_rows > INT32_MAX) return -1;
-    PagedAttnArgs a = attn_shape(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim);
+    PagedAttnArgs a = attn_shape(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim, fa);
     a.B = (int)slab_of(a);
     return (long long)paged_attn_bytes(a);
 }
@@ -76,14 +78,15 @@ extern "C" int iie_paged_attn_dev(const int64_t *q_dev, long long q_ld, const in
                                   int head_dim, int fa, long long inv_sqrt, void *work_dev, long long work_bytes, int64_t *out_dev, void *stream) {
     if (!pool_ok(n_pages, page_rows, n_seqs, table_ld) || !shape_ok(n_heads, n_kv, head_dim, fa, rope, cos_dev, sin_dev, rope_rows) ||
         q_ld < (long long)n_heads * head_dim || max_length < 0 || max_length > table_ld * page_rows || (selected_dev ? n_selected <= 0 : n_selected != 0) ||
-        (long long)n_selected * page_rows > INT32_MAX) return 1;
+        (long long)n_selected * page_rows > INT32_MAX || n_pages > INT32_MAX / page_rows / n_kv ||
+        ((reinterpret_cast<uintptr_t>(kpages_dev) | reinterpret_cast<uintptr_t>(vpages_dev) | reinterpret_cast<uintptr_t>(work_dev)) & 15)) return 1;
     if (n_seqs == 0) return 0;
     int *flags = shared_flag_word();
-    const long long need = iie_paged_attn_bytes(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim);
+    const long long need = iie_paged_attn_bytes(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim, fa);
     if (!flags || !q_dev || !kpages_dev || !vpages_dev || !table_dev || !lengths_dev || !out_dev || need < 0 || work_bytes < need || (need > 0 && !work_dev)) return 1;
-    PagedAttnArgs a = attn_shape(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim);
+    PagedAttnArgs a = attn_shape(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim, fa);
     a.q_ld = q_ld; a.kpages = kpages_dev; a.vpages = vpages_dev; a.n_pages = (int)n_pages; a.table_ld = table_ld;
-    a.cos = cos_dev; a.sin = sin_dev; a.rope_rows = rope_rows; a.rope = rope; a.fa = fa; a.inv_sqrt = inv_sqrt; a.log2e = sigmoid_log2e(fa);
+    a.cos = cos_dev; a.sin = sin_dev; a.rope_rows = rope_rows; a.rope = rope; a.inv_sqrt = inv_sqrt; a.log2e = sigmoid_log2e(fa);
     a.clip = std::min(((long long)(fa + 2) << (2 * fa)) / a.log2e, (1LL << 62) / a.log2e);
     a.work = work_dev; a.flags = flags;
     const long long slab = slab_of(a);

@@ -188,6 +188,8 @@ def _paged_pool(kpages: torch.Tensor, vpages: torch.Tensor) -> tuple:
         raise ValueError("kpages and vpages must be int32 [pages, n_kv, page rows, head_dim] of one shape")
     if not (kpages.is_contiguous() and vpages.is_contiguous()) or kpages.numel() == 0:
         raise ValueError("kpages and vpages must be contiguous and not empty")
+    if (kpages.data_ptr() | vpages.data_ptr()) & 15:
+        raise ValueError("kpages and vpages must start on 16 bytes")
     return tuple(int(n) for n in kpages.shape)
 
 
@@ -292,7 +294,7 @@ def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     lib = qk_cuda._lib()
     _same_device(q=q, kpages=kpages, vpages=vpages, table=table, lengths=lengths, pages=pages, out=out, cos=cos, sin=sin)
     picked = 0 if pages is None else int(pages.shape[2])
-    need = lib.iie_paged_attn_bytes(B, max_length, int(window), picked, page_rows, n_heads, n_kv, head_dim)
+    need = lib.iie_paged_attn_bytes(B, max_length, int(window), picked, page_rows, n_heads, n_kv, head_dim, int(fa))
     if need < 0:
         raise ValueError("a shape that paged attention does not take")
     work = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)      # the stream's own: calls on other streams have theirs

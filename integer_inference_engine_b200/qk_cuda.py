@@ -98,7 +98,7 @@ def _signatures():
         "iie_attn_decode_batch_rows_dev": ([vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, vp, vp, c_int, c_int, c_int, c_int, i64, c_int, i64, vp, vp], c_int),
         "iie_attn_decode_batch_dev": ([vp, vp, vp, vp, vp, i64, i64, i64, i64, vp, vp, c_int, c_int, c_int, c_int, i64, c_int, i64, vp, vp], c_int),
         "iie_paged_append_dev": ([vp, vp, c_int, i64, i64, i64, vp, vp, i64, i64, vp, i64, vp, vp, i64, vp, vp, i64, c_int, c_int, c_int, c_int, vp, vp], c_int),
-        "iie_paged_attn_bytes": ([i64, i64, i64, c_int, i64, c_int, c_int, c_int], i64),
+        "iie_paged_attn_bytes": ([i64, i64, i64, c_int, i64, c_int, c_int, c_int, c_int], i64),
         "iie_paged_attn_dev": ([vp, i64, vp, vp, i64, i64, vp, i64, vp, i64, i64, vp, c_int, i64, vp, vp, i64, c_int, c_int, c_int, c_int, c_int, i64, vp, i64, vp, vp], c_int),
         "iie_paged_select_dev": ([vp, i64, vp, i64, i64, vp, i64, vp, i64, c_int, c_int, c_int, i64, vp, vp, i64, c_int, c_int, c_int, c_int, c_int, vp, vp, vp], c_int),
         "iie_attn_block_dev": ([i64, i64, vp, vp, vp, i64, vp, i64, vp, vp, c_int, c_int, c_int, c_int, i64, c_int, c_int, i64, vp], c_int),

@@ -66,11 +66,11 @@ def test_tensors_of_another_device_are_refused(name):
 
 def test_scratch_of_attention(lib):
     size = lib.iie_paged_attn_bytes
-    assert 0 < size(1, 300, 0, 0, 16, 32, 4, 128) < size(1, 4096, 0, 0, 16, 32, 4, 128)
-    assert size(8, 32000, 2048, 0, 16, 32, 4, 128) < size(8, 32000, 0, 0, 16, 32, 4, 128)
-    assert size(1000, 100000, 0, 0, 16, 32, 4, 128) < 6 << 30                # parts behind one another
-    for bad in ((-1, 10, 0, 0, 16, 4, 2, 64), (1, -1, 0, 0, 16, 4, 2, 64), (1, 10, 0, -1, 16, 4, 2, 64), (1, 10, 0, 0, 0, 4, 2, 64), (1, 10, 0, 0, 16, 5, 2, 64), (1, 10, 0, 0, 16, 4, 2, 63),
-                (1, 10, 0, 1 << 30, 16, 4, 2, 64), (70000, 10, 0, 0, 16, 4, 2, 64)):
+    assert 0 < size(1, 300, 0, 0, 16, 32, 4, 128, 16) < size(1, 4096, 0, 0, 16, 32, 4, 128, 16)
+    assert size(8, 32000, 2048, 0, 16, 32, 4, 128, 16) < size(8, 32000, 0, 0, 16, 32, 4, 128, 16)
+    assert size(1000, 100000, 0, 0, 16, 32, 4, 128, 16) < 6 << 30                # parts behind one another
+    for bad in ((-1, 10, 0, 0, 16, 4, 2, 64, 16), (1, -1, 0, 0, 16, 4, 2, 64, 16), (1, 10, 0, -1, 16, 4, 2, 64, 16), (1, 10, 0, 0, 0, 4, 2, 64, 16), (1, 10, 0, 0, 16, 5, 2, 64, 16), (1, 10, 0, 0, 16, 4, 2, 63, 16), (1, 10, 0, 0, 16, 4, 2, 64, 0),
+                (1, 10, 0, 1 << 30, 16, 4, 2, 64, 16), (70000, 10, 0, 0, 16, 4, 2, 64, 16)):
         assert size(*bad) == -1, bad
 
 
@@ -86,7 +86,7 @@ def test_c_entries_refuse(lib):
     attn = lambda **c: lib.iie_paged_attn_dev(*{**dict(q=None, q_ld=256, kp=None, vp=None, n_pages=9, P=16, table=None, ld=5, lengths=None, B=3, max_length=80, sel=None, n_sel=0, window=0, cos=None, sin=None, rr=0,
                                                     rope=0, H=4, kv=2, hd=64, fa=16, inv=8192, work=None, bytes=1 << 30, out=None, stream=None), **c}.values())
     assert attn() == 1
-    for c in (dict(q_ld=255), dict(max_length=81), dict(n_sel=2), dict(H=5), dict(rope=2), dict(fa=31), dict(bytes=0), dict(max_length=-1)):
+    for c in (dict(q_ld=255), dict(max_length=81), dict(n_sel=2), dict(H=5), dict(rope=2), dict(fa=31), dict(bytes=0), dict(max_length=-1), dict(n_pages=1 << 29), dict(work=8), dict(kp=4), dict(vp=1)):
         assert attn(**c) == 1, c
     assert attn(B=0) == 0
     select = lambda **c: lib.iie_paged_select_dev(*{**dict(q=None, q_ld=256, bounds=None, n_pages=9, P=16, table=None, ld=5, lengths=None, B=3, n=4, first=1, last=1, window=0, cos=None, sin=None, rr=0, rope=0, H=4,
