@@ -400,6 +400,11 @@ cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t s) {
     const long long units = a.rows ? std::min(a.T, a.T / a.P + 2 * (long long)a.B) : a.B;
     if (units > INT32_MAX) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)units, (unsigned)a.Hkv);
+    // all of an SM's memory as shared memory, as the attention behind has it: an SM changes only while it is idle
+    for (const void *kernel : {(const void *)paged_append_kernel<int64_t>, (const void *)paged_append_kernel<int32_t>}) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return e;
+    }
     const cudaError_t e = a.narrow ? launch_behind(paged_append_kernel<int32_t>, grid, PA_THREADS, 0, s, a) : launch_behind(paged_append_kernel<int64_t>, grid, PA_THREADS, 0, s, a);
     note_launch();
     return e != cudaSuccess ? e : cudaGetLastError();

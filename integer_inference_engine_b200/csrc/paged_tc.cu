@@ -2,18 +2,20 @@
 //
 // An int32 is its four bytes, so a row of keys is a row of 4 hd bytes, and with the query's balanced base-256 digits d_a (modulo 2^64)
 //     q . k = sum_s 2^(8 s) sum_i sum_{b <= s} k_i,b d_{s-b}(q_i)          s = 0 .. 7, modulo 2^64:
-// eight products of the raw bytes with eight columns per head that hold digit s - b beside byte b.  No key is unpacked: TMA puts rows into
+// products of the raw bytes with eight columns per head that hold digit s - b beside byte b.  No key is unpacked: TMA puts rows into
 // shared memory, 128 keys x 64 columns (8 heads) x 4 hd bytes is one MMA shape, and a query of any 64 bits needs nothing else.  The top byte
 // of an int32 is signed and the others are not; an MMA takes its operand as one or the other, so that the tile is multiplied twice, by the
 // columns of bytes 0 .. 2 and by those of byte 3.  Values likewise: bytes of the value rows, transposed by the operand descriptor (the sum runs
 // over keys), times the three bytes of the probabilities floor(e 2^fa / Z) <= 2^fa; byte 3 of a value is read from the signed product,
-// the others from the unsigned one.  Every sum stays below 2^31: 4 hd 255 128 for a score, 255^2 per key for an output (segments
-// of at most 256 tiles of 128 keys).
+// the others from the unsigned one.  Every sum stays below 2^31: 4 hd 255 128 for a score, 255^2 per key for an output (at most 256 tiles
+// of 128 keys before the sums are read out).
 //
-// The softmax floors e and p, which takes the maximum and the normaliser of all keys in front of the values: three launches with the scores between
-// them in memory, as 32-bit distances below the maximum of 32 keys and eight heads (a distance beyond `clip` has no weight, so nothing
-// is lost).  Tiles of all sequences and KV heads form one list that the CTAs share evenly, whatever the lengths: a tile is sixteen
-// groups of eight rows, a group lies in one page.  A pair whose tiles fall to several CTAs adds its output sums up in memory (integers: in any order).
+// Tiles of 128 keys of all sequences and KV heads form one list that one CTA per SM share evenly, whatever the lengths.  The softmax floors e
+// and p, which takes the maximum and then the normaliser of all of a pair's keys (pair: a sequence's KV head with up to eight query heads) in
+// front of its values: a CTA takes the scores of all its tiles (in memory, as 32-bit distances below the maximum of 32 keys; one beyond
+// `clip` has no weight, so nothing is lost), the normalisers, then the values.  Pairs that lie in one CTA need nobody else; those cut
+// between CTAs (at most one begins in each) exchange maximum, normaliser and output sums in memory, in a cell of the CTA where they
+// begin.  The launch is cooperative, every wait is bounded, and integers are added in any order.  A small kernel in front clears the cells.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,56 +30,75 @@ namespace iie {
 namespace {
 
 constexpr int PT_KEYS = 128, PT_GROUPS = 16;       // keys of a tile, groups of eight
-constexpr int PT_HEADS = 8;                        // query heads of a pair: a (sequence, KV head, up to eight heads)
-constexpr int PT_WORKERS = 8;                      // warps that read TMEM out and write operands
-constexpr int PT_THREADS = 64 + 32 * PT_WORKERS;
-constexpr int PT_META = 8;                         // tiles whose group masks are kept
-constexpr int PT_MAX_STAGES = 6;
+constexpr int PT_HEADS = 8;                        // query heads of a pair at most
+constexpr int PT_WORKERS = 16;                     // warps that read TMEM out and write operands: sets of four, one for each quarter of the keys; tile i is set i % 4's
+constexpr int PT_SETS = PT_WORKERS / 4;
+constexpr int PT_FIRST = 4;                         // warps in front of them: two that request copies, one that issues products
+constexpr int PT_THREADS = 32 * (PT_FIRST + PT_WORKERS);
+constexpr int PT_MAX_SLOTS = 13;                   // of the ring, 16 KB each: 128 bytes of 128 rows
+constexpr int PT_META = 16;                        // tiles whose row masks are kept: those in the ring and two on their way out of TMEM
+constexpr uint32_t PT_SLOT = PT_KEYS * 128, PT_PROBS = PT_KEYS * 32;
 constexpr int PT_MAX_SEGMENT = 256;                // tiles that one accumulation takes: 256 * 128 * 255^2 < 2^31
+constexpr unsigned PT_POLLS = 1u << 20;            // of another CTA's count, half a microsecond and more each
+constexpr unsigned long long PT_BIAS = 1ULL << 63; // maxima are kept as unsigned: zero is below every score
 
+struct TcCell {                                    // of a pair cut between CTAs
+    unsigned long long top[PT_HEADS], z[PT_HEADS];
+    unsigned tops, zs, done[PT_WORKERS];           // tiles whose maxima and normalisers are in, counted by every warp; whose sums are, warp by warp
+};
 struct TcWork {
-    uint32_t *dist;                // [tiles][128][8] distances below the base
-    long long *base;               // [tiles][4][8] largest score of 32 keys
-    long long *top;                // [pairs][8]
-    unsigned long long *z;         // [pairs][8]
-    unsigned long long *acc;       // [pairs][8][hd]
-    unsigned *done;                // [pairs] tiles whose sums are in acc, counted by every warp
+    uint32_t *dist;                // [tiles][8 heads][4 quarters][32] distances below the base (shifted, at most the limit): key k of a quarter at (k & 3) 8 + (k >> 2), so that the
+                                   // eight keys t, t + 4, .. of a lane lie side by side
+    long long *base;               // [tiles][4 quarters][8] largest score of 32 keys
+    unsigned long long *top, *z;   // [pairs][16 warps][8] of pairs that lie in one CTA
+    TcCell *cell;                  // [CTAs]
+    unsigned long long *acc;       // [CTAs][8][hd]
 };
 __host__ __device__ inline int tc_head_groups(const PagedAttnArgs &a) { return (a.H / a.Hkv + PT_HEADS - 1) / PT_HEADS; }
 __host__ __device__ inline int tc_group_heads(const PagedAttnArgs &a) { const int g = tc_head_groups(a); return (a.H / a.Hkv + g - 1) / g; }
+// rows that a box of TMA brings, within a page (larger ones are slower: chunk after chunk of one SM alone 5.5 TB/s in all with 16 rows, 4.6 with 32 to 128)
+__host__ __device__ inline int tc_box(const PagedAttnArgs &a) { return a.P % 16 == 0 ? 16 : 8; }
 // tiles of a pair at most
 __host__ __device__ inline long long tc_tiles_most(const PagedAttnArgs &a) {
     if (a.n_sel > 0) return ((long long)a.n_sel * a.P + PT_KEYS - 1) / PT_KEYS;
-    return (a.max_slots / 8 + 2 + PT_GROUPS - 1) / PT_GROUPS;
+    return (a.max_slots + 2 * tc_box(a) + PT_KEYS - 1) / PT_KEYS;
 }
-__host__ __device__ inline TcWork tc_work(const PagedAttnArgs &a, size_t *bytes = nullptr) {
+__host__ __device__ inline TcWork tc_work(const PagedAttnArgs &a, int ctas, size_t *bytes = nullptr) {
     const long long pairs = (long long)a.B * a.Hkv * tc_head_groups(a), tiles = pairs * tc_tiles_most(a);
     TcWork w;
     w.dist = static_cast<uint32_t *>(a.work);
     w.base = reinterpret_cast<long long *>(w.dist + tiles * PT_KEYS * PT_HEADS);
-    w.top = w.base + tiles * 4 * PT_HEADS;
-    w.z = reinterpret_cast<unsigned long long *>(w.top + pairs * PT_HEADS);
-    w.acc = w.z + pairs * PT_HEADS;
-    w.done = reinterpret_cast<unsigned *>(w.acc + pairs * PT_HEADS * a.hd);
-    if (bytes) *bytes = (size_t)tiles * (PT_KEYS * PT_HEADS * 4 + 4 * PT_HEADS * 8) + (size_t)pairs * (PT_HEADS * 16 + (size_t)PT_HEADS * a.hd * 8 + 4);
+    w.top = reinterpret_cast<unsigned long long *>(w.base + tiles * 4 * PT_HEADS);
+    w.z = w.top + pairs * PT_WORKERS * PT_HEADS;
+    w.cell = reinterpret_cast<TcCell *>(w.z + pairs * PT_WORKERS * PT_HEADS);
+    w.acc = reinterpret_cast<unsigned long long *>(w.cell + ctas);
+    if (bytes) *bytes = (size_t)tiles * (PT_KEYS * PT_HEADS * 4 + 4 * PT_HEADS * 8) + (size_t)pairs * PT_WORKERS * PT_HEADS * 16 + (size_t)ctas * (sizeof(TcCell) + (size_t)PT_HEADS * a.hd * 8);
     return w;
 }
 
 __device__ __forceinline__ int tc_tiles(const PagedAttnArgs &a, const PagedSpan &s) {
     if (s.len == 0) return 0;
     if (a.sel) return (int)tc_tiles_most(a);
-    return (((s.len + 7) >> 3) - (s.lo >> 3) + PT_GROUPS - 1) / PT_GROUPS;
+    const int box = tc_box(a);
+    return (s.len - s.lo / box * box + PT_KEYS - 1) / PT_KEYS;
 }
 
-// One role's walk over the CTA's share of the list: tiles of sequence b, pair by pair.
+// A walk over a run of the list, tile by tile.
 struct TcWalk {
-    int b, pair_of, t, nt, left, tile, seg;        // pair of the sequence, tile of the pair, its tiles, tiles left, number in the list, tiles of the segment so far
+    int b, pair_of, t, nt, left, tile, part, seg;  // sequence; its pair; tile of the pair, its tiles; tiles left; number in the list; tiles of the pair and of the accumulation before this one
     PagedSpan s;
     __device__ __forceinline__ void load(const PagedAttnArgs &a) { paged_span(a, b, s); nt = tc_tiles(a, s); }
+    __device__ __forceinline__ bool ends_part() const { return t + 1 == nt || left == 1; }             // of the pair, in this CTA
+    __device__ __forceinline__ bool ends_segment() const { return ends_part() || seg + 1 == PT_MAX_SEGMENT; }
+    __device__ __forceinline__ int rest() const { return min(nt - t, left); }                        // tiles of the pair from here on, in this CTA
     __device__ __forceinline__ void next(const PagedAttnArgs &a, int per_seq) {
         seg = ends_segment() ? 0 : seg + 1;
-        left--; tile++;
-        if (++t < nt || left == 0) return;
+        part = ends_part() ? 0 : part + 1;
+        skip(a, per_seq, 1);
+    }
+    __device__ __forceinline__ void skip(const PagedAttnArgs &a, int per_seq, int n) {               // n <= rest()
+        left -= n; tile += n; t += n;
+        if (t < nt || left == 0) return;
         t = 0;
         if (++pair_of < per_seq) return;
         pair_of = 0;
@@ -86,16 +107,20 @@ struct TcWalk {
             load(a);
         } while (nt == 0);
     }
-    __device__ __forceinline__ bool ends_segment() const { return t + 1 == nt || left == 1 || seg + 1 == PT_MAX_SEGMENT; }
 };
 
-// The whole CTA: its share [first, first + left) of the list and the place where it begins.  scan: 33 ints of shared memory.
-__device__ __forceinline__ void tc_share(const PagedAttnArgs &a, int *scan, TcWalk &w, bool flag) {
+// The whole CTA: its share of the list, as up to three runs: the pair that begins in a CTA before (or goes on beyond, where there is no
+// other), the pair that goes on in the next one, the whole pairs between them.  Returns the list's length.  scan: 40 ints of shared memory.
+// Of the two cut pairs the one that an even CTA has in common with the odd one before it is run 0 of both: its maxima are there while the
+// CTAs are at the scores of the rest, its normaliser while they are at the values of whole pairs, and the other pair's while they are at the
+// values of this one.
+enum { RUN_WHOLE = 2, RUNS };
+__device__ __forceinline__ uint32_t tc_share(const PagedAttnArgs &a, int *scan, TcWalk (&run)[RUNS]) {
     const int tid = threadIdx.x, n = blockDim.x, lane = tid & 31, warp = tid >> 5, per_seq = a.Hkv * tc_head_groups(a), warps = n >> 5;
     auto count = [&](int b) {
         PagedSpan s;
         if (b >= a.B) return 0;
-        if (!paged_span(a, b, s) && flag) atomicOr(a.flags, 16);
+        if (!paged_span(a, b, s) && blockIdx.x == 0) atomicOr(a.flags, 16);
         return tc_tiles(a, s);
     };
     const int own = count(tid);
@@ -103,17 +128,15 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, int *scan, TcWa
     for (int b = tid + n; b < a.B; b += n) mine += count(b);
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) scan[warp] = mine;
+    if (tid == 0) scan[32] = scan[34] = -1;
     __syncthreads();
     int all = 0;
     for (int i = 0; i < warps; i++) all += scan[i];
     __syncthreads();
-    const long long total = (long long)all * per_seq;
-    const int from = (int)(total * blockIdx.x / gridDim.x);
-    w.left = (int)(total * (blockIdx.x + 1) / gridDim.x) - from;
-    w.tile = from; w.seg = 0;
-    if (tid == 0) scan[32] = -1;
+    const uint32_t total = (uint32_t)all * per_seq;  // (total * 256 fits 32 bits: paged_tc_ok)
+    const int from = (int)(total * blockIdx.x / gridDim.x), to = (int)(total * (blockIdx.x + 1) / gridDim.x);
     int before = 0;                                // tiles per pair of the sequences in front
-    for (int b0 = 0; b0 < a.B; b0 += n) {
+    for (int b0 = 0; b0 < a.B && from < to; b0 += n) {
         const int c = b0 == 0 ? own : count(b0 + tid);
         int upto = c;
 #pragma unroll
@@ -122,589 +145,758 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, int *scan, TcWa
         __syncthreads();
         int sum = 0;
         for (int i = 0; i < warps; i++) { if (i < warp) upto += scan[i]; sum += scan[i]; }
-        const long long lo = (long long)(before + upto - c) * per_seq;
-        if (c > 0 && from >= lo && from < lo + (long long)c * per_seq) { scan[32] = b0 + tid; scan[31] = (int)(from - lo); }
+        const int lo = (before + upto - c) * per_seq, hi = lo + c * per_seq;
+        if (from >= lo && from < hi) { scan[32] = b0 + tid; scan[33] = from - lo; }
+        if (to > lo && to <= hi) { scan[34] = b0 + tid; scan[35] = to - 1 - lo; }
         before += sum;
         __syncthreads();
-        if (scan[32] >= 0) break;
+        if (scan[32] >= 0 && scan[34] >= 0) break;
         __syncthreads();
     }
-    w.b = scan[32] < 0 ? 0 : scan[32];
-    w.load(a);
-    const int at = scan[31];
-    w.pair_of = w.nt > 0 ? at / w.nt : 0;
-    w.t = w.nt > 0 ? at - w.pair_of * w.nt : 0;
-    if (scan[32] < 0) w.left = 0;
-}
-
-// Producer's lane l < 16: rows of group l of the walk's tile that count, as a byte; the row of the pool where it lies.
-__device__ __forceinline__ uint32_t tc_group(const PagedAttnArgs &a, const TcWalk &w, int kv, int l, int &row) {
-    int logical, r, pos;
-    if (a.sel) {
-        const unsigned slot = ((unsigned)w.t * PT_GROUPS + l) * 8, i = slot / (unsigned)a.P;
-        if (i >= (unsigned)a.n_sel) return 0;
-        r = (int)(slot - i * a.P);
-        logical = a.sel[((long long)w.b * a.Hkv + kv) * a.n_sel + i];
-        if (logical < 0) return 0;
-        if (logical >= a.table_ld) { atomicOr(a.flags, 16); return 0; }
-        pos = logical * a.P + r;                   // (a table's rows are numbered in 31 bits)
-    } else {
-        pos = ((w.s.lo >> 3) + w.t * PT_GROUPS + l) * 8;
-        logical = (int)((unsigned)pos / (unsigned)a.P);
-        r = pos - logical * a.P;
+    if (tid == 0) {
+        TcWalk w = {}, none = {};
+        w.left = to - from; w.tile = from;
+        const int head = blockIdx.x & 1, tail = head ^ 1;
+        run[0] = run[1] = run[RUN_WHOLE] = none;
+        if (w.left > 0 && scan[32] >= 0 && scan[34] >= 0) {
+            w.b = scan[32];
+            w.load(a);
+            w.pair_of = scan[33] / w.nt; w.t = scan[33] - w.pair_of * w.nt;
+            if (w.rest() < w.nt) {
+                run[head] = w;
+                run[head].left = w.rest();
+                w.skip(a, per_seq, w.rest());
+            }
+            if (w.left > 0) {
+                TcWalk e = none;
+                e.b = scan[34];
+                e.load(a);
+                e.pair_of = scan[35] / e.nt;
+                e.left = scan[35] - e.pair_of * e.nt + 1;
+                e.tile = to - e.left;
+                if (e.left < e.nt) { run[tail] = e; w.left -= e.left; }
+                run[RUN_WHOLE] = w;
+            }
+        }
     }
-    const int from = max(w.s.lo - pos, 0), to = min(w.s.len - pos, 8);
-    if (from >= to) return 0;
-    const int page = a.table[(long long)w.b * a.table_ld + logical];
-    if (page < 0 || page >= a.n_pages) { atomicOr(a.flags, 16); return 0; }
-    row = (page * a.Hkv + kv) * a.P + r;
-    return ((1u << to) - 1) & ~((1u << from) - 1);
+    return total;
 }
+// the CTA where tile `tile` of the list lies
+__device__ __forceinline__ int tc_owner(int tile, uint32_t total) { return (int)((((uint32_t)tile + 1) * gridDim.x - 1) / total); }
 
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t stride, uint32_t swizzle) {      // stride between groups of eight rows
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ULL << 16) | ((uint64_t)(stride >> 4) << 32) | (1ULL << 46) | ((uint64_t)swizzle << 61);
+// Runs in the order of the scores are as they are numbered: what other CTAs wait for comes first.  Values: whole pairs first, while normalisers
+// of the others are on their way.
+__device__ __forceinline__ int tc_value_run(int u) { return u == 0 ? RUN_WHOLE : u - 1; }
+
+// Operand descriptors: the lower word has the address (in 16 bytes), the upper one the distance of groups of eight rows and the swizzle.  An
+// MMA's descriptors are a constant away from those of its chunk: with both words computed for each, a product takes 250 clocks to issue, so 48
+// (128 x 64 x 32) and 40 (128 x 32 x 32), what reading the operands from shared memory takes.
+__device__ __forceinline__ uint32_t tc_desc(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__host__ __device__ constexpr uint32_t tc_desc_upper(uint32_t stride, uint32_t swizzle) { return (stride >> 4) | (1u << 14) | (swizzle << 29); }
+// (The collector cannot keep A for the second product: it holds what the first one made of the bytes' signs.)
+template <uint32_t UPPER_A, uint32_t UPPER_B>
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t da, uint32_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %6};\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], x, y, %3, p;\n}"
+                 ::"r"(d), "r"(da), "r"(db), "r"(idesc), "r"(accumulate), "n"(UPPER_A), "n"(UPPER_B) : "memory");
 }
 constexpr uint32_t SW128 = 2, SW32 = 6;
-template <int N>
-__device__ __forceinline__ void tc_ld(uint32_t addr, int (&r)[N]) {
-    static_assert(N == 8 || N == 32, "");
-    if constexpr (N == 8)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
-    else
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-                       "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-                       "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                     : "r"(addr));
+__device__ __forceinline__ uint64_t tc_min(uint64_t x, long long most) { return x < (uint64_t)most ? x : (uint64_t)most; }
+__device__ __forceinline__ void tc_ld8(uint32_t addr, int (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr));
 }
 __device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap *map, int x, int row, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar) : "memory");
+}
 
-struct TcShape { int chunks, stages, columns; };   // 128-byte chunks of a row, tiles in flight, TMEM columns
+// 128-byte chunks of a row, ring slots, TMEM columns, those of the scores (behind the outputs, or over their second buffer)
+struct TcShape { int chunks, slots, columns, score_at; };
 
-// what both product kernels keep in shared memory beside tiles and operands
 struct TcBars {
-    uint64_t full[PT_MAX_STAGES], empty[PT_MAX_STAGES], meta[PT_META];
-    uint64_t acc_full[2], acc_free[2], op_full[2], op_free[2], drain;
+    uint64_t full[PT_MAX_SLOTS], empty[PT_MAX_SLOTS], meta[PT_META];
+    uint64_t score_full[PT_SETS], score_free[2], query_full, prob_full[PT_SETS], prob_free[PT_SETS], out_full[2], out_free[2], pair_done, drain;
     uint32_t tmem;
-    int abort, scan[33];
+    int abort, scan[40];
+    TcWalk run[RUNS];
     unsigned char mask[PT_META][PT_GROUPS];
 };
 
-// The producer warp: tiles of the list into the ring, sixteen boxes of eight rows each.
-__device__ __forceinline__ void tc_produce(const PagedAttnArgs &a, TcWalk w, const CUtensorMap *map, TcBars &s, uint32_t ring, TcShape sh, volatile int *abort_flag) {
-    const int lane = threadIdx.x & 31, per_seq = a.Hkv * tc_head_groups(a), groups = tc_head_groups(a);
-    const uint32_t group_bytes = (uint32_t)sh.chunks * 1024, tile_bytes = group_bytes * PT_GROUPS;
-    int slot = 0, issued = 0;
+struct TcRing {
+    int slot = 0;
     uint32_t pass = 0;
-    for (; w.left > 0; issued++) {
-        int row = 0;
-        const uint32_t rows = lane < PT_GROUPS ? tc_group(a, w, w.pair_of / groups, lane, row) : 0;
-        if (issued >= sh.stages && !tl_wait(tl_u32(&s.empty[slot]), pass ^ 1, abort_flag)) break;
-        if (lane < PT_GROUPS) s.mask[issued % PT_META][lane] = (unsigned char)rows;
-        const uint32_t some = __ballot_sync(0xffffffffu, rows != 0);
-        if (lane == 0) { tl_arrive(tl_u32(&s.meta[issued % PT_META])); tl_expect(tl_u32(&s.full[slot]), (uint32_t)__popc(some) * group_bytes); }
-        __syncwarp();
-        if (rows) tl_tma(ring + slot * tile_bytes + lane * group_bytes, map, 0, row, 0, tl_u32(&s.full[slot]));
-        w.next(a, per_seq);
-        if (++slot == sh.stages) { slot = 0; pass ^= 1; }
-    }
-    if (*abort_flag) {                             // copies under way end before the CTA does
-        __syncwarp();
-        for (int k = max(0, issued - sh.stages); k < issued; k++) {
-            volatile int patient = 0;
-            tl_wait(tl_u32(&s.full[k % sh.stages]), (uint32_t)(k / sh.stages) & 1, &patient);
-        }
-    }
+    __device__ __forceinline__ void step(int n) { if (++slot == n) { slot = 0; pass ^= 1; } }
+};
+
+// One thread's wait (tl_wait: a whole warp's, at twice the price).
+__device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    return tl_try(bar, parity) || tl_wait_slow(bar, parity, abort_flag);
 }
 
-__device__ __forceinline__ void tc_begin(TcBars &s, int columns, int writers) {      // writers: warps that write an operand
-    const int tid = threadIdx.x;
-    if (tid == 0) {
-        s.abort = 0;
-        for (int i = 0; i < PT_MAX_STAGES; i++) { tl_init(tl_u32(&s.full[i]), 1); tl_init(tl_u32(&s.empty[i]), 1); }
-        for (int i = 0; i < PT_META; i++) tl_init(tl_u32(&s.meta[i]), 1);
-        for (int i = 0; i < 2; i++) {
-            tl_init(tl_u32(&s.acc_full[i]), 1); tl_init(tl_u32(&s.acc_free[i]), PT_WORKERS);
-            tl_init(tl_u32(&s.op_full[i]), writers); tl_init(tl_u32(&s.op_free[i]), 1);
+// The two producer warps: the share's tiles into the ring, chunk by chunk in turn, a box per page (or part of one).  A chunk costs a thread 500
+// clocks (a wait, the bytes to expect, up to sixteen boxes), and the memory's rate is one in 700 for each SM: one warp alone, which looked every
+// box's page up in a lane of its own, took 1200.  The next tile's pages are looked up while this one's boxes are requested.
+struct TcBoxes {
+    uint32_t rows, sends, bytes;                   // this lane's rows that count; groups where a box begins; bytes of a chunk
+    int row;                                       // of the box in the pool, in the lane where it begins
+};
+// a lane's group of the tile: where its page number stands in memory (asked for a tile ahead), and what else decides its rows
+struct TcLook { uint32_t rows; int r, page; };
+// Lane l < 16: rows of group l of the walk's tile that count by their positions, as a byte; the page's number on its way.
+__device__ __forceinline__ TcLook tc_look(const PagedAttnArgs &a, const TcWalk &w, int kv, int box) {
+    const int l = threadIdx.x & 31;
+    TcLook x = {0, 0, 0};
+    int logical, pos;
+    if (w.left <= 0 || l >= PT_GROUPS) return x;
+    if (a.sel) {
+        const unsigned slot = ((unsigned)w.t * PT_GROUPS + l) * 8, i = slot / (unsigned)a.P;
+        if (i >= (unsigned)a.n_sel) return x;
+        x.r = (int)(slot - i * a.P);
+        logical = a.sel[((long long)w.b * a.Hkv + kv) * a.n_sel + i];
+        if (logical < 0) return x;
+        if (logical >= a.table_ld) { atomicOr(a.flags, 16); return x; }
+        pos = logical * a.P + x.r;                 // (a table's rows are numbered in 31 bits)
+    } else {
+        pos = w.s.lo / box * box + (w.t * PT_GROUPS + l) * 8;
+        logical = (int)((unsigned)pos / (unsigned)a.P);
+        x.r = pos - logical * a.P;
+    }
+    const int from = max(w.s.lo - pos, 0), to = min(w.s.len - pos, 8);
+    if (from >= to) return x;
+    x.rows = ((1u << to) - 1) & ~((1u << from) - 1);
+    x.page = __ldg(a.table + (long long)w.b * a.table_ld + logical);
+    return x;
+}
+__device__ __forceinline__ TcBoxes tc_boxes(const PagedAttnArgs &a, const TcLook &look, int kv, int box) {
+    const int lane = threadIdx.x & 31, in_box = box / 8, first = lane & ~(in_box - 1);
+    TcBoxes x;
+    x.rows = look.rows;
+    if (x.rows && (look.page < 0 || look.page >= a.n_pages)) { atomicOr(a.flags, 16); x.rows = 0; }
+    const int row = (look.page * a.Hkv + kv) * a.P + look.r;
+    const uint32_t some = __ballot_sync(0xffffffffu, x.rows != 0), mine = (some >> first) & ((1u << in_box) - 1);      // a box goes where one of its groups counts
+    const int known = first + (mine ? __ffs(mine) - 1 : 0);
+    x.row = __shfl_sync(0xffffffffu, row, known) - 8 * (known - first);
+    x.sends = __ballot_sync(0xffffffffu, lane < PT_GROUPS && lane == first && mine != 0);
+    x.bytes = (uint32_t)__popc(x.sends) * box * 128;
+    return x;
+}
+// IN_BOX: groups of eight rows that a box brings.  `turn`: chunks requested so far, by both warps; `tile`: tiles.  (Asking the values into L2 ahead
+// of the ring, too, while the normalisers are exchanged, was slower by a fifth: every other access waits behind them.)
+template <int IN_BOX, bool KEYS>
+__device__ __forceinline__ bool tc_produce(const PagedAttnArgs &a, TcWalk w, const CUtensorMap *map, TcBars &s, uint32_t ring, const TcShape &sh, int me, TcRing &at, int &turn, int &tile, volatile int *abort_flag) {
+    const int lane = threadIdx.x & 31, groups = tc_head_groups(a), per_seq = a.Hkv * groups;
+    constexpr uint32_t ALL = IN_BOX == 1 ? 0xFFFFu : 0x5555u;
+    if (w.left == 0) return true;
+    int kv = w.pair_of / groups;
+    TcLook look = tc_look(a, w, kv, 8 * IN_BOX);
+    while (w.left > 0) {
+        const TcBoxes x = tc_boxes(a, look, kv, 8 * IN_BOX);
+        w.next(a, per_seq);
+        kv = w.pair_of / groups;
+        look = tc_look(a, w, kv, 8 * IN_BOX);      // of the next tile: used after this one's copies
+        int row[PT_GROUPS / IN_BOX];
+#pragma unroll
+        for (int j = 0; j < PT_GROUPS / IN_BOX; j++) row[j] = __shfl_sync(0xffffffffu, x.row, j * IN_BOX);
+        for (int c = 0; c < sh.chunks; c++, turn++, at.step(sh.slots)) {
+            if ((turn & 1) != me) continue;
+            if (turn >= sh.slots && !tl_wait(tl_u32(&s.empty[at.slot]), at.pass ^ 1, abort_flag)) return false;
+            const bool marks = KEYS && c == 0;
+            if (marks) {
+                if (lane < PT_GROUPS) s.mask[tile % PT_META][lane] = (unsigned char)x.rows;
+                __syncwarp();
+            }
+            if (tl_elect()) {
+                const uint32_t bar = tl_u32(&s.full[at.slot]), to = ring + at.slot * PT_SLOT;
+                if (marks) tl_arrive(tl_u32(&s.meta[tile % PT_META]));
+                tl_expect(bar, x.bytes);
+                if (x.sends == ALL) {
+#pragma unroll
+                    for (int j = 0; j < PT_GROUPS / IN_BOX; j++) tc_tma(to + j * IN_BOX * 1024, map, 32 * c, row[j], bar);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < PT_GROUPS / IN_BOX; j++)
+                        if ((x.sends >> (j * IN_BOX)) & 1) tc_tma(to + j * IN_BOX * 1024, map, 32 * c, row[j], bar);
+                }
+            }
+            __syncwarp();
         }
-        tl_init(tl_u32(&s.drain), 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        tile++;
     }
-    if (tid >> 5 == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tl_u32(&s.tmem)), "r"(columns));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
-    tc_before();
-    __syncthreads();
-    tc_after();
+    return true;
 }
-// The issuing warp, where a wait gave up: products under way end before their TMEM is given back.
-__device__ __forceinline__ void tc_drain(TcBars &s) {
-    if (!*(volatile int *)&s.abort) return;
-    if (tl_elect()) tl_commit(tl_u32(&s.drain));
-    __syncwarp();
-    volatile int patient = 0;
-    tl_wait(tl_u32(&s.drain), 0, &patient);
-}
-__device__ __forceinline__ void tc_end(TcBars &s, int columns, int *flags) {
-    tc_before();
-    __syncthreads();
-    if (threadIdx.x >> 5 == 1) {
-        tc_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem), "r"(columns));
+template <int IN_BOX>
+__device__ __forceinline__ void tc_producer(const PagedAttnArgs &a, const CUtensorMap *kmap, const CUtensorMap *vmap, TcBars &s, uint32_t ring, const TcShape &sh, int me, volatile int *abort_flag) {
+    TcRing at;
+    int turn = 0, tile = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int u = 0; ok && u < RUNS; u++) ok = tc_produce<IN_BOX, true>(a, s.run[u], kmap, s, ring, sh, me, at, turn, tile, abort_flag);
+#pragma unroll 1
+    for (int u = 0; ok && u < RUNS; u++) ok = tc_produce<IN_BOX, false>(a, s.run[tc_value_run(u)], vmap, s, ring, sh, me, at, turn, tile, abort_flag);
+    if (!*abort_flag) return;
+    __syncwarp();                                  // copies under way end before the CTA does
+    for (int k = max(0, turn - sh.slots); k < turn; k++) {
+        volatile int patient = 0;
+        if ((k & 1) == me) tl_wait(tl_u32(&s.full[k % sh.slots]), (uint32_t)(k / sh.slots) & 1, &patient);
     }
-    if (threadIdx.x == 0 && s.abort) atomicOr(flags, FLAG_GAVE_UP);
 }
 
 // Query columns of one pair: column 8 h + s holds digit s - b of q_i at byte 4 i + b, bytes 0 .. 2 in one operand and byte 3 in the other.
-// A thread takes four dimensions of a head.
+// A thread takes four dimensions of a head and four columns.
 __device__ __forceinline__ void tc_queries(const PagedAttnArgs &a, const TcWalk &w, int heads, int padded, unsigned char *lower, unsigned char *upper, int worker) {
     const int groups = tc_head_groups(a), kv = w.pair_of / groups, h0 = kv * (a.H / a.Hkv) + (w.pair_of % groups) * tc_group_heads(a), quads = a.hd / 4, half = a.hd / 2;
     const long long pos = w.s.len - 1;
-    for (int task = worker; task < padded * quads; task += 32 * PT_WORKERS) {
-        const int h = task / quads, j = task - h * quads, d = 4 * j;
+#pragma unroll 1
+    for (int task = worker; task < 2 * padded * quads; task += 32 * PT_WORKERS) {
+        const int row = task / quads, j = task - row * quads, d = 4 * j, h = row >> 1, s0 = 4 * (row & 1);
         int64_t y[4] = {0, 0, 0, 0};
         if (h < heads) {
             const int64_t *q = a.q + (long long)w.b * a.q_ld + (long long)(h0 + h) * a.hd;
-            if (a.rope == 2) {
-                const bool second = d >= half;
-                const int i = second ? d - half : d;
+            const bool second = a.rope == 2 && d >= half;
+            // pairs (x0, x1): of rope 2 four, each giving one value; else two, each giving both
+            const int i0 = a.rope == 2 ? (second ? d - half : d) : 2 * j;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    int64_t x0 = q[i + e], x1 = q[i + e + half];
-                    paged_rotate(a.cos, a.sin, 2, a.hd, a.fa, pos, i + e, x0, x1);
+            for (int e = 0; e < 4; e++) {
+                if (a.rope == 2) {
+                    int64_t x0 = q[i0 + e], x1 = q[i0 + e + half];
+                    paged_rotate(a.cos, a.sin, 2, a.hd, a.fa, pos, i0 + e, x0, x1);
                     y[e] = second ? x1 : x0;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = q[d + e];
-                paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, pos, 2 * j, y[0], y[1]);
-                paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, pos, 2 * j + 1, y[2], y[3]);
+                } else y[e] = q[d + e];
+            }
+            if (a.rope == 1) {
+                paged_rotate(a.cos, a.sin, 1, a.hd, a.fa, pos, i0, y[0], y[1]);
+                paged_rotate(a.cos, a.sin, 1, a.hd, a.fa, pos, i0 + 1, y[2], y[3]);
             }
         }
-        uint32_t hi[4], lo[4];                     // digits, first one on top
+        uint64_t digits[4];                        // first digit on top
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const uint64_t digits = ((uint64_t)y[e] + 0x8080808080808080ULL) ^ 0x8080808080808080ULL;
-            hi[e] = __byte_perm((uint32_t)digits, 0, 0x0123); lo[e] = __byte_perm((uint32_t)(digits >> 32), 0, 0x0123);
+            const uint64_t v = ((uint64_t)y[e] + 0x8080808080808080ULL) ^ 0x8080808080808080ULL;
+            digits[e] = (uint64_t)__byte_perm((uint32_t)v, 0, 0x0123) << 32 | __byte_perm((uint32_t)(v >> 32), 0, 0x0123);
         }
-        const uint32_t at = (uint32_t)(j >> 3) * (uint32_t)padded * 1024;
-#pragma unroll
-        for (int s = 0; s < 8; s++) {
+        const uint32_t at = (uint32_t)(j >> 3) * (uint32_t)padded * 1024 + (uint32_t)h * 1024;
+#pragma unroll 1
+        for (int s = s0; s < s0 + 4; s++) {
             uint32_t x[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = s < 4 ? hi[e] >> (24 - 8 * s) : (s == 7 ? lo[e] : __funnelshift_r(lo[e], hi[e], 56 - 8 * s));
-            const uint32_t to = at + (uint32_t)(8 * h + s) * 128 + (uint32_t)(((j & 7) ^ s) * 16);
+            for (int e = 0; e < 4; e++) x[e] = (uint32_t)(digits[e] >> (56 - 8 * s));
+            const uint32_t to = at + (uint32_t)s * 128 + (uint32_t)(((j & 7) ^ s) * 16);
             *reinterpret_cast<uint4 *>(lower + to) = make_uint4(x[0] & 0xFFFFFFu, x[1] & 0xFFFFFFu, x[2] & 0xFFFFFFu, x[3] & 0xFFFFFFu);
             *reinterpret_cast<uint4 *>(upper + to) = make_uint4(x[0] & 0xFF000000u, x[1] & 0xFF000000u, x[2] & 0xFF000000u, x[3] & 0xFF000000u);
         }
     }
 }
 
-// ---- scores ---------------------------------------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(PT_THREADS, 1) paged_scores_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap map, const TcShape sh) {
-    extern __shared__ unsigned char pt_raw[];
-    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) TcBars s;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per_seq = a.Hkv * tc_head_groups(a);
-    const int heads_most = tc_group_heads(a), padded = (heads_most + 1) & ~1;
-    const uint32_t operand = (uint32_t)sh.chunks * padded * 1024, tile_bytes = (uint32_t)sh.chunks * 1024 * PT_GROUPS;
-    unsigned char *lower = smem, *upper = smem + operand;
-    const uint32_t ring = tl_u32(smem) + 2 * operand;
-    volatile int *abort_flag = &s.abort;
-    tc_begin(s, sh.columns, PT_WORKERS);
+// The cells of pairs that are cut between CTAs, cleared.  The attention's launch overlaps it: what lies in front of this kernel on the stream
+// has ended when the attention's CTAs start, so that only the cells are waited for.
+__global__ void paged_clear_kernel(TcCell *cell, unsigned long long *acc, int per_cta) {
     pdl_enter();
-    const TcWork work = tc_work(a);
-    {                                              // what the kernels behind add to
-        const long long pairs = (long long)a.B * per_seq, n = pairs * PT_HEADS * a.hd;
-        for (long long i = (long long)blockIdx.x * PT_THREADS + tid; i < n; i += (long long)gridDim.x * PT_THREADS) {
-            work.acc[i] = 0;
-            if (i < pairs) work.done[i] = 0;
-            if (i < pairs * PT_HEADS) work.z[i] = 0;
-        }
-    }
-    TcWalk w;
-    tc_share(a, s.scan, w, blockIdx.x == 0);
-    const uint32_t tmem = s.tmem;
-    if (warp == 0) tc_produce(a, w, &map, s, ring, sh, abort_flag);
-    else if (warp == 1) {
-        const uint32_t n = (uint32_t)padded * 8;
-        int slot = 0, queries = 0;
-        uint32_t pass = 0;
-        bool fresh = true;
-        for (int i = 0; w.left > 0; i++) {
-            bool ok = tl_wait(tl_u32(&s.full[slot]), pass, abort_flag);
-            if (ok && i >= 2) ok = tl_wait(tl_u32(&s.acc_free[i & 1]), ((i >> 1) & 1) ^ 1, abort_flag);
-            if (ok && fresh) { ok = tl_wait(tl_u32(&s.op_full[0]), queries & 1, abort_flag); queries++; }
-            if (!ok) break;
-            tc_after();
-            if (tl_elect()) {
-                const uint32_t tile = ring + slot * tile_bytes;
-#pragma unroll 1
-                for (int side = 0; side < 2; side++) {
-                    const uint32_t b = tl_u32(side ? upper : lower);
-#pragma unroll 1
-                    for (int c = 0; c < sh.chunks; c++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tl_mma(tmem + (i & 1) * 64, tc_desc(tile + c * 1024 + k * 32, (uint32_t)sh.chunks * 1024, SW128),
-                                   tc_desc(b + (uint32_t)c * padded * 1024 + k * 32, 1024, SW128), tl_idesc((int)n, side == 1), (side | c | k) != 0);
-                }
-                tl_commit(tl_u32(&s.empty[slot]));
-                tl_commit(tl_u32(&s.acc_full[i & 1]));
-            }
-            __syncwarp();
-            fresh = w.t + 1 == w.nt;
-            w.next(a, per_seq);
-            if (++slot == sh.stages) { slot = 0; pass ^= 1; }
-        }
-        tc_drain(s);
-    } else {
-        const int worker = tid - 64, half = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane;      // a warp reads TMEM lanes 32 (warp % 4) ..
-        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * 32;
-        const bool serves = 4 * half < heads_most;
-        bool fresh = true;
-        for (int i = 0; w.left > 0; i++) {
-            if (fresh) {                           // (the last tile of the pair in front has been multiplied: its sums were waited for)
-                const int g = w.pair_of % tc_head_groups(a);
-                tc_queries(a, w, min(heads_most, a.H / a.Hkv - g * heads_most), padded, lower, upper, worker);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) tl_arrive(tl_u32(&s.op_full[0]));
-            }
-            if (!tl_wait(tl_u32(&s.meta[i % PT_META]), (uint32_t)(i / PT_META) & 1, abort_flag)) break;
-            const bool seen = (s.mask[i % PT_META][key >> 3] >> (key & 7)) & 1;
-            if (!tl_wait(tl_u32(&s.acc_full[i & 1]), (i >> 1) & 1, abort_flag)) break;
-            tc_after();
-            int r[32];
-            if (serves) { tc_ld(from + (i & 1) * 64, r); tc_ld_wait(); }
-            tc_before();
-            __syncwarp();
-            if (lane == 0) tl_arrive(tl_u32(&s.acc_free[i & 1]));
-            if (serves) {
-                uint32_t d[4];
-                long long base = INT64_MIN;
-#pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    const int *c = r + 8 * h;
-                    const uint64_t low = (uint64_t)((long long)c[0] + (long long)c[1] * 256 + (long long)c[2] * 65536 + (long long)c[3] * 16777216);
-                    const uint32_t high = (uint32_t)c[4] + ((uint32_t)c[5] << 8) + ((uint32_t)c[6] << 16) + ((uint32_t)c[7] << 24);
-                    const long long dot = (long long)(low + ((uint64_t)high << 32));
-                    const long long score = (long long)((uint64_t)(dot >> a.fa) * (uint64_t)a.inv_sqrt) >> a.fa;
-                    // the largest of the warp's 32 keys: by the upper words, then by the lower ones where those are equal
-                    const int up = seen ? (int)(score >> 32) : INT32_MIN;
-                    const int up_most = __reduce_max_sync(0xffffffffu, up);
-                    const uint32_t low_most = __reduce_max_sync(0xffffffffu, seen && up == up_most ? (uint32_t)score : 0u);
-                    const long long most = (long long)(((uint64_t)(uint32_t)up_most << 32) | low_most);
-                    d[h] = seen ? (uint32_t)min((uint64_t)most - (uint64_t)score, (uint64_t)0xFFFFFFFEu) : 0xFFFFFFFFu;
-                    if (lane == h) base = most;
-                }
-                *reinterpret_cast<uint4 *>(work.dist + ((long long)w.tile * PT_KEYS + key) * PT_HEADS + 4 * half) = make_uint4(d[0], d[1], d[2], d[3]);
-                const bool any = __any_sync(0xffffffffu, seen);
-                if (lane < 4) work.base[((long long)w.tile * 4 + quarter) * PT_HEADS + 4 * half + lane] = any ? base : INT64_MIN;
-            }
-            fresh = w.t + 1 == w.nt;
-            w.next(a, per_seq);
-        }
-    }
-    tc_end(s, sh.columns, a.flags);
+    const int tid = threadIdx.x;
+    if (tid < (int)(sizeof(TcCell) / 8)) reinterpret_cast<unsigned long long *>(cell + blockIdx.x)[tid] = 0;
+    for (int i = tid; i < per_cta; i += blockDim.x) acc[(long long)blockIdx.x * per_cta + i] = 0;
 }
 
-// ---- normalisers: the largest score of a pair, the sum of its exponentials -------------------------------------------------------------
-constexpr int PN_THREADS = 256;
-
-template <bool SHORT>
-__global__ void __launch_bounds__(PN_THREADS) paged_norm_kernel(const PagedAttnArgs a) {
-    using Exp = std::conditional_t<SHORT, SoftmaxExp16, SoftmaxExp>;
-    __shared__ int scan[33];
-    __shared__ long long s_most[PN_THREADS / 32][PT_HEADS];
-    __shared__ unsigned long long s_z[PT_HEADS];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, per_seq = a.Hkv * tc_head_groups(a);
-    pdl_enter();
-    TcWalk w;
-    tc_share(a, scan, w, false);
-    const TcWork work = tc_work(a);
-    const Exp exp2(a.fa, a.log2e, a.clip);
-    const int half = tid & 1, key = tid >> 1, quarter = key >> 5, heads = tc_group_heads(a);
-    while (w.left > 0) {
-        const long long pair = (long long)w.b * per_seq + w.pair_of;
-        const int count = min(w.nt - w.t, w.left), first = w.tile - w.t;       // tiles of the pair here; its first one
-        long long most = INT64_MIN;
-        for (int i = tid >> 3; i < w.nt * 4; i += PN_THREADS / 8) most = max(most, work.base[((long long)first * 4 + i) * PT_HEADS + (tid & 7)]);
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
-        if (lane < 8) s_most[warp][lane] = most;
-        if (tid < PT_HEADS) s_z[tid] = 0;
-        __syncthreads();
-        long long top[4];
-#pragma unroll
-        for (int h = 0; h < 4; h++) {
-            top[h] = INT64_MIN;
-            for (int v = 0; v < PN_THREADS / 32; v++) top[h] = max(top[h], s_most[v][4 * half + h]);
-        }
-        if (w.t == 0 && tid < 2)
-            for (int h = 0; h < 4; h++) work.top[pair * PT_HEADS + 4 * half + h] = top[h];
-        unsigned long long z[4] = {0, 0, 0, 0};
-        if (4 * half < heads)
-            for (int i = 0; i < count; i++) {
-                const uint4 d4 = *reinterpret_cast<const uint4 *>(work.dist + ((long long)(w.tile + i) * PT_KEYS + key) * PT_HEADS + 4 * half);
-                const uint32_t d[4] = {d4.x, d4.y, d4.z, d4.w};
-                const long long *base = work.base + ((long long)(w.tile + i) * 4 + quarter) * PT_HEADS + 4 * half;
-#pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    if (d[h] == 0xFFFFFFFFu) continue;                     // no key
-                    const uint64_t below = min((uint64_t)top[h] - (uint64_t)base[h], (uint64_t)a.clip) + d[h];
-                    z[h] += (unsigned)exp2((uint32_t)min(below, (uint64_t)a.clip));
-                }
-            }
-#pragma unroll
-        for (int h = 0; h < 4; h++) {
-#pragma unroll
-            for (int m = 2; m < 32; m <<= 1) z[h] += __shfl_xor_sync(0xffffffffu, z[h], m);
-            if (lane < 2 && z[h]) atomicAdd(&s_z[4 * half + h], z[h]);
-        }
-        __syncthreads();
-        if (tid < heads && s_z[tid]) atomicAdd(work.z + pair * PT_HEADS + tid, s_z[tid]);
-        w.left -= count; w.tile += count; w.t += count;
-        if (w.left > 0) {                          // (the pair is through)
-            w.t = 0;
-            if (++w.pair_of == per_seq) {
-                w.pair_of = 0;
-                do {
-                    if (++w.b >= a.B) { w.left = 0; break; }
-                    w.load(a);
-                } while (w.nt == 0);
-            }
-        }
-        __syncthreads();
+// Exponential of a distance from the row's maximum, at most `limit`, where it is zero (a key that does not count stands there): of the general
+// scale, and of fa = 16, where distances are kept shifted so that every product's shift is that of its upper word: 24 clocks a warp
+// (six products of four, eight other instructions of two on another pipe) against 75.  The polynomial stays above 2^14 there.
+struct TcExp {
+    SoftmaxExp exp2;
+    static constexpr int SHIFT = 0;
+    uint32_t limit;
+    __device__ __forceinline__ TcExp(const PagedAttnArgs &a) : exp2(a.fa, a.log2e, a.clip), limit((uint32_t)a.clip) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t below) const { return (uint32_t)exp2((long long)below); }
+};
+struct TcExp16 {
+    static constexpr int SHIFT = 11;
+    uint32_t limit;                                // 18 2^32 / 94548 2^11 < 2^31
+    __device__ __forceinline__ TcExp16(const PagedAttnArgs &a) : limit((uint32_t)a.clip << SHIFT) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t below) const {
+        const uint32_t u = __umulhi(below, 94548u << 5), f = u << 16, f1 = u & 0xFFFFu, f2 = __umulhi(f, f1), f3 = __umulhi(f, f2);
+        return (65536u - __umulhi(f, 45426u) + __umulhi(f2, 15743u << 16) - __umulhi(f3, 3638u << 16)) >> (u >> 16);
     }
+};
+
+// Distances of a lane's eight keys in one tile and the base they lie below; dist, base: of the lane in tile 0.
+__device__ __forceinline__ void tc_distances(const uint32_t *dist, const long long *base, int tile, uint32_t (&d)[8], unsigned long long &biased) {
+    const uint4 *from = reinterpret_cast<const uint4 *>(dist + (long long)tile * (PT_HEADS * PT_KEYS));
+    const uint4 x = __ldcg(from), y = __ldcg(from + 1);
+    d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w; d[4] = y.x; d[5] = y.y; d[6] = y.z; d[7] = y.w;
+    biased = (uint64_t)__ldcg(base + (long long)tile * 4 * PT_HEADS) ^ PT_BIAS;
+}
+// exponential of a key `d` below a base that lies `above` below the pair's largest score, both at most the limit
+template <class Exp>
+__device__ __forceinline__ uint32_t tc_weight(const Exp &exp2, uint32_t above, uint32_t d) { return exp2(min(above + d, exp2.limit)); }
+// Sum of a head's exponentials over every fourth tile from `first` to `end`, the four lanes' keys of a quarter.  A function of its own: inlined at each
+// call its code, fetched once for every use, took longer than its work.
+template <class Exp>
+__device__ __noinline__ unsigned long long tc_normalise(const PagedAttnArgs &a, const uint32_t *dist, const long long *base, int first, int end, unsigned long long top) {
+    constexpr int DEEP = 4;                        // tiles asked for at once: behind the rows that stream in a load takes microseconds
+    const Exp exp2(a);
+    unsigned long long z = 0;
+    for (int i = first; i < end; i += DEEP * PT_SETS) {
+        uint32_t d[DEEP][8];
+        unsigned long long b[DEEP];
+#pragma unroll
+        for (int u = 0; u < DEEP; u++) tc_distances(dist, base, min(i + u * PT_SETS, end - 1), d[u], b[u]);
+#pragma unroll
+        for (int u = 0; u < DEEP; u++) {
+            if (i + u * PT_SETS >= end) break;
+            const uint32_t above = (uint32_t)tc_min(top - b[u], a.clip) << Exp::SHIFT;
+            uint32_t sum = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum += tc_weight(exp2, above, d[u][e]);
+            z += sum;
+        }
+    }
+    __syncwarp();
+    z += __shfl_xor_sync(0xffffffffu, z, 1);
+    z += __shfl_xor_sync(0xffffffffu, z, 2);
+    return z;                                      // the same in the head's four lanes
 }
 
-// ---- probabilities and values --------------------------------------------------------------------------------------------------------
-template <bool SHORT, bool SMALL>                  // SHORT: fa <= 16; SMALL: beside that every sum of exponentials at most 2^31
-__global__ void __launch_bounds__(PT_THREADS, 1) paged_values_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap map, const TcShape sh) {
-    using Exp = std::conditional_t<SHORT, SoftmaxExp16, SoftmaxExp>;
+template <bool AT16, bool SMALL>                   // AT16: fa = 16; SMALL: beside that every sum of exponentials at most 2^31
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcShape sh) {
+    using Exp = std::conditional_t<AT16, TcExp16, TcExp>;
     using Quotient = std::conditional_t<SMALL, SoftmaxQuotient16, SoftmaxQuotient>;
     extern __shared__ unsigned char pt_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) TcBars s;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, groups = tc_head_groups(a), per_seq = a.Hkv * groups;
-    const int heads_most = tc_group_heads(a);
-    const uint32_t tile_bytes = (uint32_t)sh.chunks * 1024 * PT_GROUPS;
-    unsigned char *probs = smem;                   // two tiles of probability bytes [128][32], 32-byte swizzle: byte a of head h at 8 a + h
-    const uint32_t ring = tl_u32(smem) + 2 * PT_KEYS * 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), groups = tc_head_groups(a), per_seq = a.Hkv * groups;
+    const int heads_most = tc_group_heads(a), padded = (heads_most + 1) & ~1;
+    const uint32_t operand = (uint32_t)sh.chunks * padded * 1024;
+    unsigned char *lower = smem, *upper = smem + operand, *probs = smem + 2 * operand;       // query columns; four tiles of probability bytes [128][32], byte a of head h at 8 a + h
+    const uint32_t ring = tl_u32(smem) + 2 * operand + PT_SETS * PT_PROBS;
     volatile int *abort_flag = &s.abort;
-    tc_begin(s, sh.columns, PT_WORKERS / 2);
-    TcWalk w;
-    tc_share(a, s.scan, w, false);                 // (lengths, tables and pages are older than the kernel in front, which waited for what wrote them)
-    const uint32_t tmem = s.tmem, buffer = (uint32_t)sh.chunks * 64;
-    if (warp == 0) {
-        tc_produce(a, w, &map, s, ring, sh, abort_flag);
-    } else if (warp == 1) {
-        const uint32_t idesc = (2u << 4) | (1u << 15) | (1u << 16) | ((32u >> 3) << 17) | ((128u >> 4) << 24);      // both operands transposed, unsigned
-        int slot = 0, seg = 0;
-        uint32_t pass = 0;
-        for (int i = 0; w.left > 0; i++) {
-            bool ok = tl_wait(tl_u32(&s.full[slot]), pass, abort_flag);
-            if (ok) ok = tl_wait(tl_u32(&s.op_full[i & 1]), (i >> 1) & 1, abort_flag);
-            if (ok && w.seg == 0 && seg >= 2) ok = tl_wait(tl_u32(&s.acc_free[seg & 1]), ((seg >> 1) & 1) ^ 1, abort_flag);
-            if (!ok) break;
-            tc_after();
-            const bool last = w.ends_segment();
-            if (tl_elect()) {
-                const uint32_t tile = ring + slot * tile_bytes, p = tl_u32(probs) + (i & 1) * (PT_KEYS * 32);
-#pragma unroll 1
-                for (int c = 0; c < sh.chunks; c++)
-#pragma unroll
-                    for (int side = 0; side < 2; side++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tl_mma(tmem + (seg & 1) * buffer + (2 * c + side) * 32, tc_desc(tile + c * 1024 + k * 4 * sh.chunks * 1024, (uint32_t)sh.chunks * 1024, SW128),
-                                   tc_desc(p + k * 1024, 256, SW32), idesc | (side ? 1u << 7 : 0u), (w.seg | k) != 0);
-                tl_commit(tl_u32(&s.empty[slot]));
-                tl_commit(tl_u32(&s.op_free[i & 1]));
-                if (last) tl_commit(tl_u32(&s.acc_full[seg & 1]));
-            }
-            __syncwarp();
-            if (last) seg++;
-            w.next(a, per_seq);
-            if (++slot == sh.stages) { slot = 0; pass ^= 1; }
+    if (tid == 0) {
+        s.abort = 0;
+        for (int i = 0; i < sh.slots; i++) { tl_init(tl_u32(&s.full[i]), 1); tl_init(tl_u32(&s.empty[i]), 1); }
+        for (int i = 0; i < PT_META; i++) tl_init(tl_u32(&s.meta[i]), 1);
+        for (int i = 0; i < 2; i++) {
+            tl_init(tl_u32(&s.score_free[i]), 4);
+            tl_init(tl_u32(&s.out_full[i]), 1); tl_init(tl_u32(&s.out_free[i]), PT_WORKERS);
         }
-        tc_drain(s);
-    } else {
-        pdl_enter();
-        const TcWork work = tc_work(a);
-        const int worker = tid - 64, set = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane;
+        for (int i = 0; i < PT_SETS; i++) { tl_init(tl_u32(&s.score_full[i]), 1); tl_init(tl_u32(&s.prob_full[i]), 4); tl_init(tl_u32(&s.prob_free[i]), 1); }
+        tl_init(tl_u32(&s.query_full), PT_WORKERS); tl_init(tl_u32(&s.pair_done), PT_WORKERS); tl_init(tl_u32(&s.drain), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tl_u32(&s.tmem)), "r"(sh.columns));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    const uint32_t total = tc_share(a, s.scan, s.run);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem, 0), score_at = tmem + sh.score_at, buffer = (uint32_t)sh.chunks * 64;
+    if (warp < 2) {
+        if (tc_box(a) == 16) tc_producer<2>(a, &kmap, &vmap, s, ring, sh, warp, abort_flag);
+        else tc_producer<1>(a, &kmap, &vmap, s, ring, sh, warp, abort_flag);
+    } else if (warp == 2) {
+        if (tl_elect()) {                          // one thread
+            constexpr uint32_t up = tc_desc_upper(1024, SW128), pp = tc_desc_upper(256, SW32);
+            constexpr uint32_t plain = (2u << 4) | (1u << 15) | (1u << 16) | ((32u >> 3) << 17) | ((128u >> 4) << 24), last_byte = plain | (1u << 7);      // both operands transposed; unsigned, values signed
+            const uint32_t lower_i = tl_idesc(8 * padded, false), upper_i = tl_idesc(8 * padded, true);
+            TcRing at;
+            bool ok = true, fresh = true;
+            int queries = 0, i = 0;
+            for (int u = 0; u < RUNS; u++) {       // scores
+            TcWalk v = s.run[u];
+            for (fresh = true; ok && v.left > 0; i++) {
+                if (i >= 2) ok = tc_wait(tl_u32(&s.score_free[i & 1]), ((i >> 1) & 1) ^ 1, abort_flag);
+                if (ok && fresh) { ok = tc_wait(tl_u32(&s.query_full), queries & 1, abort_flag); queries++; }
+                const uint32_t d = score_at + (i & 1) * 64;
+                uint32_t q = tc_desc(tl_u32(smem));
+                for (int c = 0; ok && c < sh.chunks; c++, q += (uint32_t)padded * 64) {
+                    ok = tc_wait(tl_u32(&s.full[at.slot]), at.pass, abort_flag);
+                    if (!ok) break;
+                    tc_after();
+                    const uint32_t keys = tc_desc(ring + at.slot * PT_SLOT), q3 = q + (operand >> 4);
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {       // 32 bytes of the rows
+                        tc_mma<up, up>(d, keys + k, q + k, lower_i, (c | k) != 0);
+                        tc_mma<up, up>(d, keys + k, q3 + k, upper_i, 1);
+                    }
+                    tl_commit(tl_u32(&s.empty[at.slot]));
+                    at.step(sh.slots);
+                }
+                if (ok) tl_commit(tl_u32(&s.score_full[i % PT_SETS]));
+                fresh = v.t + 1 == v.nt;
+                v.next(a, per_seq);
+            }
+            }
+            for (int k = max(0, i - 2); ok && k < i; k++) ok = tc_wait(tl_u32(&s.score_free[k & 1]), (k >> 1) & 1, abort_flag);      // (outputs take the scores' columns)
+            int seg = 0;
+            i = 0;
+            for (int u = 0; u < RUNS; u++) {       // values
+            TcWalk v = s.run[tc_value_run(u)];
+            for (; ok && v.left > 0; i++) {
+                ok = tc_wait(tl_u32(&s.prob_full[i % PT_SETS]), (i / PT_SETS) & 1, abort_flag);
+                if (ok && v.seg == 0 && seg >= 2) ok = tc_wait(tl_u32(&s.out_free[seg & 1]), ((seg >> 1) & 1) ^ 1, abort_flag);
+                const uint32_t p = tc_desc(tl_u32(probs) + (i % PT_SETS) * PT_PROBS);
+                uint32_t d = tmem + (seg & 1) * buffer;
+                for (int c = 0; ok && c < sh.chunks; c++, d += 64) {
+                    ok = tc_wait(tl_u32(&s.full[at.slot]), at.pass, abort_flag);
+                    if (!ok) break;
+                    tc_after();
+                    const uint32_t values = tc_desc(ring + at.slot * PT_SLOT);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {          // 32 keys
+                        tc_mma<up, pp>(d, values + 256 * k, p + 64 * k, plain, (v.seg | k) != 0);
+                        tc_mma<up, pp>(d + 32, values + 256 * k, p + 64 * k, last_byte, (v.seg | k) != 0);
+                    }
+                    tl_commit(tl_u32(&s.empty[at.slot]));
+                    at.step(sh.slots);
+                }
+                const bool last = v.ends_segment();
+                if (ok) {
+                    tl_commit(tl_u32(&s.prob_free[i % PT_SETS]));
+                    if (last) tl_commit(tl_u32(&s.out_full[seg & 1]));
+                }
+                if (last) seg++;
+                v.next(a, per_seq);
+            }
+            }
+            if (*abort_flag) {                     // products under way end before their TMEM is given back
+                tl_commit(tl_u32(&s.drain));
+                volatile int patient = 0;
+                tc_wait(tl_u32(&s.drain), 0, &patient);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= PT_FIRST) {
+        const int worker = tid - 32 * PT_FIRST, set = (warp - PT_FIRST) >> 2, quarter = warp & 3, key = quarter * 32 + lane;      // a warp reads TMEM lanes 32 (warp % 4) ..
+        const int g = lane >> 2, t = lane & 3;     // beyond the scores a lane has head g, keys t, t + 4, .. of the quarter
+        const TcWork work = tc_work(a, gridDim.x);
+        const Exp exp2(a);
+        bool ok = true;
+        // sum of the exponentials of head g over those of n tiles from `first` on that this warp has read out: the first of them is `skip` on
+        auto normalise = [&](int first, int n, int skip, unsigned long long top) {
+            return tc_normalise<Exp>(a, work.dist + g * PT_KEYS + quarter * 32 + 8 * t, work.base + quarter * PT_HEADS + g, first + skip, g < heads_most ? first + n : first, top);
+        };
+        // what is left to do with the maxima of a pair (or of its part here) once the next pair's query columns are written, so that the
+        // products go on meanwhile: exchange them; a whole pair's normaliser
+        struct { int n = 0, nt, first, index; long long pair; } behind;    // tiles, the pair's; number of the first in the list, and among this CTA's scores
+        long long largest = INT64_MIN;             // lane h: of head h, over this warp's tiles of the pair
+        int whole_pairs = 0;
+        auto settle = [&](long long most) {
+            if (behind.n == 0) return true;
+            const unsigned long long biased = (uint64_t)most ^ PT_BIAS;
+            if (behind.n == behind.nt) {
+                unsigned long long *const top = work.top + behind.pair * PT_WORKERS * PT_HEADS, *const z = work.z + behind.pair * PT_WORKERS * PT_HEADS + 4 * set * PT_HEADS + quarter * PT_HEADS;
+                if (lane < PT_HEADS) top[(4 * set + quarter) * PT_HEADS + lane] = biased;
+                __syncwarp();
+                if (lane == 0) tl_arrive(tl_u32(&s.pair_done));
+                __syncwarp();
+                if (!tl_wait(tl_u32(&s.pair_done), whole_pairs & 1, abort_flag)) return false;
+                whole_pairs++;
+                unsigned long long m = 0;          // over the warps: four for each of a head's lanes
+#pragma unroll
+                for (int w = 0; w < 4; w++) m = max(m, __ldcg(top + (4 * t + w) * PT_HEADS + g));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const unsigned long long sum = normalise(behind.first, behind.n, (set - behind.index) & 3, m);
+                if (t == 0) z[g] = sum;
+            } else {
+                TcCell *cell = work.cell + tc_owner(behind.first, total);
+                if (lane < heads_most) atomicMax(cell->top + lane, biased);
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) atomicAdd(&cell->tops, (unsigned)behind.n);
+            }
+            behind.n = 0;
+            return true;
+        };
+        // Pairs that go on in other CTAs: their normalisers as soon as every CTA's maxima are in, looked for between tiles.
+        bool due[RUN_WHOLE] = {s.run[0].left > 0, s.run[1].left > 0};
+        auto complete = [&](const unsigned *count, int nt) {
+            unsigned v;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
+            return __all_sync(0xffffffffu, v == (unsigned)nt * PT_WORKERS) != 0;
+        };
+        auto normalise_cut = [&](int x) {          // false: not yet
+            if (!due[x]) return true;
+            const int first = s.run[x].tile, n = s.run[x].left, nt = s.run[x].nt;
+            TcCell *cell = work.cell + tc_owner(first - s.run[x].t, total);
+            if (!complete(&cell->tops, nt)) return false;
+            const unsigned long long z = normalise(first, n, (set - (x == 0 ? 0 : s.run[0].left)) & 3, __ldcg(cell->top + g));
+            if (t == 0 && g < heads_most) atomicAdd(cell->z + g, z);
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) atomicAdd(&cell->zs, (unsigned)n);
+            due[x] = false;
+            return true;
+        };
+        for (int x = worker; x < (int)(PT_SETS * PT_PROBS / 16); x += 32 * PT_WORKERS) reinterpret_cast<uint4 *>(probs)[x] = make_uint4(0, 0, 0, 0);      // (the columns beyond 24 stay so)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         for (int b = blockIdx.x; b < a.B; b += gridDim.x) {                // sequences without keys
             PagedSpan none;
             paged_span(a, b, none);
             if (tc_tiles(a, none) == 0)
-                for (long long i = worker; i < (long long)a.H * a.hd; i += 32 * PT_WORKERS) a.out[(long long)b * a.H * a.hd + i] = 0;
+                for (long long x = worker; x < (long long)a.H * a.hd; x += 32 * PT_WORKERS) a.out[(long long)b * a.H * a.hd + x] = 0;
         }
-        const Exp exp2(a.fa, a.log2e, a.clip);
-        Quotient quotient[PT_HEADS] = {Quotient(0, a.fa), Quotient(0, a.fa), Quotient(0, a.fa), Quotient(0, a.fa), Quotient(0, a.fa), Quotient(0, a.fa), Quotient(0, a.fa), Quotient(0, a.fa)};
-        long long top = 0;                         // of head lane & 7
+        // ---- scores ------------------------------------------------------------------------------------------------------------------
+        int i = 0;
+        for (int u = 0; u < RUNS; u++) {
+            TcWalk v = s.run[u];
+            for (bool fresh = true; ok && v.left > 0; i++) {
+                if (fresh) {                       // the columns are free once the tile in front has been multiplied (every set has waited for one of the last four tiles: no phase is mistaken)
+                    if (i > 0 && !tl_wait(tl_u32(&s.score_full[(i - 1) % PT_SETS]), ((i - 1) / PT_SETS) & 1, abort_flag)) { ok = false; break; }
+                    const long long most = largest;
+                    largest = INT64_MIN;
+                    tc_queries(a, v, min(heads_most, a.H / a.Hkv - v.pair_of % groups * heads_most), padded, lower, upper, worker);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tl_arrive(tl_u32(&s.query_full));
+                    if (!settle(most)) { ok = false; break; }
+                }
+                if (i % PT_SETS == set) {
+                    if (!tl_wait(tl_u32(&s.meta[i % PT_META]), (uint32_t)(i / PT_META) & 1, abort_flag)) { ok = false; break; }
+                    const bool seen = (s.mask[i % PT_META][key >> 3] >> (key & 7)) & 1, any = __any_sync(0xffffffffu, seen);
+                    if (!tl_wait(tl_u32(&s.score_full[set]), (i / PT_SETS) & 1, abort_flag)) { ok = false; break; }
+                    tc_after();
+                    const uint32_t from = score_at + ((uint32_t)(quarter * 32) << 16) + (i & 1) * 64;
+                    uint32_t *to = work.dist + (long long)v.tile * PT_HEADS * PT_KEYS + quarter * 32 + (lane & 3) * 8 + (lane >> 2);
+                    long long base = INT64_MIN;
+#pragma unroll 2
+                    for (int h = 0; h < heads_most; h++) {
+                        int c[8];
+                        tc_ld8(from + 8 * h, c);
+                        tc_ld_wait();
+                        const uint64_t low = (uint64_t)((long long)c[0] + (long long)c[1] * 256 + (long long)c[2] * 65536 + (long long)c[3] * 16777216);
+                        const uint32_t high = (uint32_t)c[4] + ((uint32_t)c[5] << 8) + ((uint32_t)c[6] << 16) + ((uint32_t)c[7] << 24);
+                        const long long dot = (long long)(low + ((uint64_t)high << 32));
+                        const long long score = (long long)((uint64_t)(dot >> a.fa) * (uint64_t)a.inv_sqrt) >> a.fa;
+                        // the largest of the warp's 32 keys: by the upper words, then by the lower ones where those are equal
+                        const int up = seen ? (int)(score >> 32) : INT32_MIN;
+                        const int up_most = __reduce_max_sync(0xffffffffu, up);
+                        const uint32_t low_most = __reduce_max_sync(0xffffffffu, seen && up == up_most ? (uint32_t)score : 0u);
+                        const long long most = any ? (long long)(((uint64_t)(uint32_t)up_most << 32) | low_most) : INT64_MIN;
+                        to[h * PT_KEYS] = seen ? (uint32_t)tc_min((uint64_t)most - (uint64_t)score, a.clip) << Exp::SHIFT : exp2.limit;
+                        if (lane == h) base = most;
+                    }
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) tl_arrive(tl_u32(&s.score_free[i & 1]));
+                    if (lane < PT_HEADS) work.base[((long long)v.tile * 4 + quarter) * PT_HEADS + lane] = base;
+                    largest = max(largest, base);
+#pragma unroll 1
+                    for (int x = 0; x < u; x++) normalise_cut(x);
+                }
+                if (v.ends_part()) {
+                    behind.n = v.part + 1; behind.nt = v.nt; behind.first = v.tile - v.t; behind.index = i - v.part;
+                    behind.pair = (long long)v.b * per_seq + v.pair_of;
+                }
+                fresh = v.t + 1 == v.nt;
+                v.next(a, per_seq);
+            }
+        }
+        __syncwarp();
+        ok = ok && settle(largest);
+        // ---- probabilities and values ---------------------------------------------------------------------------------------------
+        if (ok) {                                  // what the CTA's warps left in memory
+            if (lane == 0) tl_arrive(tl_u32(&s.pair_done));
+            __syncwarp();
+            ok = tl_wait(tl_u32(&s.pair_done), whole_pairs & 1, abort_flag);
+        }
+        Quotient quotient(0, a.fa);                // of head g
+        unsigned long long top = 0, carry[2] = {0, 0};                     // of head g; output sums of earlier accumulations
         int seg = 0;
-        bool fresh = true;
-        for (int i = 0; w.left > 0; i++) {
-            const long long pair = (long long)w.b * per_seq + w.pair_of;
-            if (fresh) {
-                top = work.top[pair * PT_HEADS + (lane & 7)];
-                const Quotient mine((lane & 7) < heads_most ? work.z[pair * PT_HEADS + (lane & 7)] : 0, a.fa);
+        struct { int tiles = 0, nt, first, heads; bool ends; int64_t *out; } pending;      // sums to read out: tiles of the pair in them (and in `carry`)
+        auto read_out = [&]() {
+            if (!tl_wait(tl_u32(&s.out_full[seg & 1]), (seg >> 1) & 1, abort_flag)) return false;
+            tc_after();
+            const int byte = lane & 3, d = 32 * set + 8 * quarter + (lane >> 2), h0 = 4 * (byte >> 1) + 2 * (byte & 1);
+            const bool whole = pending.tiles == pending.nt, joins = pending.ends && !whole;
+            const int owner = joins ? tc_owner(pending.first, total) : 0;
+            unsigned long long *acc = work.acc + (long long)owner * PT_HEADS * a.hd;
+            if (set < sh.chunks) {                 // dimensions 32 set ..
+                const uint32_t from = tmem + (seg & 1) * buffer + ((uint32_t)(quarter * 32) << 16) + 2 * set * 32;
+                uint64_t sum[PT_HEADS];
 #pragma unroll
-                for (int h = 0; h < PT_HEADS; h++) {
-                    quotient[h] = mine;
-                    if constexpr (SMALL) quotient[h].m = __shfl_sync(0xffffffffu, mine.m, h);
-                    else { quotient[h].mh = __shfl_sync(0xffffffffu, mine.mh, h); quotient[h].ml = __shfl_sync(0xffffffffu, mine.ml, h); }
-                    quotient[h].post = __shfl_sync(0xffffffffu, mine.post, h);
+                for (int h = 0; h < PT_HEADS; h++) sum[h] = 0;
+#pragma unroll
+                for (int part = 0; part < 3; part++) {
+                    int x[8], y[8];
+                    tc_ld8(from + 8 * part, x); tc_ld8(from + 32 + 8 * part, y);
+                    tc_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < PT_HEADS; h++) sum[h] += (uint64_t)(int64_t)(byte == 3 ? y[h] : x[h]) << (8 * part);
+                }
+                // four lanes hold a dimension's four bytes: two exchanges leave a lane with two heads
+                const bool high = byte & 2, odd = byte & 1;
+#pragma unroll
+                for (int h = 0; h < PT_HEADS; h++) sum[h] <<= 8 * byte;
+#pragma unroll
+                for (int h = 0; h < 4; h++) {
+                    const uint64_t give = high ? sum[h] : sum[h + 4];
+                    sum[h] = (high ? sum[h + 4] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 2);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint64_t give = odd ? sum[h] : sum[h + 2];
+                    carry[h] += (odd ? sum[h + 2] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 1);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (!pending.ends || h0 + h >= pending.heads) continue;
+                    if (whole) pending.out[(long long)(h0 + h) * a.hd + d] = (int64_t)carry[h] >> a.fa;
+                    else atomicAdd(acc + (h0 + h) * a.hd + d, carry[h]);
                 }
             }
-            if ((i & 1) == set) {
-                const uint4 *d4 = reinterpret_cast<const uint4 *>(work.dist + ((long long)w.tile * PT_KEYS + key) * PT_HEADS);
-                const uint4 da = d4[0], db = heads_most > 4 ? d4[1] : make_uint4(0, 0, 0, 0);
-                const uint32_t d[PT_HEADS] = {da.x, da.y, da.z, da.w, db.x, db.y, db.z, db.w};
-                const long long base = work.base[((long long)w.tile * 4 + quarter) * PT_HEADS + (lane & 7)];
-                const uint32_t above = (uint32_t)min((uint64_t)top - (uint64_t)base, (uint64_t)a.clip);
-                uint32_t p[PT_HEADS];
-#pragma unroll
-                for (int h = 0; h < PT_HEADS; h++) {
-                    const uint64_t below = (uint64_t)__shfl_sync(0xffffffffu, above, h) + d[h];
-                    const uint32_t e = h < heads_most && d[h] != 0xFFFFFFFFu ? (uint32_t)exp2((uint32_t)min(below, (uint64_t)a.clip)) : 0u;
-                    p[h] = quotient[h](e);
+            tc_before();
+            __syncwarp();
+            if (lane == 0) tl_arrive(tl_u32(&s.out_free[seg & 1]));
+            if (pending.ends) carry[0] = carry[1] = 0;
+            if (joins && set < sh.chunks) {        // the last of the CTAs writes out what this warp and its likes have added up
+                __threadfence();
+                __syncwarp();
+                unsigned before = 0;
+                if (lane == 0) before = atomicAdd(&work.cell[owner].done[4 * set + quarter], (unsigned)pending.tiles);
+                before = __shfl_sync(0xffffffffu, before, 0);
+                if (before + pending.tiles == (unsigned)pending.nt) {
+                    __threadfence();
+                    for (int h = h0; h < min(h0 + 2, pending.heads); h++) pending.out[(long long)h * a.hd + d] = (int64_t)__ldcg(acc + h * a.hd + d) >> a.fa;
                 }
-                if (i >= 2 && !tl_wait(tl_u32(&s.op_free[set]), ((i >> 1) & 1) ^ 1, abort_flag)) break;
-                uint32_t out[8];                                           // bytes 8 a + h
+            }
+            pending.tiles = 0;
+            seg++;
+            return true;
+        };
+        i = 0;
+        for (int u = 0; u < RUNS; u++) {
+        const int run = tc_value_run(u);
+        TcWalk v = s.run[run];
+        for (bool fresh = true; ok && v.left > 0; i++) {
+            if (fresh) {
+                unsigned long long z = 0;
+                top = 0;
+                if (v.t == 0 && v.rest() == v.nt) {
+                    const long long at = ((long long)v.b * per_seq + v.pair_of) * PT_WORKERS * PT_HEADS + g;
 #pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    const uint32_t x = p[4 * q], y = p[4 * q + 1], z = p[4 * q + 2], v = p[4 * q + 3];
-                    const uint32_t t0 = __byte_perm(x, y, 0x5140), t1 = __byte_perm(x, y, 0x7362), t2 = __byte_perm(z, v, 0x5140), t3 = __byte_perm(z, v, 0x7362);
-                    out[q] = __byte_perm(t0, t2, 0x5410); out[2 + q] = __byte_perm(t0, t2, 0x7632); out[4 + q] = __byte_perm(t1, t3, 0x5410);
+                    for (int w = 0; w < 4; w++) { top = max(top, __ldcg(work.top + at + (4 * t + w) * PT_HEADS)); z += __ldcg(work.z + at + (4 * t + w) * PT_HEADS); }
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1)); z += __shfl_xor_sync(0xffffffffu, z, 1);
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2)); z += __shfl_xor_sync(0xffffffffu, z, 2);
+                } else {
+                    TcCell *cell = work.cell + tc_owner(v.tile - v.t, total);
+                    // everybody's share of the normaliser; meanwhile what others wait for
+                    bool there = false;
+                    for (unsigned polls = 0; polls < PT_POLLS && !there && !*abort_flag; polls++) {
+                        const bool mine = normalise_cut(0) & normalise_cut(1);
+                        there = complete(&cell->zs, v.nt) && (mine || !due[run]);
+                    }
+                    if (!__all_sync(0xffffffffu, there)) { *abort_flag = 1; ok = false; break; }
+                    top = __ldcg(cell->top + g); z = __ldcg(cell->z + g);
                 }
-                unsigned char *to = probs + set * (PT_KEYS * 32) + key * 32;
-                const int flip = ((key >> 2) & 1) * 16;
-                *reinterpret_cast<uint4 *>(to + flip) = make_uint4(out[0], out[1], out[2], out[3]);
-                *reinterpret_cast<uint4 *>(to + (16 ^ flip)) = make_uint4(out[4], out[5], 0, 0);
+                quotient = Quotient(g < heads_most ? z : 0, a.fa);
+            }
+            if (i % PT_SETS == set) {
+                uint32_t p[8];
+                unsigned long long base;
+                tc_distances(work.dist + g * PT_KEYS + quarter * 32 + 8 * t, work.base + quarter * PT_HEADS + g, v.tile, p, base);
+                const uint32_t above = (uint32_t)tc_min(top - base, a.clip) << Exp::SHIFT;
+#pragma unroll
+                for (int e = 0; e < 8; e++) p[e] = g < heads_most ? (uint32_t)quotient(tc_weight(exp2, above, p[e])) : 0u;
+                if (i >= PT_SETS && !tl_wait(tl_u32(&s.prob_free[set]), ((i / PT_SETS) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                unsigned char *to = probs + set * PT_PROBS + (quarter * 32 + t) * 32 + g;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {      // key t + 4 e: byte b at 8 b + g, the halves of 32 bytes swapped in every second group of four rows
+                    to[128 * e + (e & 1) * 16] = (unsigned char)p[e];
+                    to[128 * e + 8 + (e & 1) * 16] = (unsigned char)(p[e] >> 8);
+                    to[128 * e + 16 - (e & 1) * 16] = (unsigned char)(p[e] >> 16);
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) tl_arrive(tl_u32(&s.op_full[set]));
+                if (lane == 0) tl_arrive(tl_u32(&s.prob_full[set]));
             }
-            if (w.ends_segment()) {
-                if (!tl_wait(tl_u32(&s.acc_full[seg & 1]), (seg >> 1) & 1, abort_flag)) break;
-                tc_after();
-                const bool whole = w.seg + 1 == w.nt;                      // the pair's only segment
-                const int g = w.pair_of % groups, kv = w.pair_of / groups, heads = min(heads_most, a.H / a.Hkv - g * heads_most), byte = lane & 3;
-                int64_t *out = a.out + ((long long)w.b * a.H + kv * (a.H / a.Hkv) + g * heads_most) * a.hd;
-                unsigned long long *acc = work.acc + pair * PT_HEADS * a.hd;
-                for (int c = set; c < sh.chunks; c += 2) {
-                    const uint32_t from = tmem + (seg & 1) * buffer + ((uint32_t)(quarter * 32) << 16) + 2 * c * 32;
-                    uint64_t sum[PT_HEADS];
-#pragma unroll
-                    for (int h = 0; h < PT_HEADS; h++) sum[h] = 0;
-#pragma unroll
-                    for (int part = 0; part < 3; part++) {
-                        int u[8], v[8];
-                        tc_ld(from + 8 * part, u); tc_ld(from + 32 + 8 * part, v);
-                        tc_ld_wait();
-#pragma unroll
-                        for (int h = 0; h < PT_HEADS; h++) sum[h] += (uint64_t)(int64_t)(byte == 3 ? v[h] : u[h]) << (8 * part);
-                    }
-                    // four lanes hold a dimension's four bytes: two exchanges leave lane `byte` with heads 2 byte', 2 byte' + 1
-#pragma unroll
-                    for (int h = 0; h < PT_HEADS; h++) sum[h] <<= 8 * byte;
-                    const bool upper = byte & 2, odd = byte & 1;
-#pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        const uint64_t give = upper ? sum[h] : sum[h + 4];
-                        sum[h] = (upper ? sum[h + 4] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 2);
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint64_t give = odd ? sum[h] : sum[h + 2];
-                        sum[h] = (odd ? sum[h + 2] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 1);
-                    }
-                    const int d = 32 * c + 8 * quarter + (lane >> 2), h0 = 4 * (byte >> 1) + 2 * (byte & 1);
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        if (h0 + h < heads) {
-                            if (whole) out[(long long)(h0 + h) * a.hd + d] = (int64_t)sum[h] >> a.fa;
-                            else atomicAdd(acc + (h0 + h) * a.hd + d, (unsigned long long)sum[h]);
-                        }
-                }
-                tc_before();
-                __syncwarp();
-                if (lane == 0) tl_arrive(tl_u32(&s.acc_free[seg & 1]));
-                if (!whole) {                      // the warp that adds the pair's last sums writes it out
-                    __threadfence();
-                    __syncwarp();
-                    const unsigned n = (unsigned)w.seg + 1;
-                    unsigned before = 0;
-                    if (lane == 0) before = atomicAdd(work.done + pair, n);
-                    before = __shfl_sync(0xffffffffu, before, 0);
-                    if (before + n == (unsigned)w.nt * PT_WORKERS) {
-                        __threadfence();
-                        for (int at = lane; at < heads * a.hd; at += 32) out[at] = (int64_t)__ldcg(acc + at) >> a.fa;
-                    }
-                }
-                seg++;
+            if (i % PT_SETS == set) { normalise_cut(0); normalise_cut(1); }
+            // (sums are read out behind the next tile's probabilities, so that the products go on meanwhile)
+            if (pending.tiles && (i % PT_SETS == set) && !read_out()) { ok = false; break; }
+            if (v.ends_segment()) {
+                if (pending.tiles && !read_out()) { ok = false; break; }
+                const int group = v.pair_of % groups, kv = v.pair_of / groups;
+                pending.tiles = v.part + 1; pending.nt = v.nt; pending.ends = v.ends_part(); pending.first = v.tile - v.t;
+                pending.heads = min(heads_most, a.H / a.Hkv - group * heads_most);
+                pending.out = a.out + ((long long)v.b * a.H + kv * (a.H / a.Hkv) + group * heads_most) * a.hd;
             }
-            fresh = w.t + 1 == w.nt;
-            w.next(a, per_seq);
+            fresh = v.t + 1 == v.nt;
+            v.next(a, per_seq);
         }
+        }
+        if (ok && pending.tiles) read_out();
     }
-    tc_end(s, sh.columns, a.flags);
+    tc_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(sh.columns));
+    }
+    if (tid == 0 && s.abort) atomicOr(a.flags, FLAG_GAVE_UP);
 }
 
 bool tc_map(CUtensorMap *map, const int32_t *pool, const PagedAttnArgs &a) {
-    const cuuint64_t dims[3] = {32, (cuuint64_t)a.n_pages * a.Hkv * a.P, (cuuint64_t)a.hd / 32}, strides[2] = {(cuuint64_t)a.hd * 4, 128};
-    const cuuint32_t box[3] = {32, 8, (cuuint32_t)a.hd / 32}, step[3] = {1, 1, 1};
-    return tl_encode()(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, const_cast<int32_t *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    const cuuint64_t dims[2] = {(cuuint64_t)a.hd, (cuuint64_t)a.n_pages * a.Hkv * a.P}, strides[1] = {(cuuint64_t)a.hd * 4};
+    const cuuint32_t box[2] = {32, (cuuint32_t)tc_box(a)}, step[2] = {1, 1};
+    return tl_encode()(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<int32_t *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename K>
-cudaError_t tc_configure(K kernel, size_t smem) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+// SMs of the current device: CTAs of a launch at most (one is resident on each, as a cooperative launch needs)
+int tc_sms() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); return 0; }
+    return n;
 }
+constexpr int PT_MOST_CTAS = 256;                  // cells in the scratch
 
-template <bool SHORT, bool SMALL>
+template <bool AT16, bool SMALL>
 cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     CUtensorMap kmap, vmap;
     if (!tl_encode() || !tc_map(&kmap, a.kpages, a) || !tc_map(&vmap, a.vpages, a)) return cudaErrorInvalidValue;
-    constexpr size_t room = 226 * 1024 - 2048;     // beside the static part
-    const int chunks = a.hd / 32, padded = (tc_group_heads(a) + 1) & ~1;
-    const size_t tile = (size_t)chunks * 1024 * PT_GROUPS, queries = 2 * (size_t)chunks * padded * 1024, probs = 2 * PT_KEYS * 32;
-    const TcShape ks = {chunks, (int)std::min<size_t>(PT_MAX_STAGES, (room - 1024 - queries) / tile), 128};
-    const TcShape vs = {chunks, (int)std::min<size_t>(PT_MAX_STAGES, (room - 1024 - probs) / tile), chunks == 1 ? 128 : chunks == 2 ? 256 : 512};
-    const size_t ksm = 1024 + queries + ks.stages * tile, vsm = 1024 + probs + vs.stages * tile;
-    cudaError_t e = tc_configure(paged_scores_kernel, ksm);
-    if (e == cudaSuccess) e = tc_configure(paged_values_kernel<SHORT, SMALL>, vsm);
+    const int chunks = a.hd / 32, padded = (tc_group_heads(a) + 1) & ~1, sms = tc_sms();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    const size_t fixed = 1024 + 2 * (size_t)chunks * padded * 1024 + PT_SETS * PT_PROBS, room = 227 * 1024 - sizeof(TcBars) - 64;
+    const int slots = (int)std::min<size_t>(PT_MAX_SLOTS, (room - fixed) / PT_SLOT);
+    // outputs: two buffers of 64 columns a chunk; scores: two of 64, behind them or, at four chunks, over the end of the second
+    const TcShape sh = {chunks, slots, chunks == 1 ? 256 : 512, chunks == 4 ? 384 : 128 * chunks};
+    const size_t smem = fixed + (size_t)slots * PT_SLOT;
+    cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<AT16, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_clear_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);      // else the attention waits for idle SMs
     if (e != cudaSuccess) return e;
     const long long most = (long long)a.B * a.Hkv * tc_head_groups(a) * tc_tiles_most(a);
-    const unsigned ctas = (unsigned)std::min<long long>(148, std::max<long long>(1, most));
-    e = launch_behind(paged_scores_kernel, ctas, PT_THREADS, ksm, s, a, kmap, ks);
-    if (e == cudaSuccess) e = launch_behind(paged_norm_kernel<SHORT>, (unsigned)std::min<long long>(296, std::max<long long>(1, most)), PN_THREADS, 0, s, a);
-    if (e == cudaSuccess) e = launch_behind(paged_values_kernel<SHORT, SMALL>, ctas, PT_THREADS, vsm, s, a, vmap, vs);
-    note_launch(3);
+    const unsigned ctas = (unsigned)std::min<long long>(std::min(sms, PT_MOST_CTAS), std::max<long long>(1, most));
+    const TcWork w = tc_work(a, (int)ctas);
+    e = launch_behind(paged_clear_kernel, ctas, 128, 0, s, w.cell, w.acc, PT_HEADS * a.hd);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(PT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeCooperative; attr[0].val.cooperative = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<AT16, SMALL>, a, kmap, vmap, sh);
+    note_launch(2);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace
 
-// Rows that are whole 128-byte chunks (up to four), pages of whole groups of eight rows, probabilities of three bytes.
+// Rows that are whole 128-byte chunks (up to four), pages of whole groups of eight rows, probabilities of three bytes, a list whose place times the
+// CTAs fits 32 bits.
 bool paged_tc_ok(const PagedAttnArgs &a) {
-    return a.hd % 32 == 0 && a.hd <= 128 && a.P % 8 == 0 && a.fa <= 23;
+    return a.hd % 32 == 0 && a.hd <= 128 && a.P % 8 == 0 && a.fa <= 23 && tc_tiles_most(a) * a.Hkv * tc_head_groups(a) <= 1 << 23;
 }
 size_t paged_tc_bytes(const PagedAttnArgs &a) {
     size_t n;
-    tc_work(a, &n);
+    tc_work(a, PT_MOST_CTAS, &n);
     return n;
 }
 cudaError_t launch_paged_tc(const PagedAttnArgs &a, cudaStream_t s) {
-    if (a.fa > 16) return launch_tc<false, false>(a, s);
-    return a.max_slots <= 1LL << (31 - a.fa) ? launch_tc<true, true>(a, s) : launch_tc<true, false>(a, s);
+    if (a.fa != 16) return launch_tc<false, false>(a, s);
+    return a.max_slots <= 1LL << 15 ? launch_tc<true, true>(a, s) : launch_tc<true, false>(a, s);
 }
 
 }  // namespace iie

@@ -6,8 +6,8 @@ from oracle import qk_oracle as o
 
 def rows_of(pool, table_row, kv, positions):
     """[n, hd] int64 rows of one KV head at the given positions of a sequence."""
-    P = pool.shape[2]
-    return np.array([pool[table_row[t // P], kv, t % P] for t in positions], np.int64).reshape(len(positions), pool.shape[3])
+    P, at = pool.shape[2], np.asarray(positions, np.int64)
+    return pool[np.asarray(table_row)[at // P], kv, at % P].astype(np.int64)
 
 
 def turn(x, cos, sin, pos, rope, fa):

@@ -84,6 +84,25 @@ def test_attention(shape):
     assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize(("B", "most", "H", "Hkv", "hd", "P", "window", "seed"), [
+    (40, 4500, 4, 4, 64, 16, 0, 1), (12, 9000, 8, 4, 32, 8, 0, 2), (300, 300, 8, 8, 32, 16, 0, 3), (3, 40000, 4, 2, 64, 64, 0, 4), (1, 70000, 2, 1, 32, 128, 0, 5),
+    (60, 6000, 8, 2, 128, 32, 1500, 6), (700, 150, 2, 2, 64, 8, 0, 7), (25, 3000, 12, 4, 96, 16, 0, 8)])
+def test_long_lists(B, most, H, Hkv, hd, P, window, seed):
+    """Enough tiles that every CTA has many: pairs within a CTA, cut between two and more, sequences without keys among them."""
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(seed)
+    lengths = [most] + [int(n) for n in rng.integers(1, most + 1, size=B - 1)]
+    if B > 4:
+        lengths[B // 2] = lengths[1] = 0
+    kp, vp, table = pool(rng, lengths, P, Hkv, hd, 18)
+    q = rng.integers(-(1 << 17), 1 << 17, size=(B, H * hd), dtype=np.int64)
+    cos, sin = tables(most, hd, 16)
+    device.read_flags()
+    got = attend(q, kp, vp, table, lengths, window=window, cos=cos, sin=sin, rope=1)
+    assert device.read_flags() == 0
+    assert np.array_equal(got, po.attention(q, kp, vp, table, lengths, 16, window, cos, sin, 1))
+
+
 @pytest.mark.parametrize(("P", "hd", "H", "Hkv", "window"), [(16, 128, 8, 2, 0), (16, 64, 4, 4, 0), (32, 128, 8, 1, 100), (8, 128, 6, 2, 0), (64, 64, 12, 2, 300), (5, 64, 4, 2, 0), (128, 128, 8, 2, 0)])
 def test_attention_over_chosen_pages(P, hd, H, Hkv, window):
     """Lists with empty entries in front, between and behind, of a page twice, of pages beyond the keys and out of the window, of nothing."""
