@@ -2,11 +2,16 @@
 // sequence in its general form (any head dimension, page size and number of query heads).  Arithmetic of the attention: attn.cu.
 //
 // The general form keeps scores and exponentials in memory and takes five launches: it carries the shapes that have no other.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
+#include "tile_ops.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace iie {
 
@@ -320,76 +325,250 @@ __global__ void __launch_bounds__(256) paged_rank_kernel(const PagedSelectArgs a
     if (bad && lane == 0) atomicOr(a.flags, 16);
 }
 
-// The n_sel best pages of one (sequence, KV head): radix selection of the n_sel-th largest 64-bit score, then the pages above it and the first
-// ones equal to it, in order.
-constexpr int PS_THREADS = 1024;
-__global__ void __launch_bounds__(PS_THREADS) paged_pick_kernel(const PagedSelectArgs a) {
-    pdl_enter();
-    __shared__ int s_hist[256], s_scan[2][32], s_digit, s_left;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = blockIdx.x, b = blockIdx.y;
-    int *out = a.out + ((long long)b * a.Hkv + kv) * a.n_sel;
-    PagedSpan s;
-    const bool ok = paged_span(a, b, s);
-    const int first = s.lo / a.P, n = ok && s.len > 0 ? (s.len - 1) / a.P - first + 1 : 0, take = min(n, a.n_sel);
-    for (int i = take + tid; i < a.n_sel; i += PS_THREADS) out[i] = -1;
-    if (n <= a.n_sel) {
-        for (int i = tid; i < n; i += PS_THREADS) out[i] = first + i;
-        return;
+// ---- the best pages of one (sequence, KV head), by one CTA -------------------------------------------------------------------------
+// Pages that always count apart, the rest by radix selection from the highest bit in which scores differ: eight bits a pass, until a bin ends
+// where the selection does (two passes as a rule; from the top byte, which nearly all share, every count would hit one bin).  Equal scores: the
+// lowest pages.  Then the pages in order.
+constexpr int PS_THREADS = 256;
+struct PickScratch {
+    int hist[256], scan[2][PS_THREADS / 32], digit, left, count;
+    unsigned long long ends[2][PS_THREADS / 32];
+};
+template <typename Score>                          // score of the i-th visible page
+__device__ void pick_pages(const PagedSelectArgs &a, PickScratch &s, int first, int n, int *out, Score score) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, from = min(a.keep_first, n), to = max(from, n - a.keep_last);      // ranked: from .. to - 1
+    int left = min(n, a.n_sel) - (n - (to - from));                // of the ranked pages
+    auto key = [&](int i) -> uint64_t { return (uint64_t)score(i) ^ (1ULL << 63); };
+    uint64_t lo = ~0ULL, hi = 0;
+    for (int i = from + tid; i < to; i += PS_THREADS) { const uint64_t u = key(i); lo = u < lo ? u : lo; hi = u > hi ? u : hi; }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        const uint64_t l2 = __shfl_xor_sync(0xffffffffu, lo, m), h2 = __shfl_xor_sync(0xffffffffu, hi, m);
+        lo = l2 < lo ? l2 : lo; hi = h2 > hi ? h2 : hi;
     }
-    const long long *score = a.score + ((long long)b * a.Hkv + kv) * a.table_ld;
-    auto key = [&](int i) -> uint64_t {                            // ascending as unsigned; pages that always count come out on top
-        if (i < a.keep_first || i >= n - a.keep_last) return ~0ULL;
-        return min((uint64_t)score[i] ^ (1ULL << 63), ~0ULL - 1);
-    };
-    uint64_t limit = 0;
-    int left = take;                                               // of the pages that share the digits found so far
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        if (tid < 256) s_hist[tid] = 0;
+    if (lane == 0) { s.ends[0][warp] = lo; s.ends[1][warp] = hi; }
+    __syncthreads();
+    for (int w = 0; w < PS_THREADS / 32; w++) { lo = s.ends[0][w] < lo ? s.ends[0][w] : lo; hi = s.ends[1][w] > hi ? s.ends[1][w] : hi; }
+    int shift = 64 - __clzll((long long)(lo ^ hi));                // bits from `shift` on are everyone's
+    uint64_t limit = shift < 64 ? hi >> shift : 0;                 // of the digits found so far
+    while (shift > 0 && left > 0) {                                // (uniform)
+        const int bits = min(8, shift);
+        shift -= bits;
+        s.hist[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += PS_THREADS) {
+        for (int i = from + tid; i < to; i += PS_THREADS) {
             const uint64_t u = key(i);
-            if (shift == 56 || (u >> (shift + 8)) == (limit >> (shift + 8))) atomicAdd(&s_hist[(u >> shift) & 255], 1);
+            if (shift + bits == 64 || (u >> (shift + bits)) == limit) atomicAdd(&s.hist[(u >> shift) & ((1u << bits) - 1)], 1);
         }
         __syncthreads();
-        if (warp == 0) {                                           // the digit in which the left-th largest lies: lane l has digits 255 - 8l ..
+        if (warp == 0) {                                           // the digit where the left-th largest lies: lane l has digits 255 - 8l ..
             int mine = 0;
-            for (int d = 0; d < 8; d++) mine += s_hist[255 - 8 * lane - d];
+            for (int d = 0; d < 8; d++) mine += s.hist[255 - 8 * lane - d];
             int upto = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
             int above = upto - mine;
             if (above < left && upto >= left)
                 for (int d = 0; d < 8; d++) {
-                    const int c = s_hist[255 - 8 * lane - d];
-                    if (above + c >= left) { s_digit = 255 - 8 * lane - d; s_left = left - above; break; }
+                    const int c = s.hist[255 - 8 * lane - d];
+                    if (above + c >= left) { s.digit = 255 - 8 * lane - d; s.left = left - above; s.count = c; break; }
                     above += c;
                 }
         }
         __syncthreads();
-        limit |= (uint64_t)s_digit << shift;
-        left = s_left;
+        limit = (shift + bits == 64 ? 0 : limit << bits) | (uint64_t)s.digit;
+        left = s.left;
+        const bool all = s.count == left;
         __syncthreads();
+        if (all) break;
     }
-    int done = 0, equal_done = 0;                                  // pages written, pages equal to the limit met
-    for (int i0 = 0; i0 < n; i0 += PS_THREADS) {
-        const int i = i0 + tid;
-        const uint64_t u = i < n ? key(i) : 0;
-        const bool eq = i < n && u == limit;
-        const unsigned eqs = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) s_scan[0][warp] = __popc(eqs);
-        __syncthreads();
-        int eq_before = equal_done + __popc(eqs & ((1u << lane) - 1)), eq_all = 0;
-        for (int w2 = 0; w2 < PS_THREADS / 32; w2++) { if (w2 < warp) eq_before += s_scan[0][w2]; eq_all += s_scan[0][w2]; }
-        const bool in = i < n && (u > limit || (eq && eq_before < left));
-        const unsigned ins = __ballot_sync(0xffffffffu, in);
-        if (lane == 0) s_scan[1][warp] = __popc(ins);
-        __syncthreads();
-        int at = done + __popc(ins & ((1u << lane) - 1)), in_all = 0;
-        for (int w2 = 0; w2 < PS_THREADS / 32; w2++) { if (w2 < warp) at += s_scan[1][w2]; in_all += s_scan[1][w2]; }
-        if (in) out[at] = first + i;
-        done += in_all; equal_done += eq_all;
-        __syncthreads();
+    if (shift == 64) shift = 0;                                    // (nothing ranked: lo ^ hi has its top bit)
+    // a warp has a run of pages: what it takes is counted, then written behind what the warps before it take
+    const int strips = (n + PS_THREADS - 1) / PS_THREADS, i0 = warp * strips * 32;
+    auto look = [&](int i, bool &sure, bool &eq) {
+        const bool ranked = i >= from && i < to;
+        const uint64_t u = ranked ? key(i) >> shift : 0;
+        sure = i < n && (!ranked || (left > 0 && u > limit));
+        eq = ranked && left > 0 && u == limit;
+    };
+    int sures = 0, eqs = 0;
+    for (int k = 0; k < strips; k++) {
+        bool sure, eq;
+        look(i0 + 32 * k + lane, sure, eq);
+        sures += __popc(__ballot_sync(0xffffffffu, sure)); eqs += __popc(__ballot_sync(0xffffffffu, eq));
     }
+    if (lane == 0) { s.scan[0][warp] = sures; s.scan[1][warp] = eqs; }
+    __syncthreads();
+    int at = 0, eq_before = 0;
+    for (int w = 0; w < warp; w++) { at += s.scan[0][w] + max(0, min(s.scan[1][w], left - eq_before)); eq_before += s.scan[1][w]; }
+    for (int k = 0; k < strips; k++) {
+        const int i = i0 + 32 * k + lane;
+        const unsigned below = (1u << lane) - 1;
+        bool sure, eq;
+        look(i, sure, eq);
+        const unsigned eq_all = __ballot_sync(0xffffffffu, eq);
+        const bool in = sure || (eq && eq_before + __popc(eq_all & below) < left);
+        const unsigned in_all = __ballot_sync(0xffffffffu, in);
+        if (in) out[at + __popc(in_all & below)] = first + i;
+        at += __popc(in_all); eq_before += __popc(eq_all);
+    }
+}
+// Visible pages first .. first + n - 1; what is not ranked is written: the whole list where they all fit, -1 behind its end.
+__device__ __forceinline__ bool pick_begin(const PagedSelectArgs &a, int b, int kv, int &first, int &n, int *&out) {
+    PagedSpan s;
+    const bool ok = paged_span(a, b, s);
+    out = a.out + ((long long)b * a.Hkv + kv) * a.n_sel;
+    first = s.lo / a.P;
+    n = ok && s.len > 0 ? (s.len - 1) / a.P - first + 1 : 0;
+    return n > a.n_sel;
+}
+__device__ __forceinline__ void pick_rest(const PagedSelectArgs &a, int first, int n, int *out) {
+    for (int i = threadIdx.x; i < a.n_sel; i += blockDim.x)
+        if (i >= n) out[i] = -1;
+        else if (n <= a.n_sel) out[i] = first + i;
+}
+
+__global__ void __launch_bounds__(PS_THREADS) paged_pick_kernel(const PagedSelectArgs a) {
+    pdl_enter();
+    __shared__ PickScratch s;
+    const int kv = blockIdx.x, b = blockIdx.y;
+    int first, n, *out;
+    const bool rank = pick_begin(a, b, kv, first, n, out);
+    pick_rest(a, first, n, out);
+    const long long *score = a.score + ((long long)b * a.Hkv + kv) * a.table_ld;
+    if (rank) pick_pages(a, s, first, n, out, [&](int i) { return score[i]; });
+}
+
+// Both in one launch where head dimension and page count allow: a cluster of CTAs per (sequence, KV head) ranks the pages, 64 at a time each,
+// into the first CTA's shared memory, and that one picks.  A warp has the bounds of eight pages copied into shared memory (a page's 8 hd bytes lie
+// side by side; a gap behind each keeps the banks apart); four lanes share a page, a lane takes every fourth group of four dimensions of eight
+// heads: 32 x 32 -> 64-bit multiply-adds (four clocks a warp) of a query value with the bound that its sign selects (four clocks on the
+// other pipe).  What bounds it: those, 4.3 us for the 39 MB of 38500 pages of two bounds of 128 and 8 heads on 148 SMs; memory alone 6.  (Loads
+// into registers instead, two pages a lane: four round trips a page, 20 us.)  A query beyond int32 takes 64-bit products.
+constexpr int PR_PAGES = 8;                        // pages of a warp at a time
+constexpr int PR_GAP = 64;
+constexpr int PR_MOST = 8192;                      // pages of a sequence: 64 KB of scores
+__host__ __device__ inline int rank_heads(int rep) { return rep <= 4 ? 4 : (rep + 7) / 8 * 8; }
+__host__ __device__ inline size_t rank_stage(int hd) { return (size_t)PR_PAGES * (8 * hd + PR_GAP); }       // of a warp
+template <bool WIDE, int HEADS>                   // HEADS at a time: the queries are padded with zeros to a multiple
+__device__ __forceinline__ bool rank_pages(const PagedSelectArgs &a, const int *q32, const int64_t *q64, unsigned char *stage, uint64_t *bar, int rep, int b, int kv, int first, int n, long long *to, int block,
+                                           int blocks, bool &bad, volatile int *abort_flag) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, g = lane >> 2, ld = 8 * a.hd + PR_GAP;
+    const uint32_t bar_at = tl_u32(bar), to_at = tl_u32(stage);
+    uint32_t pass = 0;
+    const int step = blocks * (PS_THREADS / 32) * PR_PAGES;
+    for (int p0 = (block * (PS_THREADS / 32) + warp) * PR_PAGES; p0 < n; p0 += step, pass ^= 1) {
+        // the warp's pages; one outside the pool counts as lowest
+        int page = -1;
+        if (lane < PR_PAGES && p0 + lane < n) {
+            page = a.table[(long long)b * a.table_ld + first + p0 + lane];
+            if (page < 0 || page >= a.n_pages) { bad = true; page = -1; }
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) tl_expect(bar_at, (uint32_t)__popc(there) * 8 * a.hd);
+        __syncwarp();
+        if (page >= 0)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(to_at + lane * ld), "l"(a.bounds + ((long long)page * a.Hkv + kv) * 2 * a.hd), "r"(8 * a.hd), "r"(bar_at) : "memory");
+        if (!tl_wait(bar_at, pass, abort_flag)) return false;
+        const int4 *row = reinterpret_cast<const int4 *>(stage + g * ld) + t;
+        long long best = INT64_MIN;
+        for (int h0 = 0; h0 < rep; h0 += HEADS) {
+            long long sum[HEADS];
+#pragma unroll
+            for (int h = 0; h < HEADS; h++) sum[h] = 0;
+            const int4 *q4 = reinterpret_cast<const int4 *>(q32 + h0 * a.hd) + t;
+#pragma unroll 1
+            for (int d = 0; d < a.hd; d += 16) {
+                const int4 mx = row[d / 4], mn = row[(a.hd + d) / 4];
+                if (!WIDE) {
+                    int4 q[HEADS];
+#pragma unroll
+                    for (int h = 0; h < HEADS; h++) q[h] = q4[(h * a.hd + d) / 4];
+#pragma unroll
+                    for (int h = 0; h < HEADS; h++) sum[h] += (long long)q[h].x * (q[h].x < 0 ? mn.x : mx.x);
+#pragma unroll
+                    for (int h = 0; h < HEADS; h++) sum[h] += (long long)q[h].y * (q[h].y < 0 ? mn.y : mx.y);
+#pragma unroll
+                    for (int h = 0; h < HEADS; h++) sum[h] += (long long)q[h].z * (q[h].z < 0 ? mn.z : mx.z);
+#pragma unroll
+                    for (int h = 0; h < HEADS; h++) sum[h] += (long long)q[h].w * (q[h].w < 0 ? mn.w : mx.w);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < HEADS; h++)
+#pragma unroll 1
+                        for (int e = 0; e < 4; e++) {
+                            const int64_t q = q64[(h0 + h) * a.hd + d + 4 * t + e];
+                            const int4 v = q < 0 ? mn : mx;
+                            sum[h] = (long long)((uint64_t)sum[h] + (uint64_t)q * (uint64_t)(int64_t)(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w));
+                        }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < HEADS; h++) {
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+                if (h0 + h < rep) best = max(best, sum[h]);
+            }
+        }
+        if (t == 0 && p0 + g < n) to[p0 + g] = (there >> g) & 1 ? best : INT64_MIN;
+        __syncwarp();                                              // the stage may be filled again
+    }
+    return true;
+}
+__global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const PagedSelectArgs a) {
+    pdl_enter();
+    extern __shared__ __align__(16) int64_t pr_q[];                // queries [rep][hd] as int64, then as int32; the warps' pages; scores
+    __shared__ PickScratch s;
+    __shared__ __align__(8) uint64_t s_bar[PS_THREADS / 32];
+    __shared__ int s_wide, s_abort;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, rep = a.H / a.Hkv, half = a.hd / 2, block = blockIdx.x, blocks = gridDim.x, kv = blockIdx.y, b = blockIdx.z;
+    const int padded = rank_heads(rep);
+    int *q32 = reinterpret_cast<int *>(pr_q + padded * a.hd);
+    unsigned char *stage = reinterpret_cast<unsigned char *>(q32 + padded * a.hd);
+    long long *score = reinterpret_cast<long long *>(stage + PS_THREADS / 32 * rank_stage(a.hd));
+    int first, n, *out;
+    const bool rank = pick_begin(a, b, kv, first, n, out);
+    if (block == 0) pick_rest(a, first, n, out);
+    if (!rank) {                                                   // the whole cluster
+        PagedSpan span;
+        if (tid == 0 && block == 0 && kv == 0 && !paged_span(a, b, span)) atomicOr(a.flags, 16);
+        return;
+    }
+    if (tid == 0) {
+        s_wide = 0; s_abort = 0;
+        for (int w = 0; w < PS_THREADS / 32; w++) tl_init(tl_u32(&s_bar[w]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    bool wide = false, bad = false;
+    const long long pos = a.lengths[b] - 1;
+    for (int idx = tid; idx < padded * half; idx += PS_THREADS) {
+        const int h = idx / half, i = idx - h * half, d0 = a.rope == 2 ? i : 2 * i, d1 = a.rope == 2 ? i + half : 2 * i + 1;
+        int64_t x0 = 0, x1 = 0;
+        if (h < rep) {
+            const int64_t *src = a.q + b * a.q_ld + (long long)(kv * rep + h) * a.hd;
+            x0 = src[d0]; x1 = src[d1];
+            paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, pos, i, x0, x1);
+        }
+        pr_q[h * a.hd + d0] = x0; pr_q[h * a.hd + d1] = x1;
+        q32[h * a.hd + d0] = (int)x0; q32[h * a.hd + d1] = (int)x1;
+        wide = wide || x0 != (int)x0 || x1 != (int)x1;
+    }
+    if (wide) s_wide = 1;
+    if (blocks > 1) cluster.sync();                                // (the first CTA has started)
+    else __syncthreads();
+    long long *to = blocks > 1 ? cluster.map_shared_rank(score, 0) : score;
+    unsigned char *mine = stage + (tid >> 5) * rank_stage(a.hd);
+    const bool ok = s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort)
+                  : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort)
+                             : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort);
+    if (!ok) { volatile int patient = 0; tl_wait_slow(tl_u32(&s_bar[tid >> 5]), 0, &patient); atomicOr(a.flags, FLAG_GAVE_UP); }      // (a copy under way ends first)
+    if (bad) atomicOr(a.flags, 16);
+    if (blocks > 1) cluster.sync();
+    else __syncthreads();
+    if (block == 0) pick_pages(a, s, first, n, out, [&](int i) { return score[i]; });
 }
 
 }  // namespace
@@ -432,7 +611,26 @@ cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s) {
 }
 
 cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
-    const size_t smem = (size_t)(a.H / a.Hkv) * a.hd * 8;
+    const int rep = a.H / a.Hkv;
+    const size_t fused = (size_t)rank_heads(rep) * a.hd * 12 + PS_THREADS / 32 * rank_stage(a.hd) + (size_t)a.table_ld * 8;
+    if (a.hd % 16 == 0 && a.table_ld <= PR_MOST && fused <= 220 * 1024 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0) {
+        cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e != cudaSuccess) return e;
+        // a cluster of up to eight, a round of 64 pages for each
+        const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>(8, (a.table_ld + 63) / (PR_PAGES * (PS_THREADS / 32))));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(blocks, (unsigned)a.Hkv, (unsigned)a.B); cfg.blockDim = dim3(PS_THREADS); cfg.dynamicSmemBytes = fused; cfg.stream = s;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = blocks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 2;
+        e = cudaLaunchKernelEx(&cfg, paged_select_kernel, a);
+        note_launch();
+        return e != cudaSuccess ? e : cudaGetLastError();
+    }
+    const size_t smem = (size_t)rep * a.hd * 8;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(paged_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;

@@ -79,12 +79,12 @@ __host__ __device__ inline TcWork tc_work(const PagedAttnArgs &a, int ctas, size
 __device__ __forceinline__ int tc_tiles(const PagedAttnArgs &a, const PagedSpan &s) {
     if (s.len == 0) return 0;
     if (a.sel) return (int)tc_tiles_most(a);
-    const int box = tc_box(a);
-    return (s.len - s.lo / box * box + PT_KEYS - 1) / PT_KEYS;
+    return (s.len - (s.lo & ~(tc_box(a) - 1)) + PT_KEYS - 1) / PT_KEYS;
 }
 
 // A walk over a run of the list, tile by tile.
 struct TcWalk {
+    int owner;                                     // of a cut pair: the CTA whose cell it has
     int b, pair_of, t, nt, left, tile, part, seg;  // sequence; its pair; tile of the pair, its tiles; tiles left; number in the list; tiles of the pair and of the accumulation before this one
     PagedSpan s;
     __device__ __forceinline__ void load(const PagedAttnArgs &a) { paged_span(a, b, s); nt = tc_tiles(a, s); }
@@ -109,83 +109,109 @@ struct TcWalk {
     }
 };
 
-// The whole CTA: its share of the list, as up to three runs: the pair that begins in a CTA before (or goes on beyond, where there is no
-// other), the pair that goes on in the next one, the whole pairs between them.  Returns the list's length.  scan: 40 ints of shared memory.
-// Of the two cut pairs the one that an even CTA has in common with the odd one before it is run 0 of both: its maxima are there while the
-// CTAs are at the scores of the rest, its normaliser while they are at the values of whole pairs, and the other pair's while they are at the
-// values of this one.
+// One warp: the CTA's share of the list, as up to three runs: two pairs that it has in common with other CTAs, and whole pairs.  A pair that is cut costs its CTAs an exchange, some six microseconds or four tiles; a second pair costs other query columns.
+//  * Whole pairs, dealt out in order, where the longest pairs so dealt make a CTA no more than four tiles above the average.
+//  * Else each pair has CTAs of its own in proportion to its tiles, where there are enough CTAs and no part is more than two tiles above it.
+//  * Else the list is cut evenly: a CTA has the end of a pair, whole ones, the beginning of another.  (Cut pairs in an order that has two neighbours at
+//    the same one first, normalised between tiles as soon as the maxima are in, came to the same: what is looked up between tiles holds them up.)
 enum { RUN_WHOLE = 2, RUNS };
-__device__ __forceinline__ uint32_t tc_share(const PagedAttnArgs &a, int *scan, TcWalk (&run)[RUNS]) {
-    const int tid = threadIdx.x, n = blockDim.x, lane = tid & 31, warp = tid >> 5, per_seq = a.Hkv * tc_head_groups(a), warps = n >> 5;
-    auto count = [&](int b) {
-        PagedSpan s;
-        if (b >= a.B) return 0;
-        if (!paged_span(a, b, s) && blockIdx.x == 0) atomicOr(a.flags, 16);
-        return tc_tiles(a, s);
-    };
-    const int own = count(tid);
-    int mine = own;
-    for (int b = tid + n; b < a.B; b += n) mine += count(b);
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) scan[warp] = mine;
-    if (tid == 0) scan[32] = scan[34] = -1;
-    __syncthreads();
-    int all = 0;
-    for (int i = 0; i < warps; i++) all += scan[i];
-    __syncthreads();
-    const uint32_t total = (uint32_t)all * per_seq;  // (total * 256 fits 32 bits: paged_tc_ok)
-    const int from = (int)(total * blockIdx.x / gridDim.x), to = (int)(total * (blockIdx.x + 1) / gridDim.x);
-    int before = 0;                                // tiles per pair of the sequences in front
-    for (int b0 = 0; b0 < a.B && from < to; b0 += n) {
-        const int c = b0 == 0 ? own : count(b0 + tid);
-        int upto = c;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
-        if (lane == 31) scan[warp] = upto;
-        __syncthreads();
-        int sum = 0;
-        for (int i = 0; i < warps; i++) { if (i < warp) upto += scan[i]; sum += scan[i]; }
-        const int lo = (before + upto - c) * per_seq, hi = lo + c * per_seq;
-        if (from >= lo && from < hi) { scan[32] = b0 + tid; scan[33] = from - lo; }
-        if (to > lo && to <= hi) { scan[34] = b0 + tid; scan[35] = to - 1 - lo; }
-        before += sum;
-        __syncthreads();
-        if (scan[32] >= 0 && scan[34] >= 0) break;
-        __syncthreads();
+__device__ __noinline__ int tc_count(const PagedAttnArgs &a, int b) {
+    PagedSpan s;
+    if (b >= a.B) return 0;
+    if (!paged_span(a, b, s) && blockIdx.x == 0) atomicOr(a.flags, 16);
+    return tc_tiles(a, s);
+}
+__device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[RUNS]) {
+    const int lane = threadIdx.x & 31, per_seq = a.Hkv * tc_head_groups(a), ctas = gridDim.x, me = blockIdx.x;
+    const int own = tc_count(a, lane);             // (32 sequences at a time; the first ones kept)
+    auto count = [&](int b) { return b < 32 ? own : tc_count(a, b); };
+    int sum = 0, some = 0, longest = 0;
+#pragma unroll 1
+    for (int b = lane; b - lane < a.B; b += 32) { const int c = count(b); sum += c; some += c > 0; longest = max(longest, c); }
+    const int total = __reduce_add_sync(0xffffffffu, sum) * per_seq, pairs = __reduce_add_sync(0xffffffffu, some) * per_seq, most = __reduce_max_sync(0xffffffffu, longest);      // (total * 256 fits 32 bits: paged_tc_ok)
+    const int average = total / ctas;
+    // CTAs of a pair of c tiles that has its own, and the tiles of one
+    auto parts = [&](int c) { return c == 0 ? 0 : max(1, min(c, (int)((uint32_t)c * ctas / total))); };
+    auto part = [&](int c) { return c == 0 ? 0 : (c + parts(c) - 1) / parts(c); };
+    enum { WHOLE_PAIRS, OWN_CTAS, EVEN } way = EVEN;
+    if ((pairs + ctas - 1) / ctas * most <= average + 4) way = WHOLE_PAIRS;
+    else if (pairs <= ctas) {
+        int ps = 0, pl = 0;
+#pragma unroll 1
+        for (int b = lane; b - lane < a.B; b += 32) { const int c = count(b); ps += parts(c); pl = max(pl, part(c)); }
+        if ((int)__reduce_add_sync(0xffffffffu, ps) * per_seq <= ctas && (int)__reduce_max_sync(0xffffffffu, pl) <= average + 2) way = OWN_CTAS;
     }
-    if (tid == 0) {
-        TcWalk w = {}, none = {};
-        w.left = to - from; w.tile = from;
-        const int head = blockIdx.x & 1, tail = head ^ 1;
-        run[0] = run[1] = run[RUN_WHOLE] = none;
-        if (w.left > 0 && scan[32] >= 0 && scan[34] >= 0) {
-            w.b = scan[32];
-            w.load(a);
-            w.pair_of = scan[33] / w.nt; w.t = scan[33] - w.pair_of * w.nt;
-            if (w.rest() < w.nt) {
-                run[head] = w;
-                run[head].left = w.rest();
-                w.skip(a, per_seq, w.rest());
-            }
-            if (w.left > 0) {
-                TcWalk e = none;
-                e.b = scan[34];
-                e.load(a);
-                e.pair_of = scan[35] / e.nt;
-                e.left = scan[35] - e.pair_of * e.nt + 1;
-                e.tile = to - e.left;
-                if (e.left < e.nt) { run[tail] = e; w.left -= e.left; }
-                run[RUN_WHOLE] = w;
+    // the share in units of the way, and where in the list its first and last unit are
+    const int all = way == EVEN ? total : pairs, from = way == OWN_CTAS ? me : (int)((uint32_t)all * me / ctas), to = way == OWN_CTAS ? me + 1 : (int)((uint32_t)all * (me + 1) / ctas);
+    int at[2] = {-1, -1}, in[2] = {0, 0}, first[2] = {0, 0};       // sequence, unit in it, its first tile
+    int before = 0, tiles_before = 0;              // units and tiles per pair of the sequences in front
+#pragma unroll 1
+    for (int b0 = 0; b0 < a.B && from < to && (at[0] < 0 || at[1] < 0); b0 += 32) {
+        const int c = count(b0 + lane), mine = way == EVEN ? c : way == OWN_CTAS ? parts(c) : (int)(c > 0);
+        int upto = mine, tiles = c;
+#pragma unroll 1
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, d), p = __shfl_up_sync(0xffffffffu, tiles, d);
+            if (lane >= d) { upto += o; tiles += p; }
+        }
+        const int lo = (before + upto - mine) * per_seq, hi = lo + mine * per_seq;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int unit = e ? to - 1 : from;
+            const uint32_t here = __ballot_sync(0xffffffffu, unit >= lo && unit < hi);
+            if (here && at[e] < 0) {
+                const int l = __ffs(here) - 1;
+                at[e] = b0 + l;
+                in[e] = __shfl_sync(0xffffffffu, unit - lo, l);
+                first[e] = __shfl_sync(0xffffffffu, (tiles_before + tiles - c) * per_seq, l);
             }
         }
+        before += __shfl_sync(0xffffffffu, upto, 31); tiles_before += __shfl_sync(0xffffffffu, tiles, 31);
     }
-    return total;
+    if (lane != 0) return;
+    TcWalk w = {}, none = {};
+    run[0] = run[1] = run[RUN_WHOLE] = none;
+    if (from >= to || at[0] < 0 || at[1] < 0) return;
+    w.b = at[0];
+    w.load(a);
+    TcWalk e = none;
+    e.b = at[1];
+    e.load(a);
+    if (way == OWN_CTAS) {
+        const int ps = parts(w.nt), size = part(w.nt), piece = in[0] % ps;
+        w.pair_of = in[0] / ps;
+        w.t = piece * size;
+        w.left = max(0, min(size, w.nt - w.t));
+        w.tile = first[0] + w.pair_of * w.nt + w.t;
+        w.owner = me - piece;
+        if (w.left > 0) run[w.left == w.nt ? RUN_WHOLE : 0] = w;
+    } else if (way == WHOLE_PAIRS) {
+        w.pair_of = in[0];
+        w.tile = first[0] + w.pair_of * w.nt;
+        w.left = first[1] + (in[1] + 1) * e.nt - w.tile;
+        run[RUN_WHOLE] = w;
+    } else {
+        auto owner = [&](int tile) { return (int)((((uint32_t)tile + 1) * ctas - 1) / total); };
+        w.pair_of = in[0] / w.nt; w.t = in[0] - w.pair_of * w.nt;
+        w.left = to - from; w.tile = from;
+        w.owner = owner(w.tile - w.t);
+        if (w.rest() < w.nt) {
+            run[0] = w;
+            run[0].left = w.rest();
+            w.skip(a, per_seq, w.rest());
+        }
+        if (w.left > 0) {
+            e.pair_of = in[1] / e.nt;
+            e.left = in[1] - e.pair_of * e.nt + 1;
+            e.tile = to - e.left;
+            e.owner = owner(e.tile);
+            if (e.left < e.nt) { run[1] = e; w.left -= e.left; }
+            run[RUN_WHOLE] = w;
+        }
+    }
 }
-// the CTA where tile `tile` of the list lies
-__device__ __forceinline__ int tc_owner(int tile, uint32_t total) { return (int)((((uint32_t)tile + 1) * gridDim.x - 1) / total); }
 
-// Runs in the order of the scores are as they are numbered: what other CTAs wait for comes first.  Values: whole pairs first, while normalisers
-// of the others are on their way.
+// Scores: the cut pairs first, which other CTAs wait for.  Values: whole pairs first, while normalisers of the others are on their way.
 __device__ __forceinline__ int tc_value_run(int u) { return u == 0 ? RUN_WHOLE : u - 1; }
 
 // Operand descriptors: the lower word has the address (in 16 bytes), the upper one the distance of groups of eight rows and the swizzle.  An
@@ -220,7 +246,7 @@ struct TcBars {
     uint64_t full[PT_MAX_SLOTS], empty[PT_MAX_SLOTS], meta[PT_META];
     uint64_t score_full[PT_SETS], score_free[2], query_full, prob_full[PT_SETS], prob_free[PT_SETS], out_full[2], out_free[2], pair_done, drain;
     uint32_t tmem;
-    int abort, scan[40];
+    int abort;
     TcWalk run[RUNS];
     unsigned char mask[PT_META][PT_GROUPS];
 };
@@ -260,7 +286,7 @@ __device__ __forceinline__ TcLook tc_look(const PagedAttnArgs &a, const TcWalk &
         if (logical >= a.table_ld) { atomicOr(a.flags, 16); return x; }
         pos = logical * a.P + x.r;                 // (a table's rows are numbered in 31 bits)
     } else {
-        pos = w.s.lo / box * box + (w.t * PT_GROUPS + l) * 8;
+        pos = (w.s.lo & ~(box - 1)) + (w.t * PT_GROUPS + l) * 8;
         logical = (int)((unsigned)pos / (unsigned)a.P);
         x.r = pos - logical * a.P;
     }
@@ -390,6 +416,19 @@ __device__ __forceinline__ void tc_queries(const PagedAttnArgs &a, const TcWalk 
     }
 }
 
+// A warp's wait for a count that other CTAs raise: false where it gave up.
+__device__ __forceinline__ bool tc_poll(const unsigned *count, unsigned target, volatile int *abort_flag) {
+    bool done = false;
+    for (unsigned i = 0; i < PT_POLLS && !done && !*abort_flag; i++) {
+        unsigned v;
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
+        done = v == target;
+    }
+    done = __all_sync(0xffffffffu, done);
+    if (!done) *abort_flag = 1;
+    return done;
+}
+
 // The cells of pairs that are cut between CTAs, cleared.  The attention's launch overlaps it: what lies in front of this kernel on the stream
 // has ended when the attention's CTAs start, so that only the cells are waited for.
 __global__ void paged_clear_kernel(TcCell *cell, unsigned long long *acc, int per_cta) {
@@ -422,9 +461,9 @@ struct TcExp16 {
 // Distances of a lane's eight keys in one tile and the base they lie below; dist, base: of the lane in tile 0.
 __device__ __forceinline__ void tc_distances(const uint32_t *dist, const long long *base, int tile, uint32_t (&d)[8], unsigned long long &biased) {
     const uint4 *from = reinterpret_cast<const uint4 *>(dist + (long long)tile * (PT_HEADS * PT_KEYS));
-    const uint4 x = __ldcg(from), y = __ldcg(from + 1);
+    const uint4 x = from[0], y = from[1];          // (the CTA's own: its SM's cache may hold them)
     d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w; d[4] = y.x; d[5] = y.y; d[6] = y.z; d[7] = y.w;
-    biased = (uint64_t)__ldcg(base + (long long)tile * 4 * PT_HEADS) ^ PT_BIAS;
+    biased = (uint64_t)base[(long long)tile * 4 * PT_HEADS] ^ PT_BIAS;
 }
 // exponential of a key `d` below a base that lies `above` below the pair's largest score, both at most the limit
 template <class Exp>
@@ -486,7 +525,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tl_u32(&s.tmem)), "r"(sh.columns));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    const uint32_t total = tc_share(a, s.scan, s.run);
+    if (warp == 3) tc_share(a, s.run);
     tc_before();
     __syncthreads();
     tc_after();
@@ -578,7 +617,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         };
         // what is left to do with the maxima of a pair (or of its part here) once the next pair's query columns are written, so that the
         // products go on meanwhile: exchange them; a whole pair's normaliser
-        struct { int n = 0, nt, first, index; long long pair; } behind;    // tiles, the pair's; number of the first in the list, and among this CTA's scores
+        struct { int n = 0, nt, first, index, owner; long long pair; } behind;     // tiles, the pair's; number of the first in the list, and among this CTA's scores
         long long largest = INT64_MIN;             // lane h: of head h, over this warp's tiles of the pair
         int whole_pairs = 0;
         auto settle = [&](long long most) {
@@ -600,7 +639,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 const unsigned long long sum = normalise(behind.first, behind.n, (set - behind.index) & 3, m);
                 if (t == 0) z[g] = sum;
             } else {
-                TcCell *cell = work.cell + tc_owner(behind.first, total);
+                asm volatile("griddepcontrol.wait;" ::: "memory");      // the cells are clear
+                TcCell *cell = work.cell + behind.owner;
                 if (lane < heads_most) atomicMax(cell->top + lane, biased);
                 __threadfence();
                 __syncwarp();
@@ -609,28 +649,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             behind.n = 0;
             return true;
         };
-        // Pairs that go on in other CTAs: their normalisers as soon as every CTA's maxima are in, looked for between tiles.
-        bool due[RUN_WHOLE] = {s.run[0].left > 0, s.run[1].left > 0};
-        auto complete = [&](const unsigned *count, int nt) {
-            unsigned v;
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
-            return __all_sync(0xffffffffu, v == (unsigned)nt * PT_WORKERS) != 0;
-        };
-        auto normalise_cut = [&](int x) {          // false: not yet
-            if (!due[x]) return true;
-            const int first = s.run[x].tile, n = s.run[x].left, nt = s.run[x].nt;
-            TcCell *cell = work.cell + tc_owner(first - s.run[x].t, total);
-            if (!complete(&cell->tops, nt)) return false;
-            const unsigned long long z = normalise(first, n, (set - (x == 0 ? 0 : s.run[0].left)) & 3, __ldcg(cell->top + g));
-            if (t == 0 && g < heads_most) atomicAdd(cell->z + g, z);
-            __threadfence();
-            __syncwarp();
-            if (lane == 0) atomicAdd(&cell->zs, (unsigned)n);
-            due[x] = false;
-            return true;
-        };
         for (int x = worker; x < (int)(PT_SETS * PT_PROBS / 16); x += 32 * PT_WORKERS) reinterpret_cast<uint4 *>(probs)[x] = make_uint4(0, 0, 0, 0);      // (the columns beyond 24 stay so)
-        asm volatile("griddepcontrol.wait;" ::: "memory");
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         for (int b = blockIdx.x; b < a.B; b += gridDim.x) {                // sequences without keys
             PagedSpan none;
@@ -683,11 +702,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                     if (lane == 0) tl_arrive(tl_u32(&s.score_free[i & 1]));
                     if (lane < PT_HEADS) work.base[((long long)v.tile * 4 + quarter) * PT_HEADS + lane] = base;
                     largest = max(largest, base);
-#pragma unroll 1
-                    for (int x = 0; x < u; x++) normalise_cut(x);
                 }
                 if (v.ends_part()) {
-                    behind.n = v.part + 1; behind.nt = v.nt; behind.first = v.tile - v.t; behind.index = i - v.part;
+                    behind.n = v.part + 1; behind.nt = v.nt; behind.first = v.tile - v.t; behind.index = i - v.part; behind.owner = v.owner;
                     behind.pair = (long long)v.b * per_seq + v.pair_of;
                 }
                 fresh = v.t + 1 == v.nt;
@@ -696,6 +713,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         }
         __syncwarp();
         ok = ok && settle(largest);
+        // ---- normalisers of the pairs that go on in other CTAs, once everybody's maxima are in ---------------------------------------
+        for (int x = 0, index = 0; ok && x < RUN_WHOLE; x++) {
+            const int n = s.run[x].left;
+            if (n == 0) continue;
+            TcCell *cell = work.cell + s.run[x].owner;
+            ok = tc_poll(&cell->tops, (unsigned)s.run[x].nt * PT_WORKERS, abort_flag);
+            if (!ok) break;
+            const unsigned long long z = normalise(s.run[x].tile, n, (set - index) & 3, __ldcg(cell->top + g));
+            if (t == 0 && g < heads_most) atomicAdd(cell->z + g, z);
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) atomicAdd(&cell->zs, (unsigned)n);
+            index += n;
+        }
+        asm volatile("griddepcontrol.wait;" ::: "memory");      // (whatever the share: what is launched behind counts on it)
         // ---- probabilities and values ---------------------------------------------------------------------------------------------
         if (ok) {                                  // what the CTA's warps left in memory
             if (lane == 0) tl_arrive(tl_u32(&s.pair_done));
@@ -705,14 +737,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         Quotient quotient(0, a.fa);                // of head g
         unsigned long long top = 0, carry[2] = {0, 0};                     // of head g; output sums of earlier accumulations
         int seg = 0;
-        struct { int tiles = 0, nt, first, heads; bool ends; int64_t *out; } pending;      // sums to read out: tiles of the pair in them (and in `carry`)
+        struct { int tiles = 0, nt, owner, heads; bool ends; int64_t *out; } pending;      // sums to read out: tiles of the pair in them (and in `carry`)
         auto read_out = [&]() {
             if (!tl_wait(tl_u32(&s.out_full[seg & 1]), (seg >> 1) & 1, abort_flag)) return false;
             tc_after();
             const int byte = lane & 3, d = 32 * set + 8 * quarter + (lane >> 2), h0 = 4 * (byte >> 1) + 2 * (byte & 1);
             const bool whole = pending.tiles == pending.nt, joins = pending.ends && !whole;
-            const int owner = joins ? tc_owner(pending.first, total) : 0;
-            unsigned long long *acc = work.acc + (long long)owner * PT_HEADS * a.hd;
+            unsigned long long *acc = work.acc + (long long)pending.owner * PT_HEADS * a.hd;
             if (set < sh.chunks) {                 // dimensions 32 set ..
                 const uint32_t from = tmem + (seg & 1) * buffer + ((uint32_t)(quarter * 32) << 16) + 2 * set * 32;
                 uint64_t sum[PT_HEADS];
@@ -755,7 +786,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 __threadfence();
                 __syncwarp();
                 unsigned before = 0;
-                if (lane == 0) before = atomicAdd(&work.cell[owner].done[4 * set + quarter], (unsigned)pending.tiles);
+                if (lane == 0) before = atomicAdd(&work.cell[pending.owner].done[4 * set + quarter], (unsigned)pending.tiles);
                 before = __shfl_sync(0xffffffffu, before, 0);
                 if (before + pending.tiles == (unsigned)pending.nt) {
                     __threadfence();
@@ -781,14 +812,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1)); z += __shfl_xor_sync(0xffffffffu, z, 1);
                     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2)); z += __shfl_xor_sync(0xffffffffu, z, 2);
                 } else {
-                    TcCell *cell = work.cell + tc_owner(v.tile - v.t, total);
-                    // everybody's share of the normaliser; meanwhile what others wait for
-                    bool there = false;
-                    for (unsigned polls = 0; polls < PT_POLLS && !there && !*abort_flag; polls++) {
-                        const bool mine = normalise_cut(0) & normalise_cut(1);
-                        there = complete(&cell->zs, v.nt) && (mine || !due[run]);
-                    }
-                    if (!__all_sync(0xffffffffu, there)) { *abort_flag = 1; ok = false; break; }
+                    TcCell *cell = work.cell + v.owner;
+                    if (!tc_poll(&cell->zs, (unsigned)v.nt * PT_WORKERS, abort_flag)) { ok = false; break; }
                     top = __ldcg(cell->top + g); z = __ldcg(cell->z + g);
                 }
                 quotient = Quotient(g < heads_most ? z : 0, a.fa);
@@ -812,13 +837,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 __syncwarp();
                 if (lane == 0) tl_arrive(tl_u32(&s.prob_full[set]));
             }
-            if (i % PT_SETS == set) { normalise_cut(0); normalise_cut(1); }
             // (sums are read out behind the next tile's probabilities, so that the products go on meanwhile)
             if (pending.tiles && (i % PT_SETS == set) && !read_out()) { ok = false; break; }
             if (v.ends_segment()) {
                 if (pending.tiles && !read_out()) { ok = false; break; }
                 const int group = v.pair_of % groups, kv = v.pair_of / groups;
-                pending.tiles = v.part + 1; pending.nt = v.nt; pending.ends = v.ends_part(); pending.first = v.tile - v.t;
+                pending.tiles = v.part + 1; pending.nt = v.nt; pending.ends = v.ends_part(); pending.owner = v.owner;
                 pending.heads = min(heads_most, a.H / a.Hkv - group * heads_most);
                 pending.out = a.out + ((long long)v.b * a.H + kv * (a.H / a.Hkv) + group * heads_most) * a.hd;
             }

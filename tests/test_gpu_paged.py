@@ -253,6 +253,9 @@ SELECT = [
     (2, 2, 32, 1, [2500, 40], 0, 1, 64, 1, 1, 18),
     (4, 1, 256, 64, [3000], 1000, 1, 6, 0, 1, 18),
     (4, 2, 128, 16, [3000, 1], 0, 1, 1, 0, 1, 18),
+    (12, 1, 128, 16, [4000, 2500, 100], 0, 2, 40, 3, 2, 18),
+    (8, 8, 128, 8, [20000, 5, 9000], 0, 1, 128, 1, 1, 18),
+    (8, 1, 64, 4, [3000], 0, 1, 20, 1, 1, 62),
 ]
 
 
