@@ -5,6 +5,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -571,6 +572,19 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const Paged
     if (block == 0) pick_pages(a, s, first, n, out, [&](int i) { return score[i]; });
 }
 
+// a device's first launch of a kernel sets its attributes
+template <typename F>
+cudaError_t paged_once(std::atomic<unsigned long long> &devices, F set) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = device < 64 ? 1ULL << device : 0;
+    if (devices & bit) return cudaSuccess;
+    e = set();
+    if (e == cudaSuccess) devices |= bit;
+    return e;
+}
+
 }  // namespace
 
 cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t s) {
@@ -580,10 +594,12 @@ cudaError_t launch_paged_append(const PagedAppendArgs &a, cudaStream_t s) {
     if (units > INT32_MAX) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)units, (unsigned)a.Hkv);
     // all of an SM's memory as shared memory, as the attention behind has it: an SM changes only while it is idle
-    for (const void *kernel : {(const void *)paged_append_kernel<int64_t>, (const void *)paged_append_kernel<int32_t>}) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        if (e != cudaSuccess) return e;
-    }
+    static std::atomic<unsigned long long> configured;
+    const cudaError_t c = paged_once(configured, [] {
+        const cudaError_t e = cudaFuncSetAttribute(paged_append_kernel<int64_t>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_append_kernel<int32_t>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    });
+    if (c != cudaSuccess) return c;
     const cudaError_t e = a.narrow ? launch_behind(paged_append_kernel<int32_t>, grid, PA_THREADS, 0, s, a) : launch_behind(paged_append_kernel<int64_t>, grid, PA_THREADS, 0, s, a);
     note_launch();
     return e != cudaSuccess ? e : cudaGetLastError();
@@ -614,8 +630,11 @@ cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
     const int rep = a.H / a.Hkv;
     const size_t fused = (size_t)rank_heads(rep) * a.hd * 12 + PS_THREADS / 32 * rank_stage(a.hd) + (size_t)a.table_ld * 8;
     if (a.hd % 16 == 0 && a.table_ld <= PR_MOST && fused <= 220 * 1024 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0) {
-        cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        static std::atomic<unsigned long long> configured;
+        cudaError_t e = paged_once(configured, [] {
+            const cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+            return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        });
         if (e != cudaSuccess) return e;
         // a cluster of up to eight, a round of 64 pages for each
         const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>(8, (a.table_ld + 63) / (PR_PAGES * (PS_THREADS / 32))));

@@ -17,6 +17,7 @@
 // between CTAs (at most one begins in each) exchange maximum, normaliser and output sums in memory, in a cell of the CTA where they
 // begin.  The launch is cooperative, every wait is bounded, and integers are added in any order.  A small kernel in front clears the cells.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -869,9 +870,12 @@ bool tc_map(CUtensorMap *map, const int32_t *pool, const PagedAttnArgs &a) {
 }
 
 // SMs of the current device: CTAs of a launch at most (one is resident on each, as a cooperative launch needs)
-int tc_sms() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); return 0; }
+int tc_sms(int device) {
+    static std::atomic<int> known[64];
+    if (device >= 0 && device < 64 && known[device] > 0) return known[device];
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return 0; }
+    if (device >= 0 && device < 64) known[device] = n;
     return n;
 }
 constexpr int PT_MOST_CTAS = 256;                  // cells in the scratch
@@ -880,16 +884,25 @@ template <bool AT16, bool SMALL>
 cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     CUtensorMap kmap, vmap;
     if (!tl_encode() || !tc_map(&kmap, a.kpages, a) || !tc_map(&vmap, a.vpages, a)) return cudaErrorInvalidValue;
-    const int chunks = a.hd / 32, padded = (tc_group_heads(a) + 1) & ~1, sms = tc_sms();
+    const int chunks = a.hd / 32, padded = (tc_group_heads(a) + 1) & ~1;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const int sms = tc_sms(device);
     if (sms <= 0) return cudaErrorInvalidDevice;
     const size_t fixed = 1024 + 2 * (size_t)chunks * padded * 1024 + PT_SETS * PT_PROBS, room = 227 * 1024 - sizeof(TcBars) - 64;
     const int slots = (int)std::min<size_t>(PT_MAX_SLOTS, (room - fixed) / PT_SLOT);
     // outputs: two buffers of 64 columns a chunk; scores: two of 64, behind them or, at four chunks, over the end of the second
     const TcShape sh = {chunks, slots, chunks == 1 ? 256 : 512, chunks == 4 ? 384 : 128 * chunks};
     const size_t smem = fixed + (size_t)slots * PT_SLOT;
-    cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<AT16, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_clear_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);      // else the attention waits for idle SMs
-    if (e != cudaSuccess) return e;
+    static std::atomic<unsigned long long> configured;             // devices, a bit each
+    const unsigned long long bit = device < 64 ? 1ULL << device : 0;
+    if (!(configured & bit)) {
+        e = cudaFuncSetAttribute(paged_attn_kernel<AT16, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(room));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_clear_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);      // else the attention waits for idle SMs
+        if (e != cudaSuccess) return e;
+        configured |= bit;
+    }
     const long long most = (long long)a.B * a.Hkv * tc_head_groups(a) * tc_tiles_most(a);
     const unsigned ctas = (unsigned)std::min<long long>(std::min(sms, PT_MOST_CTAS), std::max<long long>(1, most));
     const TcWork w = tc_work(a, (int)ctas);

@@ -18,7 +18,8 @@ from .qk_cuda import Q4_K, Q6_K, _BLOCK_BYTES, _CUDA_LOCK, CudaContextError, Cud
 
 
 def _stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream as the library takes it (a stream object costs three microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def register_weight(raw, out_f: int, n_blocks: int, qtype: int) -> int:
@@ -175,36 +176,38 @@ def attention_decode_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc
     return out
 
 
-def _same_device(**tensors) -> None:
+def _on_current_device(names: str, *tensors) -> None:
     """Every tensor given lies on the current device, where the kernels run."""
-    here = torch.device("cuda", torch.cuda.current_device())
-    for name, t in tensors.items():
-        if t is not None and t.device != here:
-            raise ValueError(f"{name} lies on {t.device}, the current device is {here}")
+    here = torch.cuda.current_device()
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"{names.split()[i]} lies on {t.device}, the current device is cuda:{here}")
 
 
 def _paged_pool(kpages: torch.Tensor, vpages: torch.Tensor) -> tuple:
-    if kpages.dim() != 4 or kpages.shape != vpages.shape or kpages.dtype != torch.int32 or vpages.dtype != torch.int32:
+    shape = kpages.shape
+    if len(shape) != 4 or shape != vpages.shape or kpages.dtype != torch.int32 or vpages.dtype != torch.int32:
         raise ValueError("kpages and vpages must be int32 [pages, n_kv, page rows, head_dim] of one shape")
-    if not (kpages.is_contiguous() and vpages.is_contiguous()) or kpages.numel() == 0:
+    if not (kpages.is_contiguous() and vpages.is_contiguous()) or 0 in shape:
         raise ValueError("kpages and vpages must be contiguous and not empty")
     if (kpages.data_ptr() | vpages.data_ptr()) & 15:
         raise ValueError("kpages and vpages must start on 16 bytes")
-    return tuple(int(n) for n in kpages.shape)
+    return shape
 
 
-def _paged_table(table: torch.Tensor, per_seq: dict) -> tuple:
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous() or table.shape[1] == 0:
+def _paged_table(table: torch.Tensor, name: str, each: torch.Tensor) -> tuple:
+    shape = table.shape
+    if len(shape) != 2 or table.dtype != torch.int32 or not table.is_contiguous() or shape[1] == 0:
         raise ValueError("table must be a contiguous int32 [sequences, pages of a sequence]")
-    for name, t in per_seq.items():
-        if t.dtype != torch.int32 or t.shape != (table.shape[0],) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 vector with an entry per row of table")
-    return int(table.shape[0]), int(table.shape[1])
+    if each.dtype != torch.int32 or each.shape != shape[:1] or not each.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector with an entry per row of table")
+    return shape
 
 
 def _rows_apart(t: torch.Tensor) -> bool:
     """Whether a matrix is rows of adjacent values that do not overlap (any distance apart)."""
-    return (t.shape[0] == 0 or t.stride(1) == 1) and (t.shape[0] < 2 or t.stride(0) >= t.shape[1])
+    rows, columns = t.shape
+    return (rows == 0 or t.stride(1) == 1) and (rows < 2 or t.stride(0) >= columns)
 
 
 def _paged_rope(rope: int, cos, sin, head_dim: int) -> tuple:
@@ -213,17 +216,17 @@ def _paged_rope(rope: int, cos, sin, head_dim: int) -> tuple:
         raise ValueError("rope is 0 (none), 1 (pairs 2i, 2i + 1) or 2 (pairs i, i + head_dim / 2)")
     if rope == 0:
         return None, None, 0
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t is None or t.dtype != torch.int64 or t.dim() != 2 or t.shape[1] != head_dim // 2 or not t.is_contiguous() or t.shape != cos.shape:
-            raise ValueError(f"{name} must be a contiguous int64 [positions, head_dim / 2]")
-    return cos.data_ptr(), sin.data_ptr(), int(cos.shape[0])
+    if cos is None or sin is None or cos.dtype != torch.int64 or sin.dtype != torch.int64 or cos.dim() != 2 or cos.shape[1] != head_dim // 2 or cos.shape != sin.shape \
+            or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("cos and sin must be contiguous int64 [positions, head_dim / 2] of one shape")
+    return cos.data_ptr(), sin.data_ptr(), cos.shape[0]
 
 
 def _paged_query(q: torch.Tensor, n_seqs: int, n_kv: int, head_dim: int) -> int:
     """Query heads of q [sequences, heads * head_dim]."""
     if q.dtype != torch.int64 or q.dim() != 2 or q.shape[0] != n_seqs or q.shape[1] == 0 or q.shape[1] % (n_kv * head_dim) or not _rows_apart(q):
         raise ValueError("q must be int64 [sequences, heads * head_dim], heads a multiple of the KV heads, columns adjacent")
-    return int(q.shape[1]) // head_dim
+    return q.shape[1] // head_dim
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
@@ -240,7 +243,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages:
     met, up to the last one written: what :func:`paged_select` ranks pages by.  A value beyond int32 raises bit 2, a position or page
     outside the cache (it is left out) bit 4 of :func:`read_flags`."""
     n_pages, n_kv, page_rows, head_dim = _paged_pool(kpages, vpages)
-    B, per_seq = _paged_table(table, {"start": start})
+    B, per_seq = _paged_table(table, "start", start)
     if k.dtype not in (torch.int64, torch.int32) or v.dtype != k.dtype or k.dim() != 2 or k.shape != v.shape or k.shape[1] != n_kv * head_dim:
         raise ValueError("k and v must be int64 or int32 [rows, n_kv * head_dim] of one shape")
     if not (_rows_apart(k) and _rows_apart(v)):
@@ -253,7 +256,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages:
         raise ValueError("bounds must be a contiguous int32 [pages, n_kv, 2, head_dim]")
     cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
     lib = qk_cuda._lib()
-    _same_device(k=k, v=v, kpages=kpages, vpages=vpages, table=table, start=start, rows=rows, bounds=bounds, cos=cos, sin=sin)
+    _on_current_device("k v kpages vpages table start rows bounds cos sin", k, v, kpages, vpages, table, start, rows, bounds, cos if rope else None, sin if rope else None)
     with _CUDA_LOCK:
         rc = lib.iie_paged_append_dev(k.data_ptr(), v.data_ptr(), int(k.dtype == torch.int32), max(k.stride(0), k.shape[1]), max(v.stride(0), v.shape[1]), k.shape[0],
                                       kpages.data_ptr(), vpages.data_ptr(), n_pages, page_rows, table.data_ptr(), per_seq, start.data_ptr(),
@@ -274,7 +277,7 @@ def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     width (scratch and launch go by it; a longer sequence is left out with bit 4 of :func:`read_flags`).  Returns [B, heads * head_dim]
     int64, the bytes :func:`attention_decode` gives over the same keys."""
     n_pages, n_kv, page_rows, head_dim = _paged_pool(kpages, vpages)
-    B, per_seq = _paged_table(table, {"lengths": lengths})
+    B, per_seq = _paged_table(table, "lengths", lengths)
     n_heads = _paged_query(q, B, n_kv, head_dim)
     if pages is not None and (pages.dtype != torch.int32 or pages.dim() != 3 or pages.shape[:2] != (B, n_kv) or pages.shape[2] == 0 or not pages.is_contiguous()):
         raise ValueError("pages must be a contiguous int32 [sequences, n_kv, n] with n > 0")
@@ -287,13 +290,13 @@ def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     if inv_sqrt is None:
         inv_sqrt = int(round((1.0 / head_dim ** 0.5) * (1 << fa)))
     if out is None:
-        out = torch.empty((B, n_heads * head_dim), dtype=torch.int64, device=q.device)
+        out = q.new_empty((B, n_heads * head_dim))
     elif out.dtype != torch.int64 or out.shape != (B, n_heads * head_dim) or not out.is_contiguous():
         raise ValueError("out must be a contiguous int64 [sequences, heads * head_dim]")
     cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
     lib = qk_cuda._lib()
-    _same_device(q=q, kpages=kpages, vpages=vpages, table=table, lengths=lengths, pages=pages, out=out, cos=cos, sin=sin)
-    picked = 0 if pages is None else int(pages.shape[2])
+    _on_current_device("q kpages vpages table lengths pages out cos sin", q, kpages, vpages, table, lengths, pages, out, cos if rope else None, sin if rope else None)
+    picked = 0 if pages is None else pages.shape[2]
     need = lib.iie_paged_attn_bytes(B, max_length, int(window), picked, page_rows, n_heads, n_kv, head_dim, int(fa))
     if need < 0:
         raise ValueError("a shape that paged attention does not take")
@@ -317,21 +320,21 @@ def paged_select(q: torch.Tensor, bounds: torch.Tensor, table: torch.Tensor, len
     the last: its ``pages``."""
     if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.dtype != torch.int32 or not bounds.is_contiguous() or bounds.numel() == 0:
         raise ValueError("bounds must be a contiguous int32 [pages, n_kv, 2, head_dim]")
-    n_pages, n_kv, _, head_dim = (int(n) for n in bounds.shape)
-    B, per_seq = _paged_table(table, {"lengths": lengths})
+    n_pages, n_kv, _, head_dim = bounds.shape
+    B, per_seq = _paged_table(table, "lengths", lengths)
     n_heads = _paged_query(q, B, n_kv, head_dim)
     if page_rows <= 0 or n_select <= 0 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > n_select:
         raise ValueError("page_rows and n_select must be positive, keep_first + keep_last at most n_select")
     if window < 0:
         raise ValueError("window must not be negative (0: every key)")
     if out is None:
-        out = torch.empty((B, n_kv, n_select), dtype=torch.int32, device=q.device)
+        out = lengths.new_empty((B, n_kv, n_select))
     elif out.dtype != torch.int32 or out.shape != (B, n_kv, n_select) or not out.is_contiguous():
         raise ValueError("out must be a contiguous int32 [sequences, n_kv, n_select]")
     cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
     lib = qk_cuda._lib()
-    _same_device(q=q, bounds=bounds, table=table, lengths=lengths, out=out, cos=cos, sin=sin)
-    score = torch.empty((B, n_kv, per_seq), dtype=torch.int64, device=q.device)
+    _on_current_device("q bounds table lengths out cos sin", q, bounds, table, lengths, out, cos if rope else None, sin if rope else None)
+    score = q.new_empty((B, n_kv, per_seq))
     with _CUDA_LOCK:
         rc = lib.iie_paged_select_dev(q.data_ptr(), max(q.stride(0), q.shape[1]), bounds.data_ptr(), n_pages, int(page_rows), table.data_ptr(), per_seq, lengths.data_ptr(), B, int(n_select),
                                       int(keep_first), int(keep_last), int(window), cos_p, sin_p, rope_rows, int(rope), n_heads, n_kv, head_dim, int(fa),
