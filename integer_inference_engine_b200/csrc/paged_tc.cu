@@ -43,17 +43,18 @@ constexpr int PT_MAX_SEGMENT = 256;                // tiles that one accumulatio
 constexpr unsigned PT_POLLS = 1u << 20;            // of another CTA's count, half a microsecond and more each
 constexpr unsigned long long PT_BIAS = 1ULL << 63; // maxima are kept as unsigned: zero is below every score
 
-struct TcCell {                                    // of a pair cut between CTAs
-    unsigned long long top[PT_HEADS], z[PT_HEADS];
-    unsigned tops, zs, done[PT_WORKERS];           // tiles whose maxima and normalisers are in, counted by every warp; whose sums are, warp by warp
-};
+constexpr int PT_COUNT = 56;                       // bit of an output sum where its parts are counted: the sum stays within 2^31 2^fa <= 2^54, as the probabilities' does within 2^fa
+
+// What a CTA tells the others of a pair cut between them, one value per head: two words, each half a value and a bit that says that it is there.
+struct TcNote { ulonglong2 head[PT_HEADS]; };
+struct TcNotes { TcNote begins, goes_on; };        // of the pair that begins in a CTA, of the one that began in front of it
 struct TcWork {
     uint32_t *dist;                // [tiles][8 heads][4 quarters][32] distances below the base (shifted, at most the limit): key k of a quarter at (k & 3) 8 + (k >> 2), so that the
                                    // eight keys t, t + 4, .. of a lane lie side by side
     long long *base;               // [tiles][4 quarters][8] largest score of 32 keys
-    unsigned long long *top, *z;   // [pairs][16 warps][8] of pairs that lie in one CTA
-    TcCell *cell;                  // [CTAs]
-    unsigned long long *acc;       // [CTAs][8][hd]
+    unsigned long long *top, *z;   // [pairs][8], [pairs][16 warps][8] of pairs that lie in one CTA
+    TcNotes *notes;                // [2: maxima, normalisers][CTAs]
+    unsigned long long *acc;       // [CTAs][8][hd] output sums of the pair that begins in a CTA, and in bits 56 .. how many parts are in
 };
 __host__ __device__ inline int tc_head_groups(const PagedAttnArgs &a) { return (a.H / a.Hkv + PT_HEADS - 1) / PT_HEADS; }
 __host__ __device__ inline int tc_group_heads(const PagedAttnArgs &a) { const int g = tc_head_groups(a); return (a.H / a.Hkv + g - 1) / g; }
@@ -70,10 +71,10 @@ __host__ __device__ inline TcWork tc_work(const PagedAttnArgs &a, int ctas, size
     w.dist = static_cast<uint32_t *>(a.work);
     w.base = reinterpret_cast<long long *>(w.dist + tiles * PT_KEYS * PT_HEADS);
     w.top = reinterpret_cast<unsigned long long *>(w.base + tiles * 4 * PT_HEADS);
-    w.z = w.top + pairs * PT_WORKERS * PT_HEADS;
-    w.cell = reinterpret_cast<TcCell *>(w.z + pairs * PT_WORKERS * PT_HEADS);
-    w.acc = reinterpret_cast<unsigned long long *>(w.cell + ctas);
-    if (bytes) *bytes = (size_t)tiles * (PT_KEYS * PT_HEADS * 4 + 4 * PT_HEADS * 8) + (size_t)pairs * PT_WORKERS * PT_HEADS * 16 + (size_t)ctas * (sizeof(TcCell) + (size_t)PT_HEADS * a.hd * 8);
+    w.z = w.top + pairs * PT_HEADS;
+    w.notes = reinterpret_cast<TcNotes *>(w.z + pairs * PT_WORKERS * PT_HEADS);
+    w.acc = reinterpret_cast<unsigned long long *>(w.notes + 2 * ctas);
+    if (bytes) *bytes = (size_t)tiles * (PT_KEYS * PT_HEADS * 4 + 4 * PT_HEADS * 8) + (size_t)pairs * (PT_WORKERS + 1) * PT_HEADS * 8 + (size_t)ctas * (2 * sizeof(TcNotes) + (size_t)PT_HEADS * a.hd * 8);
     return w;
 }
 
@@ -85,7 +86,7 @@ __device__ __forceinline__ int tc_tiles(const PagedAttnArgs &a, const PagedSpan 
 
 // A walk over a run of the list, tile by tile.
 struct TcWalk {
-    int owner;                                     // of a cut pair: the CTA whose cell it has
+    int owner, parts;                              // of a cut pair: the CTA where it begins, those that have a part
     int b, pair_of, t, nt, left, tile, part, seg;  // sequence; its pair; tile of the pair, its tiles; tiles left; number in the list; tiles of the pair and of the accumulation before this one
     PagedSpan s;
     __device__ __forceinline__ void load(const PagedAttnArgs &a) { paged_span(a, b, s); nt = tc_tiles(a, s); }
@@ -184,7 +185,7 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
         w.t = piece * size;
         w.left = max(0, min(size, w.nt - w.t));
         w.tile = first[0] + w.pair_of * w.nt + w.t;
-        w.owner = me - piece;
+        w.owner = me - piece; w.parts = (w.nt + size - 1) / size;
         if (w.left > 0) run[w.left == w.nt ? RUN_WHOLE : 0] = w;
     } else if (way == WHOLE_PAIRS) {
         w.pair_of = in[0];
@@ -195,7 +196,7 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
         auto owner = [&](int tile) { return (int)((((uint32_t)tile + 1) * ctas - 1) / total); };
         w.pair_of = in[0] / w.nt; w.t = in[0] - w.pair_of * w.nt;
         w.left = to - from; w.tile = from;
-        w.owner = owner(w.tile - w.t);
+        w.owner = owner(w.tile - w.t); w.parts = owner(w.tile - w.t + w.nt - 1) - w.owner + 1;
         if (w.rest() < w.nt) {
             run[0] = w;
             run[0].left = w.rest();
@@ -205,10 +206,11 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
             e.pair_of = in[1] / e.nt;
             e.left = in[1] - e.pair_of * e.nt + 1;
             e.tile = to - e.left;
-            e.owner = owner(e.tile);
+            e.owner = owner(e.tile); e.parts = owner(e.tile + e.nt - 1) - e.owner + 1;
             if (e.left < e.nt) { run[1] = e; w.left -= e.left; }
             run[RUN_WHOLE] = w;
         }
+        if (me & 1) { const TcWalk x = run[0]; run[0] = run[1]; run[1] = x; }      // two neighbours have the pair between them first, the next two last
     }
 }
 
@@ -235,9 +237,16 @@ __device__ __forceinline__ void tc_ld8(uint32_t addr, int (&r)[8]) {
 __device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap *map, int x, int row, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar) : "memory");
+// Rows are read once: the second-level cache gives their lines up first, and keeps the distances that are written between them and read again
+// (64 x 4096 keys 144 -> 129 us, from a flushed cache 158 -> 149).
+__device__ __forceinline__ uint64_t tc_once() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap *map, int x, int row, uint32_t bar, uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar), "l"(policy) : "memory");
 }
 
 // 128-byte chunks of a row, ring slots, TMEM columns, those of the scores (behind the outputs, or over their second buffer)
@@ -246,9 +255,12 @@ struct TcShape { int chunks, slots, columns, score_at; };
 struct TcBars {
     uint64_t full[PT_MAX_SLOTS], empty[PT_MAX_SLOTS], meta[PT_META];
     uint64_t score_full[PT_SETS], score_free[2], query_full, prob_full[PT_SETS], prob_free[PT_SETS], out_full[2], out_free[2], pair_done, drain;
+    uint64_t part_in[2], known[2];                 // of a cut pair: every warp's maxima, then normalisers; those of all CTAs
     uint32_t tmem;
     int abort;
     TcWalk run[RUNS];
+    unsigned long long part[2][PT_WORKERS][PT_HEADS], top[2][PT_HEADS], z[2][PT_HEADS];     // of the cut pairs
+    unsigned long long pair_top[2][PT_WORKERS][PT_HEADS];      // maxima of a whole pair and of the next
     unsigned char mask[PT_META][PT_GROUPS];
 };
 
@@ -261,6 +273,13 @@ struct TcRing {
 // One thread's wait (tl_wait: a whole warp's, at twice the price).
 __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
     return tl_try(bar, parity) || tl_wait_slow(bar, parity, abort_flag);
+}
+
+// Whether a phase has ended, without a wait; the whole warp's answer.
+__device__ __forceinline__ bool tc_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, ok);
 }
 
 // The two producer warps: the share's tiles into the ring, chunk by chunk in turn, a box per page (or part of one).  A chunk costs a thread 500
@@ -317,6 +336,7 @@ __device__ __forceinline__ bool tc_produce(const PagedAttnArgs &a, TcWalk w, con
     const int lane = threadIdx.x & 31, groups = tc_head_groups(a), per_seq = a.Hkv * groups;
     constexpr uint32_t ALL = IN_BOX == 1 ? 0xFFFFu : 0x5555u;
     if (w.left == 0) return true;
+    const uint64_t once = tc_once();
     int kv = w.pair_of / groups;
     TcLook look = tc_look(a, w, kv, 8 * IN_BOX);
     while (w.left > 0) {
@@ -341,11 +361,11 @@ __device__ __forceinline__ bool tc_produce(const PagedAttnArgs &a, TcWalk w, con
                 tl_expect(bar, x.bytes);
                 if (x.sends == ALL) {
 #pragma unroll
-                    for (int j = 0; j < PT_GROUPS / IN_BOX; j++) tc_tma(to + j * IN_BOX * 1024, map, 32 * c, row[j], bar);
+                    for (int j = 0; j < PT_GROUPS / IN_BOX; j++) tc_tma(to + j * IN_BOX * 1024, map, 32 * c, row[j], bar, once);
                 } else {
 #pragma unroll
                     for (int j = 0; j < PT_GROUPS / IN_BOX; j++)
-                        if ((x.sends >> (j * IN_BOX)) & 1) tc_tma(to + j * IN_BOX * 1024, map, 32 * c, row[j], bar);
+                        if ((x.sends >> (j * IN_BOX)) & 1) tc_tma(to + j * IN_BOX * 1024, map, 32 * c, row[j], bar, once);
                 }
             }
             __syncwarp();
@@ -372,71 +392,126 @@ __device__ __forceinline__ void tc_producer(const PagedAttnArgs &a, const CUtens
 }
 
 // Query columns of one pair: column 8 h + s holds digit s - b of q_i at byte 4 i + b, bytes 0 .. 2 in one operand and byte 3 in the other.
-// A thread takes four dimensions of a head and four columns.
+// A thread rotates one value and writes its word of the eight columns: little code, fetched once and run once, is what counts (a thread with four
+// values and columns, whole 16 bytes at a time, took 2.1 us instead of 1.1).
 __device__ __forceinline__ void tc_queries(const PagedAttnArgs &a, const TcWalk &w, int heads, int padded, unsigned char *lower, unsigned char *upper, int worker) {
-    const int groups = tc_head_groups(a), kv = w.pair_of / groups, h0 = kv * (a.H / a.Hkv) + (w.pair_of % groups) * tc_group_heads(a), quads = a.hd / 4, half = a.hd / 2;
-    const long long pos = w.s.len - 1;
+    const int groups = tc_head_groups(a), kv = w.pair_of / groups, h0 = kv * (a.H / a.Hkv) + (w.pair_of % groups) * tc_group_heads(a), half = a.hd / 2;
+    const int at_once = 32 * PT_WORKERS / a.hd, d = worker % a.hd;
+    int h = worker / a.hd;
+    if (h >= at_once) return;
+    // the pair (x0, x1) that holds dimension d
+    const bool pairs = a.rope == 1, second = pairs ? d & 1 : d >= half;
+    const int i = pairs ? d >> 1 : second ? d - half : d, d0 = pairs ? d & ~1 : i, d1 = pairs ? d | 1 : i + half;
+    const int64_t *q = a.q + (long long)w.b * a.q_ld + (long long)h0 * a.hd;
+    uint64_t c = 0, n = 0, x0 = 0, x1 = 0;
+    auto load = [&](int h) {
+        x0 = x1 = 0;
+        if (h >= heads) return;
+        x0 = (uint64_t)q[h * a.hd + (a.rope ? d0 : d)];
+        if (a.rope) x1 = (uint64_t)q[h * a.hd + d1];
+    };
+    load(h);
+    if (a.rope) { c = (uint64_t)a.cos[(long long)(w.s.len - 1) * half + i]; n = (uint64_t)a.sin[(long long)(w.s.len - 1) * half + i]; }
 #pragma unroll 1
-    for (int task = worker; task < 2 * padded * quads; task += 32 * PT_WORKERS) {
-        const int row = task / quads, j = task - row * quads, d = 4 * j, h = row >> 1, s0 = 4 * (row & 1);
-        int64_t y[4] = {0, 0, 0, 0};
-        if (h < heads) {
-            const int64_t *q = a.q + (long long)w.b * a.q_ld + (long long)(h0 + h) * a.hd;
-            const bool second = a.rope == 2 && d >= half;
-            // pairs (x0, x1): of rope 2 four, each giving one value; else two, each giving both
-            const int i0 = a.rope == 2 ? (second ? d - half : d) : 2 * j;
+    for (; h < padded; h += at_once) {
+        const uint64_t y = a.rope ? (uint64_t)((int64_t)(second ? x0 * n + x1 * c : x0 * c - x1 * n) >> a.fa) : x0;
+        load(h + at_once);
+        const uint64_t v = (y + 0x8080808080808080ULL) ^ 0x8080808080808080ULL;
+        const uint32_t first = __byte_perm((uint32_t)v, 0, 0x0123), last = __byte_perm((uint32_t)(v >> 32), 0, 0x0123);       // first digit on top
+        uint32_t to = (uint32_t)(d >> 5) * (uint32_t)padded * 1024 + (uint32_t)h * 1024 + (uint32_t)(d & 3) * 4;
+        const uint32_t j = (uint32_t)(d >> 2) & 7;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (a.rope == 2) {
-                    int64_t x0 = q[i0 + e], x1 = q[i0 + e + half];
-                    paged_rotate(a.cos, a.sin, 2, a.hd, a.fa, pos, i0 + e, x0, x1);
-                    y[e] = second ? x1 : x0;
-                } else y[e] = q[d + e];
-            }
-            if (a.rope == 1) {
-                paged_rotate(a.cos, a.sin, 1, a.hd, a.fa, pos, i0, y[0], y[1]);
-                paged_rotate(a.cos, a.sin, 1, a.hd, a.fa, pos, i0 + 1, y[2], y[3]);
-            }
-        }
-        uint64_t digits[4];                        // first digit on top
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint64_t v = ((uint64_t)y[e] + 0x8080808080808080ULL) ^ 0x8080808080808080ULL;
-            digits[e] = (uint64_t)__byte_perm((uint32_t)v, 0, 0x0123) << 32 | __byte_perm((uint32_t)(v >> 32), 0, 0x0123);
-        }
-        const uint32_t at = (uint32_t)(j >> 3) * (uint32_t)padded * 1024 + (uint32_t)h * 1024;
-#pragma unroll 1
-        for (int s = s0; s < s0 + 4; s++) {
-            uint32_t x[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = (uint32_t)(digits[e] >> (56 - 8 * s));
-            const uint32_t to = at + (uint32_t)s * 128 + (uint32_t)(((j & 7) ^ s) * 16);
-            *reinterpret_cast<uint4 *>(lower + to) = make_uint4(x[0] & 0xFFFFFFu, x[1] & 0xFFFFFFu, x[2] & 0xFFFFFFu, x[3] & 0xFFFFFFu);
-            *reinterpret_cast<uint4 *>(upper + to) = make_uint4(x[0] & 0xFF000000u, x[1] & 0xFF000000u, x[2] & 0xFF000000u, x[3] & 0xFF000000u);
+        for (uint32_t s = 0; s < 8; s++, to += 128) {
+            const uint32_t x = s < 4 ? first >> (24 - 8 * s) : __funnelshift_r(last, first, 56 - 8 * s);
+            *reinterpret_cast<uint32_t *>(lower + to + (j ^ s) * 16) = x & 0xFFFFFFu;
+            *reinterpret_cast<uint32_t *>(upper + to + (j ^ s) * 16) = x & 0xFF000000u;
         }
     }
 }
 
-// A warp's wait for a count that other CTAs raise: false where it gave up.
-__device__ __forceinline__ bool tc_poll(const unsigned *count, unsigned target, volatile int *abort_flag) {
-    bool done = false;
-    for (unsigned i = 0; i < PT_POLLS && !done && !*abort_flag; i++) {
-        unsigned v;
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
-        done = v == target;
+// One warp: a value per head of a cut pair (in the lanes 0 .. 7) told to the other CTAs, and the largest, or the sum, of what all of them tell.  A value comes with
+// its own word that it is there: nothing waits for a fence, and nobody looks twice.
+__device__ __forceinline__ TcNote *tc_note(TcNotes *notes, int cta, bool begins) { return begins ? &notes[cta].begins : &notes[cta].goes_on; }
+__device__ __forceinline__ void tc_tell(TcNotes *notes, const TcWalk &w, unsigned long long x) {
+    const int lane = threadIdx.x & 31;
+    if (lane < PT_HEADS)
+        asm volatile("st.relaxed.gpu.global.v2.u64 [%0], {%1, %2};" ::"l"(tc_note(notes, blockIdx.x, w.t == 0)->head + lane), "l"(x | 0xFFFFFFFFULL), "l"(x << 32 | 0xFFFFFFFFULL) : "memory");
+}
+template <bool LARGEST>
+__device__ __forceinline__ bool tc_gather(TcNotes *notes, const TcWalk &w, unsigned long long *result, volatile int *abort_flag) {
+    constexpr int DEEP = 8;                        // notes a lane asks for at once
+    const int lane = threadIdx.x & 31, head = lane & 7;
+    unsigned long long sum = 0;
+    for (int c0 = lane >> 3; c0 - (lane >> 3) < w.parts; c0 += 4 * DEEP) {
+        unsigned long long x;
+        bool there = false;
+        for (unsigned i = 0; i < PT_POLLS && !there && !*abort_flag; i++) {
+            there = true;
+            x = 0;
+#pragma unroll
+            for (int u = 0; u < DEEP; u++) {
+                const int c = c0 + 4 * u;
+                if (c >= w.parts) continue;
+                unsigned long long high, low;
+                asm volatile("ld.relaxed.gpu.global.v2.u64 {%0, %1}, [%2];" : "=l"(high), "=l"(low) : "l"(tc_note(notes, w.owner + c, c == 0)->head + head) : "memory");
+                there = there && (uint32_t)high && (uint32_t)low;
+                const unsigned long long y = (high & 0xFFFFFFFF00000000ULL) | low >> 32;
+                x = LARGEST ? max(x, y) : x + y;
+            }
+        }
+        if (!__all_sync(0xffffffffu, there)) { *abort_flag = 1; return false; }
+        sum = LARGEST ? max(sum, x) : sum + x;
     }
-    done = __all_sync(0xffffffffu, done);
-    if (!done) *abort_flag = 1;
-    return done;
+#pragma unroll
+    for (int d = 8; d < 32; d <<= 1) {
+        const unsigned long long o = __shfl_xor_sync(0xffffffffu, sum, d);
+        sum = LARGEST ? max(sum, o) : sum + o;
+    }
+    if (lane < PT_HEADS) result[lane] = sum;
+    __syncwarp();
+    return true;
+}
+// The warp that planned the share, afterwards: what the CTA's warps found about the cut pairs, exchanged.
+__device__ __forceinline__ void tc_exchange(TcBars &s, const TcWork &work, volatile int *abort_flag) {
+    const int lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");      // the notes are clear
+#pragma unroll 1
+    for (int round = 0; round < 2; round++) {      // maxima, normalisers
+        TcNotes *notes = work.notes + round * gridDim.x;
+#pragma unroll 1
+        for (int x = 0; x < RUN_WHOLE; x++) {
+            if (s.run[x].left == 0) continue;
+            if (!tl_wait(tl_u32(&s.part_in[x]), round, abort_flag)) return;
+            unsigned long long v = 0;
+#pragma unroll 4
+            for (int w = lane >> 3; w < PT_WORKERS; w += 4) {
+                const unsigned long long y = s.part[x][w][lane & 7];
+                v = round ? v + y : max(v, y);
+            }
+#pragma unroll
+            for (int d = 8; d < 32; d <<= 1) {
+                const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, d);
+                v = round ? v + o : max(v, o);
+            }
+            tc_tell(notes, s.run[x], v);
+        }
+#pragma unroll 1
+        for (int x = 0; x < RUN_WHOLE; x++) {
+            if (s.run[x].left == 0) continue;
+            if (!(round ? tc_gather<false>(notes, s.run[x], s.z[x], abort_flag) : tc_gather<true>(notes, s.run[x], s.top[x], abort_flag))) return;
+            if (lane == 0) tl_arrive(tl_u32(&s.known[x]));
+        }
+    }
 }
 
-// The cells of pairs that are cut between CTAs, cleared.  The attention's launch overlaps it: what lies in front of this kernel on the stream
-// has ended when the attention's CTAs start, so that only the cells are waited for.
-__global__ void paged_clear_kernel(TcCell *cell, unsigned long long *acc, int per_cta) {
+// What a CTA's cut pairs need, cleared.  The attention's launch overlaps it: what lies in front of this kernel on the stream has ended when the
+// attention's CTAs start, so that only this is waited for.
+__global__ void paged_clear_kernel(TcNotes *notes, unsigned long long *acc, int per_cta) {
     pdl_enter();
     const int tid = threadIdx.x;
-    if (tid < (int)(sizeof(TcCell) / 8)) reinterpret_cast<unsigned long long *>(cell + blockIdx.x)[tid] = 0;
-    for (int i = tid; i < per_cta; i += blockDim.x) acc[(long long)blockIdx.x * per_cta + i] = 0;
+    constexpr int WORDS = 2 * sizeof(TcNotes) / 16;
+    for (int i = tid; i < WORDS; i += blockDim.x) reinterpret_cast<ulonglong2 *>(notes)[(long long)blockIdx.x * WORDS + i] = make_ulonglong2(0, 0);
+    for (int i = tid; i < per_cta / 2; i += blockDim.x) reinterpret_cast<ulonglong2 *>(acc)[(long long)blockIdx.x * (per_cta / 2) + i] = make_ulonglong2(0, 0);
 }
 
 // Exponential of a distance from the row's maximum, at most `limit`, where it is zero (a key that does not count stands there): of the general
@@ -481,14 +556,19 @@ __device__ __noinline__ unsigned long long tc_normalise(const PagedAttnArgs &a, 
         unsigned long long b[DEEP];
 #pragma unroll
         for (int u = 0; u < DEEP; u++) tc_distances(dist, base, min(i + u * PT_SETS, end - 1), d[u], b[u]);
-#pragma unroll
-        for (int u = 0; u < DEEP; u++) {
-            if (i + u * PT_SETS >= end) break;
-            const uint32_t above = (uint32_t)tc_min(top - b[u], a.clip) << Exp::SHIFT;
+#pragma unroll 1
+        for (int u = i; u < min(i + DEEP * PT_SETS, end); u += PT_SETS) {      // (one tile's code, the others' registers moved up: four times the code takes longer to fetch)
+            const uint32_t above = (uint32_t)tc_min(top - b[0], a.clip) << Exp::SHIFT;
             uint32_t sum = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum += tc_weight(exp2, above, d[u][e]);
+            for (int e = 0; e < 8; e++) sum += tc_weight(exp2, above, d[0][e]);
             z += sum;
+#pragma unroll
+            for (int v = 1; v < DEEP; v++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) d[v - 1][e] = d[v][e];
+                b[v - 1] = b[v];
+            }
         }
     }
     __syncwarp();
@@ -520,6 +600,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         }
         for (int i = 0; i < PT_SETS; i++) { tl_init(tl_u32(&s.score_full[i]), 1); tl_init(tl_u32(&s.prob_full[i]), 4); tl_init(tl_u32(&s.prob_free[i]), 1); }
         tl_init(tl_u32(&s.query_full), PT_WORKERS); tl_init(tl_u32(&s.pair_done), PT_WORKERS); tl_init(tl_u32(&s.drain), 1);
+        for (int i = 0; i < 2; i++) { tl_init(tl_u32(&s.part_in[i]), PT_WORKERS); tl_init(tl_u32(&s.known[i]), 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
@@ -606,7 +687,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             }
         }
         __syncwarp();
-    } else if (warp >= PT_FIRST) {
+    } else if (warp == 3) {
+        tc_exchange(s, tc_work(a, gridDim.x), abort_flag);
+    } else {
         const int worker = tid - 32 * PT_FIRST, set = (warp - PT_FIRST) >> 2, quarter = warp & 3, key = quarter * 32 + lane;      // a warp reads TMEM lanes 32 (warp % 4) ..
         const int g = lane >> 2, t = lane & 3;     // beyond the scores a lane has head g, keys t, t + 4, .. of the quarter
         const TcWork work = tc_work(a, gridDim.x);
@@ -618,15 +701,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         };
         // what is left to do with the maxima of a pair (or of its part here) once the next pair's query columns are written, so that the
         // products go on meanwhile: exchange them; a whole pair's normaliser
-        struct { int n = 0, nt, first, index, owner; long long pair; } behind;     // tiles, the pair's; number of the first in the list, and among this CTA's scores
+        struct { int n = 0, nt, first, index, run; long long pair; } behind;       // tiles, the pair's; number of the first in the list, and among this CTA's scores
         long long largest = INT64_MIN;             // lane h: of head h, over this warp's tiles of the pair
         int whole_pairs = 0;
         auto settle = [&](long long most) {
             if (behind.n == 0) return true;
             const unsigned long long biased = (uint64_t)most ^ PT_BIAS;
             if (behind.n == behind.nt) {
-                unsigned long long *const top = work.top + behind.pair * PT_WORKERS * PT_HEADS, *const z = work.z + behind.pair * PT_WORKERS * PT_HEADS + 4 * set * PT_HEADS + quarter * PT_HEADS;
-                if (lane < PT_HEADS) top[(4 * set + quarter) * PT_HEADS + lane] = biased;
+                unsigned long long (&tops)[PT_WORKERS][PT_HEADS] = s.pair_top[whole_pairs & 1];
+                if (lane < PT_HEADS) tops[4 * set + quarter][lane] = biased;
                 __syncwarp();
                 if (lane == 0) tl_arrive(tl_u32(&s.pair_done));
                 __syncwarp();
@@ -634,20 +717,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 whole_pairs++;
                 unsigned long long m = 0;          // over the warps: four for each of a head's lanes
 #pragma unroll
-                for (int w = 0; w < 4; w++) m = max(m, __ldcg(top + (4 * t + w) * PT_HEADS + g));
+                for (int w = 0; w < 4; w++) m = max(m, tops[4 * t + w][g]);
                 m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 const unsigned long long sum = normalise(behind.first, behind.n, (set - behind.index) & 3, m);
-                if (t == 0) z[g] = sum;
+                if (t == 0) work.z[(behind.pair * PT_WORKERS + 4 * set + quarter) * PT_HEADS + g] = sum;
+                if (t == 0 && set + quarter == 0) work.top[behind.pair * PT_HEADS + g] = m;
             } else {
-                asm volatile("griddepcontrol.wait;" ::: "memory");      // the cells are clear
-                TcCell *cell = work.cell + behind.owner;
-                if (lane < heads_most) atomicMax(cell->top + lane, biased);
-                __threadfence();
+                if (lane < PT_HEADS) s.part[behind.run][4 * set + quarter][lane] = biased;
                 __syncwarp();
-                if (lane == 0) atomicAdd(&cell->tops, (unsigned)behind.n);
+                if (lane == 0) tl_arrive(tl_u32(&s.part_in[behind.run]));
             }
             behind.n = 0;
+            return true;
+        };
+        // normalisers of the pairs that go on in other CTAs, once everybody's maxima are in: some tiles at a time, behind those whose scores are read out
+        struct { int run = 0, done = 0, index = 0; unsigned long long z = 0; } cut;          // tiles of the run that are in z; the run's place among this CTA's scores
+        auto advance = [&](bool patient) {
+            const int x = cut.run, n = s.run[x].left;
+            if (cut.done < n) {
+                if (cut.done == 0) {
+                    if (patient ? !tl_wait(tl_u32(&s.known[x]), 0, abort_flag) : !tc_test(tl_u32(&s.known[x]), 0)) return !patient;
+                }
+                const int m = patient ? n - cut.done : min(n - cut.done, 4 * PT_SETS);
+                cut.z += normalise(s.run[x].tile + cut.done, m, (set - cut.index - cut.done) & 3, s.top[x][g]);
+                cut.done += m;
+                if (cut.done < n) return true;
+                if (t == 0) s.part[x][4 * set + quarter][g] = cut.z;
+                __syncwarp();
+                if (lane == 0) tl_arrive(tl_u32(&s.part_in[x]));
+                cut.z = 0;
+            }
+            cut.run++; cut.index += n; cut.done = 0;
             return true;
         };
         for (int x = worker; x < (int)(PT_SETS * PT_PROBS / 16); x += 32 * PT_WORKERS) reinterpret_cast<uint4 *>(probs)[x] = make_uint4(0, 0, 0, 0);      // (the columns beyond 24 stay so)
@@ -703,9 +804,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                     if (lane == 0) tl_arrive(tl_u32(&s.score_free[i & 1]));
                     if (lane < PT_HEADS) work.base[((long long)v.tile * 4 + quarter) * PT_HEADS + lane] = base;
                     largest = max(largest, base);
+                    if (cut.run < u) advance(false);
                 }
                 if (v.ends_part()) {
-                    behind.n = v.part + 1; behind.nt = v.nt; behind.first = v.tile - v.t; behind.index = i - v.part; behind.owner = v.owner;
+                    behind.n = v.part + 1; behind.nt = v.nt; behind.first = v.tile - v.t; behind.index = i - v.part; behind.run = u;
                     behind.pair = (long long)v.b * per_seq + v.pair_of;
                 }
                 fresh = v.t + 1 == v.nt;
@@ -714,20 +816,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         }
         __syncwarp();
         ok = ok && settle(largest);
-        // ---- normalisers of the pairs that go on in other CTAs, once everybody's maxima are in ---------------------------------------
-        for (int x = 0, index = 0; ok && x < RUN_WHOLE; x++) {
-            const int n = s.run[x].left;
-            if (n == 0) continue;
-            TcCell *cell = work.cell + s.run[x].owner;
-            ok = tc_poll(&cell->tops, (unsigned)s.run[x].nt * PT_WORKERS, abort_flag);
-            if (!ok) break;
-            const unsigned long long z = normalise(s.run[x].tile, n, (set - index) & 3, __ldcg(cell->top + g));
-            if (t == 0 && g < heads_most) atomicAdd(cell->z + g, z);
-            __threadfence();
-            __syncwarp();
-            if (lane == 0) atomicAdd(&cell->zs, (unsigned)n);
-            index += n;
-        }
+        while (ok && cut.run < RUN_WHOLE) ok = advance(true);
         asm volatile("griddepcontrol.wait;" ::: "memory");      // (whatever the share: what is launched behind counts on it)
         // ---- probabilities and values ---------------------------------------------------------------------------------------------
         if (ok) {                                  // what the CTA's warps left in memory
@@ -738,12 +827,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         Quotient quotient(0, a.fa);                // of head g
         unsigned long long top = 0, carry[2] = {0, 0};                     // of head g; output sums of earlier accumulations
         int seg = 0;
-        struct { int tiles = 0, nt, owner, heads; bool ends; int64_t *out; } pending;      // sums to read out: tiles of the pair in them (and in `carry`)
+        struct { int tiles = 0, nt, owner, parts, heads; bool ends; int64_t *out; } pending;      // sums to read out: tiles of the pair in them (and in `carry`)
         auto read_out = [&]() {
             if (!tl_wait(tl_u32(&s.out_full[seg & 1]), (seg >> 1) & 1, abort_flag)) return false;
             tc_after();
             const int byte = lane & 3, d = 32 * set + 8 * quarter + (lane >> 2), h0 = 4 * (byte >> 1) + 2 * (byte & 1);
-            const bool whole = pending.tiles == pending.nt, joins = pending.ends && !whole;
+            const bool whole = pending.tiles == pending.nt;
             unsigned long long *acc = work.acc + (long long)pending.owner * PT_HEADS * a.hd;
             if (set < sh.chunks) {                 // dimensions 32 set ..
                 const uint32_t from = tmem + (seg & 1) * buffer + ((uint32_t)(quarter * 32) << 16) + 2 * set * 32;
@@ -775,25 +864,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     if (!pending.ends || h0 + h >= pending.heads) continue;
-                    if (whole) pending.out[(long long)(h0 + h) * a.hd + d] = (int64_t)carry[h] >> a.fa;
-                    else atomicAdd(acc + (h0 + h) * a.hd + d, carry[h]);
+                    if (!whole) {                  // added up in memory: who adds the last part finds the sum
+                        const unsigned long long part = carry[h] + (1ULL << PT_COUNT), all = atomicAdd(acc + (h0 + h) * a.hd + d, part) + part, parts = (all + (1ULL << (PT_COUNT - 1))) >> PT_COUNT;
+                        if (((parts ^ pending.parts) & 0xFF) != 0) continue;
+                        carry[h] = all - (parts << PT_COUNT);
+                    }
+                    pending.out[(long long)(h0 + h) * a.hd + d] = (int64_t)carry[h] >> a.fa;
                 }
             }
             tc_before();
             __syncwarp();
             if (lane == 0) tl_arrive(tl_u32(&s.out_free[seg & 1]));
             if (pending.ends) carry[0] = carry[1] = 0;
-            if (joins && set < sh.chunks) {        // the last of the CTAs writes out what this warp and its likes have added up
-                __threadfence();
-                __syncwarp();
-                unsigned before = 0;
-                if (lane == 0) before = atomicAdd(&work.cell[pending.owner].done[4 * set + quarter], (unsigned)pending.tiles);
-                before = __shfl_sync(0xffffffffu, before, 0);
-                if (before + pending.tiles == (unsigned)pending.nt) {
-                    __threadfence();
-                    for (int h = h0; h < min(h0 + 2, pending.heads); h++) pending.out[(long long)h * a.hd + d] = (int64_t)__ldcg(acc + h * a.hd + d) >> a.fa;
-                }
-            }
             pending.tiles = 0;
             seg++;
             return true;
@@ -807,15 +889,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 unsigned long long z = 0;
                 top = 0;
                 if (v.t == 0 && v.rest() == v.nt) {
-                    const long long at = ((long long)v.b * per_seq + v.pair_of) * PT_WORKERS * PT_HEADS + g;
+                    const long long pair = (long long)v.b * per_seq + v.pair_of;
+                    top = __ldcg(work.top + pair * PT_HEADS + g);
 #pragma unroll
-                    for (int w = 0; w < 4; w++) { top = max(top, __ldcg(work.top + at + (4 * t + w) * PT_HEADS)); z += __ldcg(work.z + at + (4 * t + w) * PT_HEADS); }
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1)); z += __shfl_xor_sync(0xffffffffu, z, 1);
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2)); z += __shfl_xor_sync(0xffffffffu, z, 2);
+                    for (int w = 0; w < 4; w++) z += __ldcg(work.z + (pair * PT_WORKERS + 4 * t + w) * PT_HEADS + g);
+                    z += __shfl_xor_sync(0xffffffffu, z, 1);
+                    z += __shfl_xor_sync(0xffffffffu, z, 2);
                 } else {
-                    TcCell *cell = work.cell + v.owner;
-                    if (!tc_poll(&cell->zs, (unsigned)v.nt * PT_WORKERS, abort_flag)) { ok = false; break; }
-                    top = __ldcg(cell->top + g); z = __ldcg(cell->z + g);
+                    if (!tl_wait(tl_u32(&s.known[run]), 1, abort_flag)) { ok = false; break; }
+                    top = s.top[run][g]; z = s.z[run][g];
                 }
                 quotient = Quotient(g < heads_most ? z : 0, a.fa);
             }
@@ -843,7 +925,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             if (v.ends_segment()) {
                 if (pending.tiles && !read_out()) { ok = false; break; }
                 const int group = v.pair_of % groups, kv = v.pair_of / groups;
-                pending.tiles = v.part + 1; pending.nt = v.nt; pending.ends = v.ends_part(); pending.owner = v.owner;
+                pending.tiles = v.part + 1; pending.nt = v.nt; pending.ends = v.ends_part(); pending.owner = v.owner; pending.parts = v.parts;
                 pending.heads = min(heads_most, a.H / a.Hkv - group * heads_most);
                 pending.out = a.out + ((long long)v.b * a.H + kv * (a.H / a.Hkv) + group * heads_most) * a.hd;
             }
@@ -906,7 +988,7 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     const long long most = (long long)a.B * a.Hkv * tc_head_groups(a) * tc_tiles_most(a);
     const unsigned ctas = (unsigned)std::min<long long>(std::min(sms, PT_MOST_CTAS), std::max<long long>(1, most));
     const TcWork w = tc_work(a, (int)ctas);
-    e = launch_behind(paged_clear_kernel, ctas, 128, 0, s, w.cell, w.acc, PT_HEADS * a.hd);
+    e = launch_behind(paged_clear_kernel, ctas, 128, 0, s, w.notes, w.acc, PT_HEADS * a.hd);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(PT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
