@@ -49,9 +49,9 @@ constexpr int PT_COUNT = 56;                       // bit of an output sum where
 struct TcNote { ulonglong2 head[PT_HEADS]; };
 struct TcNotes { TcNote begins, goes_on; };        // of the pair that begins in a CTA, of the one that began in front of it
 struct TcWork {
-    uint32_t *dist;                // [tiles][8 heads][4 quarters][32] distances below the base (shifted, at most the limit): key k of a quarter at (k & 3) 8 + (k >> 2), so that the
-                                   // eight keys t, t + 4, .. of a lane lie side by side
-    long long *base;               // [tiles][4 quarters][8] largest score of 32 keys
+    uint32_t *dist;                // [tiles][N heads, 4 or 8][4 quarters][32] distances below the base (shifted, at most the limit): key k of a quarter at k % (32 / N) N + k / (32 / N), so
+                                   // that the N keys of a lane lie side by side
+    long long *base;               // [tiles][4 quarters][N] largest score of 32 keys
     unsigned long long *top, *z;   // [pairs][8], [pairs][16 warps][8] of pairs that lie in one CTA
     TcNotes *notes;                // [2: maxima, normalisers][CTAs]
     unsigned long long *acc;       // [CTAs][8][hd] output sums of the pair that begins in a CTA, and in bits 56 .. how many parts are in
@@ -65,16 +65,19 @@ __host__ __device__ inline long long tc_tiles_most(const PagedAttnArgs &a) {
     if (a.n_sel > 0) return ((long long)a.n_sel * a.P + PT_KEYS - 1) / PT_KEYS;
     return (a.max_slots + 2 * tc_box(a) + PT_KEYS - 1) / PT_KEYS;
 }
+// heads that warps are laid out for
+__host__ __device__ inline int tc_room(const PagedAttnArgs &a) { return tc_group_heads(a) <= 4 ? 4 : 8; }
 __host__ __device__ inline TcWork tc_work(const PagedAttnArgs &a, int ctas, size_t *bytes = nullptr) {
     const long long pairs = (long long)a.B * a.Hkv * tc_head_groups(a), tiles = pairs * tc_tiles_most(a);
+    const int room = tc_room(a);
     TcWork w;
     w.dist = static_cast<uint32_t *>(a.work);
-    w.base = reinterpret_cast<long long *>(w.dist + tiles * PT_KEYS * PT_HEADS);
-    w.top = reinterpret_cast<unsigned long long *>(w.base + tiles * 4 * PT_HEADS);
+    w.base = reinterpret_cast<long long *>(w.dist + tiles * PT_KEYS * room);
+    w.top = reinterpret_cast<unsigned long long *>(w.base + tiles * 4 * room);
     w.z = w.top + pairs * PT_HEADS;
     w.notes = reinterpret_cast<TcNotes *>(w.z + pairs * PT_WORKERS * PT_HEADS);
     w.acc = reinterpret_cast<unsigned long long *>(w.notes + 2 * ctas);
-    if (bytes) *bytes = (size_t)tiles * (PT_KEYS * PT_HEADS * 4 + 4 * PT_HEADS * 8) + (size_t)pairs * (PT_WORKERS + 1) * PT_HEADS * 8 + (size_t)ctas * (2 * sizeof(TcNotes) + (size_t)PT_HEADS * a.hd * 8);
+    if (bytes) *bytes = (size_t)tiles * room * (PT_KEYS * 4 + 4 * 8) + (size_t)pairs * (PT_WORKERS + 1) * PT_HEADS * 8 + (size_t)ctas * (2 * sizeof(TcNotes) + (size_t)PT_HEADS * a.hd * 8);
     return w;
 }
 
@@ -534,50 +537,56 @@ struct TcExp16 {
     }
 };
 
-// Distances of a lane's eight keys in one tile and the base they lie below; dist, base: of the lane in tile 0.
-__device__ __forceinline__ void tc_distances(const uint32_t *dist, const long long *base, int tile, uint32_t (&d)[8], unsigned long long &biased) {
-    const uint4 *from = reinterpret_cast<const uint4 *>(dist + (long long)tile * (PT_HEADS * PT_KEYS));
-    const uint4 x = from[0], y = from[1];          // (the CTA's own: its SM's cache may hold them)
-    d[0] = x.x; d[1] = x.y; d[2] = x.z; d[3] = x.w; d[4] = y.x; d[5] = y.y; d[6] = y.z; d[7] = y.w;
-    biased = (uint64_t)base[(long long)tile * 4 * PT_HEADS] ^ PT_BIAS;
+// Distances of a lane's N keys in one tile and the base they lie below; dist, base: of the lane in tile 0.
+template <int N>
+__device__ __forceinline__ void tc_distances(const uint32_t *dist, const long long *base, int tile, uint32_t (&d)[N], unsigned long long &biased) {
+    const uint4 *from = reinterpret_cast<const uint4 *>(dist + (long long)tile * (N * PT_KEYS));
+#pragma unroll
+    for (int i = 0; i < N / 4; i++) {              // (the CTA's own: its SM's cache may hold them)
+        const uint4 x = from[i];
+        d[4 * i] = x.x; d[4 * i + 1] = x.y; d[4 * i + 2] = x.z; d[4 * i + 3] = x.w;
+    }
+    biased = (uint64_t)base[(long long)tile * 4 * N] ^ PT_BIAS;
 }
 // exponential of a key `d` below a base that lies `above` below the pair's largest score, both at most the limit
 template <class Exp>
 __device__ __forceinline__ uint32_t tc_weight(const Exp &exp2, uint32_t above, uint32_t d) { return exp2(min(above + d, exp2.limit)); }
-// Sum of a head's exponentials over every fourth tile from `first` to `end`, the four lanes' keys of a quarter.  A function of its own: inlined at each
+// Sum of a head's exponentials over every fourth tile from `first` to `end`, the keys of a quarter.  A function of its own: inlined at each
 // call its code, fetched once for every use, took longer than its work.
-template <class Exp>
+template <class Exp, int N>
 __device__ __noinline__ unsigned long long tc_normalise(const PagedAttnArgs &a, const uint32_t *dist, const long long *base, int first, int end, unsigned long long top) {
     constexpr int DEEP = 4;                        // tiles asked for at once: behind the rows that stream in a load takes microseconds
     const Exp exp2(a);
     unsigned long long z = 0;
     for (int i = first; i < end; i += DEEP * PT_SETS) {
-        uint32_t d[DEEP][8];
+        uint32_t d[DEEP][N];
         unsigned long long b[DEEP];
 #pragma unroll
-        for (int u = 0; u < DEEP; u++) tc_distances(dist, base, min(i + u * PT_SETS, end - 1), d[u], b[u]);
+        for (int u = 0; u < DEEP; u++) tc_distances<N>(dist, base, min(i + u * PT_SETS, end - 1), d[u], b[u]);
 #pragma unroll 1
         for (int u = i; u < min(i + DEEP * PT_SETS, end); u += PT_SETS) {      // (one tile's code, the others' registers moved up: four times the code takes longer to fetch)
             const uint32_t above = (uint32_t)tc_min(top - b[0], a.clip) << Exp::SHIFT;
             uint32_t sum = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum += tc_weight(exp2, above, d[0][e]);
+            for (int e = 0; e < N; e++) sum += tc_weight(exp2, above, d[0][e]);
             z += sum;
 #pragma unroll
             for (int v = 1; v < DEEP; v++) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) d[v - 1][e] = d[v][e];
+                for (int e = 0; e < N; e++) d[v - 1][e] = d[v][e];
                 b[v - 1] = b[v];
             }
         }
     }
     __syncwarp();
-    z += __shfl_xor_sync(0xffffffffu, z, 1);
-    z += __shfl_xor_sync(0xffffffffu, z, 2);
-    return z;                                      // the same in the head's four lanes
+#pragma unroll
+    for (int d = 1; d < 32 / N; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+    return z;                                      // the same in all lanes of the head
 }
 
-template <bool AT16, bool SMALL>                   // AT16: fa = 16; SMALL: beside that every sum of exponentials at most 2^31
+// AT16: fa = 16; SMALL: beside that every sum of exponentials at most 2^31; N: heads that a warp's lanes are dealt to, and keys of a lane (of four heads in a layout
+// for eight, half of the lanes' exponentials would be for nothing)
+template <bool AT16, bool SMALL, int N>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcShape sh) {
     using Exp = std::conditional_t<AT16, TcExp16, TcExp>;
     using Quotient = std::conditional_t<SMALL, SoftmaxQuotient16, SoftmaxQuotient>;
@@ -691,13 +700,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         tc_exchange(s, tc_work(a, gridDim.x), abort_flag);
     } else {
         const int worker = tid - 32 * PT_FIRST, set = (warp - PT_FIRST) >> 2, quarter = warp & 3, key = quarter * 32 + lane;      // a warp reads TMEM lanes 32 (warp % 4) ..
-        const int g = lane >> 2, t = lane & 3;     // beyond the scores a lane has head g, keys t, t + 4, .. of the quarter
+        constexpr int LANES = 32 / N;              // of a head
+        const int g = lane / LANES, t = lane % LANES;        // beyond the scores a lane has head g, keys t, t + LANES, .. of the quarter
         const TcWork work = tc_work(a, gridDim.x);
         const Exp exp2(a);
         bool ok = true;
         // sum of the exponentials of head g over those of n tiles from `first` on that this warp has read out: the first of them is `skip` on
         auto normalise = [&](int first, int n, int skip, unsigned long long top) {
-            return tc_normalise<Exp>(a, work.dist + g * PT_KEYS + quarter * 32 + 8 * t, work.base + quarter * PT_HEADS + g, first + skip, g < heads_most ? first + n : first, top);
+            return tc_normalise<Exp, N>(a, work.dist + g * PT_KEYS + quarter * 32 + N * t, work.base + quarter * N + g, first + skip, g < heads_most ? first + n : first, top);
         };
         // what is left to do with the maxima of a pair (or of its part here) once the next pair's query columns are written, so that the
         // products go on meanwhile: exchange them; a whole pair's normaliser
@@ -715,11 +725,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 __syncwarp();
                 if (!tl_wait(tl_u32(&s.pair_done), whole_pairs & 1, abort_flag)) return false;
                 whole_pairs++;
-                unsigned long long m = 0;          // over the warps: four for each of a head's lanes
+                unsigned long long m = 0;          // over the warps: some for each of a head's lanes
 #pragma unroll
-                for (int w = 0; w < 4; w++) m = max(m, tops[4 * t + w][g]);
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                for (int w = 0; w < PT_WORKERS / LANES; w++) m = max(m, tops[LANES * w + t][g]);
+#pragma unroll
+                for (int d = 1; d < LANES; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
                 const unsigned long long sum = normalise(behind.first, behind.n, (set - behind.index) & 3, m);
                 if (t == 0) work.z[(behind.pair * PT_WORKERS + 4 * set + quarter) * PT_HEADS + g] = sum;
                 if (t == 0 && set + quarter == 0) work.top[behind.pair * PT_HEADS + g] = m;
@@ -780,7 +790,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                     if (!tl_wait(tl_u32(&s.score_full[set]), (i / PT_SETS) & 1, abort_flag)) { ok = false; break; }
                     tc_after();
                     const uint32_t from = score_at + ((uint32_t)(quarter * 32) << 16) + (i & 1) * 64;
-                    uint32_t *to = work.dist + (long long)v.tile * PT_HEADS * PT_KEYS + quarter * 32 + (lane & 3) * 8 + (lane >> 2);
+                    uint32_t *to = work.dist + (long long)v.tile * N * PT_KEYS + quarter * 32 + lane % LANES * N + lane / LANES;
                     long long base = INT64_MIN;
 #pragma unroll 2
                     for (int h = 0; h < heads_most; h++) {
@@ -802,7 +812,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                     tc_before();
                     __syncwarp();
                     if (lane == 0) tl_arrive(tl_u32(&s.score_free[i & 1]));
-                    if (lane < PT_HEADS) work.base[((long long)v.tile * 4 + quarter) * PT_HEADS + lane] = base;
+                    if (lane < N) work.base[((long long)v.tile * 4 + quarter) * N + lane] = base;
                     largest = max(largest, base);
                     if (cut.run < u) advance(false);
                 }
@@ -825,44 +835,45 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             ok = tl_wait(tl_u32(&s.pair_done), whole_pairs & 1, abort_flag);
         }
         Quotient quotient(0, a.fa);                // of head g
-        unsigned long long top = 0, carry[2] = {0, 0};                     // of head g; output sums of earlier accumulations
+        constexpr int HELD = N / 4;                // heads of a lane in the sums
+        unsigned long long top = 0, carry[HELD] = {};                     // of head g; output sums of earlier accumulations
         int seg = 0;
         struct { int tiles = 0, nt, owner, parts, heads; bool ends; int64_t *out; } pending;      // sums to read out: tiles of the pair in them (and in `carry`)
         auto read_out = [&]() {
             if (!tl_wait(tl_u32(&s.out_full[seg & 1]), (seg >> 1) & 1, abort_flag)) return false;
             tc_after();
-            const int byte = lane & 3, d = 32 * set + 8 * quarter + (lane >> 2), h0 = 4 * (byte >> 1) + 2 * (byte & 1);
+            const int byte = lane & 3, d = 32 * set + 8 * quarter + (lane >> 2), h0 = HELD * byte;
             const bool whole = pending.tiles == pending.nt;
             unsigned long long *acc = work.acc + (long long)pending.owner * PT_HEADS * a.hd;
             if (set < sh.chunks) {                 // dimensions 32 set ..
                 const uint32_t from = tmem + (seg & 1) * buffer + ((uint32_t)(quarter * 32) << 16) + 2 * set * 32;
-                uint64_t sum[PT_HEADS];
+                uint64_t sum[N];
 #pragma unroll
-                for (int h = 0; h < PT_HEADS; h++) sum[h] = 0;
+                for (int h = 0; h < N; h++) sum[h] = 0;
 #pragma unroll
                 for (int part = 0; part < 3; part++) {
                     int x[8], y[8];
                     tc_ld8(from + 8 * part, x); tc_ld8(from + 32 + 8 * part, y);
                     tc_ld_wait();
 #pragma unroll
-                    for (int h = 0; h < PT_HEADS; h++) sum[h] += (uint64_t)(int64_t)(byte == 3 ? y[h] : x[h]) << (8 * part);
+                    for (int h = 0; h < N; h++) sum[h] += (uint64_t)(int64_t)(byte == 3 ? y[h] : x[h]) << (8 * part);
                 }
-                // four lanes hold a dimension's four bytes: two exchanges leave a lane with two heads
+                // four lanes hold a dimension's four bytes: two exchanges leave a lane with a quarter of the heads
                 const bool high = byte & 2, odd = byte & 1;
 #pragma unroll
-                for (int h = 0; h < PT_HEADS; h++) sum[h] <<= 8 * byte;
+                for (int h = 0; h < N; h++) sum[h] <<= 8 * byte;
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    const uint64_t give = high ? sum[h] : sum[h + 4];
-                    sum[h] = (high ? sum[h + 4] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 2);
+                for (int h = 0; h < 2 * HELD; h++) {
+                    const uint64_t give = high ? sum[h] : sum[h + 2 * HELD];
+                    sum[h] = (high ? sum[h + 2 * HELD] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 2);
                 }
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint64_t give = odd ? sum[h] : sum[h + 2];
-                    carry[h] += (odd ? sum[h + 2] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 1);
+                for (int h = 0; h < HELD; h++) {
+                    const uint64_t give = odd ? sum[h] : sum[h + HELD];
+                    carry[h] += (odd ? sum[h + HELD] : sum[h]) + __shfl_xor_sync(0xffffffffu, give, 1);
                 }
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < HELD; h++) {
                     if (!pending.ends || h0 + h >= pending.heads) continue;
                     if (!whole) {                  // added up in memory: who adds the last part finds the sum
                         const unsigned long long part = carry[h] + (1ULL << PT_COUNT), all = atomicAdd(acc + (h0 + h) * a.hd + d, part) + part, parts = (all + (1ULL << (PT_COUNT - 1))) >> PT_COUNT;
@@ -875,7 +886,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             tc_before();
             __syncwarp();
             if (lane == 0) tl_arrive(tl_u32(&s.out_free[seg & 1]));
-            if (pending.ends) carry[0] = carry[1] = 0;
+            if (pending.ends)
+                for (int h = 0; h < HELD; h++) carry[h] = 0;
             pending.tiles = 0;
             seg++;
             return true;
@@ -892,9 +904,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                     const long long pair = (long long)v.b * per_seq + v.pair_of;
                     top = __ldcg(work.top + pair * PT_HEADS + g);
 #pragma unroll
-                    for (int w = 0; w < 4; w++) z += __ldcg(work.z + (pair * PT_WORKERS + 4 * t + w) * PT_HEADS + g);
-                    z += __shfl_xor_sync(0xffffffffu, z, 1);
-                    z += __shfl_xor_sync(0xffffffffu, z, 2);
+                    for (int w = 0; w < PT_WORKERS / LANES; w++) z += __ldcg(work.z + (pair * PT_WORKERS + LANES * w + t) * PT_HEADS + g);
+#pragma unroll
+                    for (int d = 1; d < LANES; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
                 } else {
                     if (!tl_wait(tl_u32(&s.known[run]), 1, abort_flag)) { ok = false; break; }
                     top = s.top[run][g]; z = s.z[run][g];
@@ -902,19 +914,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 quotient = Quotient(g < heads_most ? z : 0, a.fa);
             }
             if (i % PT_SETS == set) {
-                uint32_t p[8];
+                uint32_t p[N];
                 unsigned long long base;
-                tc_distances(work.dist + g * PT_KEYS + quarter * 32 + 8 * t, work.base + quarter * PT_HEADS + g, v.tile, p, base);
+                tc_distances<N>(work.dist + g * PT_KEYS + quarter * 32 + N * t, work.base + quarter * N + g, v.tile, p, base);
                 const uint32_t above = (uint32_t)tc_min(top - base, a.clip) << Exp::SHIFT;
 #pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = g < heads_most ? (uint32_t)quotient(tc_weight(exp2, above, p[e])) : 0u;
+                for (int e = 0; e < N; e++) p[e] = g < heads_most ? (uint32_t)quotient(tc_weight(exp2, above, p[e])) : 0u;
                 if (i >= PT_SETS && !tl_wait(tl_u32(&s.prob_free[set]), ((i / PT_SETS) & 1) ^ 1, abort_flag)) { ok = false; break; }
                 unsigned char *to = probs + set * PT_PROBS + (quarter * 32 + t) * 32 + g;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {      // key t + 4 e: byte b at 8 b + g, the halves of 32 bytes swapped in every second group of four rows
-                    to[128 * e + (e & 1) * 16] = (unsigned char)p[e];
-                    to[128 * e + 8 + (e & 1) * 16] = (unsigned char)(p[e] >> 8);
-                    to[128 * e + 16 - (e & 1) * 16] = (unsigned char)(p[e] >> 16);
+                for (int e = 0; e < N; e++) {      // key t + LANES e: byte b at 8 b + g, the halves of 32 bytes swapped in every second group of four rows
+                    const int at = LANES * 32 * e, swap = (((t + LANES * e) >> 2) & 1) * 16;
+                    to[at + swap] = (unsigned char)p[e];
+                    to[at + 8 + swap] = (unsigned char)(p[e] >> 8);
+                    to[at + 16 - swap] = (unsigned char)(p[e] >> 16);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -962,7 +975,7 @@ int tc_sms(int device) {
 }
 constexpr int PT_MOST_CTAS = 256;                  // cells in the scratch
 
-template <bool AT16, bool SMALL>
+template <bool AT16, bool SMALL, int N>
 cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     CUtensorMap kmap, vmap;
     if (!tl_encode() || !tc_map(&kmap, a.kpages, a) || !tc_map(&vmap, a.vpages, a)) return cudaErrorInvalidValue;
@@ -980,7 +993,7 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     static std::atomic<unsigned long long> configured;             // devices, a bit each
     const unsigned long long bit = device < 64 ? 1ULL << device : 0;
     if (!(configured & bit)) {
-        e = cudaFuncSetAttribute(paged_attn_kernel<AT16, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(room));
+        e = cudaFuncSetAttribute(paged_attn_kernel<AT16, SMALL, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(room));
         if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_clear_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);      // else the attention waits for idle SMs
         if (e != cudaSuccess) return e;
         configured |= bit;
@@ -996,7 +1009,7 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     attr[0].id = cudaLaunchAttributeCooperative; attr[0].val.cooperative = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<AT16, SMALL>, a, kmap, vmap, sh);
+    e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<AT16, SMALL, N>, a, kmap, vmap, sh);
     note_launch(2);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -1014,8 +1027,9 @@ size_t paged_tc_bytes(const PagedAttnArgs &a) {
     return n;
 }
 cudaError_t launch_paged_tc(const PagedAttnArgs &a, cudaStream_t s) {
-    if (a.fa != 16) return launch_tc<false, false>(a, s);
-    return a.max_slots <= 1LL << 15 ? launch_tc<true, true>(a, s) : launch_tc<true, false>(a, s);
+    const bool at16 = a.fa == 16, small = a.max_slots <= 1LL << 15;
+    if (tc_room(a) == 4) return !at16 ? launch_tc<false, false, 4>(a, s) : small ? launch_tc<true, true, 4>(a, s) : launch_tc<true, false, 4>(a, s);
+    return !at16 ? launch_tc<false, false, 8>(a, s) : small ? launch_tc<true, true, 8>(a, s) : launch_tc<true, false, 8>(a, s);
 }
 
 }  // namespace iie
