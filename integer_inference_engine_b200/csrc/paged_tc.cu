@@ -213,7 +213,6 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
             if (e.left < e.nt) { run[1] = e; w.left -= e.left; }
             run[RUN_WHOLE] = w;
         }
-        if (me & 1) { const TcWalk x = run[0]; run[0] = run[1]; run[1] = x; }      // two neighbours have the pair between them first, the next two last
     }
 }
 
@@ -276,13 +275,6 @@ struct TcRing {
 // One thread's wait (tl_wait: a whole warp's, at twice the price).
 __device__ __forceinline__ bool tc_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
     return tl_try(bar, parity) || tl_wait_slow(bar, parity, abort_flag);
-}
-
-// Whether a phase has ended, without a wait; the whole warp's answer.
-__device__ __forceinline__ bool tc_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return __all_sync(0xffffffffu, ok);
 }
 
 // The two producer warps: the share's tiles into the ring, chunk by chunk in turn, a box per page (or part of one).  A chunk costs a thread 500
@@ -555,28 +547,17 @@ __device__ __forceinline__ uint32_t tc_weight(const Exp &exp2, uint32_t above, u
 // call its code, fetched once for every use, took longer than its work.
 template <class Exp, int N>
 __device__ __noinline__ unsigned long long tc_normalise(const PagedAttnArgs &a, const uint32_t *dist, const long long *base, int first, int end, unsigned long long top) {
-    constexpr int DEEP = 4;                        // tiles asked for at once: behind the rows that stream in a load takes microseconds
     const Exp exp2(a);
     unsigned long long z = 0;
-    for (int i = first; i < end; i += DEEP * PT_SETS) {
-        uint32_t d[DEEP][N];
-        unsigned long long b[DEEP];
-#pragma unroll
-        for (int u = 0; u < DEEP; u++) tc_distances<N>(dist, base, min(i + u * PT_SETS, end - 1), d[u], b[u]);
 #pragma unroll 1
-        for (int u = i; u < min(i + DEEP * PT_SETS, end); u += PT_SETS) {      // (one tile's code, the others' registers moved up: four times the code takes longer to fetch)
-            const uint32_t above = (uint32_t)tc_min(top - b[0], a.clip) << Exp::SHIFT;
-            uint32_t sum = 0;
+    for (int i = first; i < end; i += PT_SETS) {   // (two or four tiles' loads at once: registers that the rest of the kernel lacks, 64 x 4096 keys 128 instead of 122 us)
+        uint32_t d[N], sum = 0;
+        unsigned long long b;
+        tc_distances<N>(dist, base, i, d, b);
+        const uint32_t above = (uint32_t)tc_min(top - b, a.clip) << Exp::SHIFT;
 #pragma unroll
-            for (int e = 0; e < N; e++) sum += tc_weight(exp2, above, d[0][e]);
-            z += sum;
-#pragma unroll
-            for (int v = 1; v < DEEP; v++) {
-#pragma unroll
-                for (int e = 0; e < N; e++) d[v - 1][e] = d[v][e];
-                b[v - 1] = b[v];
-            }
-        }
+        for (int e = 0; e < N; e++) sum += tc_weight(exp2, above, d[e]);
+        z += sum;
     }
     __syncwarp();
 #pragma unroll
@@ -741,26 +722,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             behind.n = 0;
             return true;
         };
-        // normalisers of the pairs that go on in other CTAs, once everybody's maxima are in: some tiles at a time, behind those whose scores are read out
-        struct { int run = 0, done = 0, index = 0; unsigned long long z = 0; } cut;          // tiles of the run that are in z; the run's place among this CTA's scores
-        auto advance = [&](bool patient) {
-            const int x = cut.run, n = s.run[x].left;
-            if (cut.done < n) {
-                if (cut.done == 0) {
-                    if (patient ? !tl_wait(tl_u32(&s.known[x]), 0, abort_flag) : !tc_test(tl_u32(&s.known[x]), 0)) return !patient;
-                }
-                const int m = patient ? n - cut.done : min(n - cut.done, 4 * PT_SETS);
-                cut.z += normalise(s.run[x].tile + cut.done, m, (set - cut.index - cut.done) & 3, s.top[x][g]);
-                cut.done += m;
-                if (cut.done < n) return true;
-                if (t == 0) s.part[x][4 * set + quarter][g] = cut.z;
-                __syncwarp();
-                if (lane == 0) tl_arrive(tl_u32(&s.part_in[x]));
-                cut.z = 0;
-            }
-            cut.run++; cut.index += n; cut.done = 0;
-            return true;
-        };
         for (int x = worker; x < (int)(PT_SETS * PT_PROBS / 16); x += 32 * PT_WORKERS) reinterpret_cast<uint4 *>(probs)[x] = make_uint4(0, 0, 0, 0);      // (the columns beyond 24 stay so)
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         for (int b = blockIdx.x; b < a.B; b += gridDim.x) {                // sequences without keys
@@ -814,7 +775,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                     if (lane == 0) tl_arrive(tl_u32(&s.score_free[i & 1]));
                     if (lane < N) work.base[((long long)v.tile * 4 + quarter) * N + lane] = base;
                     largest = max(largest, base);
-                    if (cut.run < u) advance(false);
                 }
                 if (v.ends_part()) {
                     behind.n = v.part + 1; behind.nt = v.nt; behind.first = v.tile - v.t; behind.index = i - v.part; behind.run = u;
@@ -826,7 +786,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         }
         __syncwarp();
         ok = ok && settle(largest);
-        while (ok && cut.run < RUN_WHOLE) ok = advance(true);
+        // ---- normalisers of the pairs that go on in other CTAs, once everybody's maxima are in ---------------------------------------
+        for (int x = 0, index = 0; ok && x < RUN_WHOLE; x++) {
+            const int n = s.run[x].left;
+            if (n == 0) continue;
+            ok = tl_wait(tl_u32(&s.known[x]), 0, abort_flag);
+            if (!ok) break;
+            const unsigned long long z = normalise(s.run[x].tile, n, (set - index) & 3, s.top[x][g]);
+            if (t == 0) s.part[x][4 * set + quarter][g] = z;
+            __syncwarp();
+            if (lane == 0) tl_arrive(tl_u32(&s.part_in[x]));
+            index += n;
+        }
         asm volatile("griddepcontrol.wait;" ::: "memory");      // (whatever the share: what is launched behind counts on it)
         // ---- probabilities and values ---------------------------------------------------------------------------------------------
         if (ok) {                                  // what the CTA's warps left in memory
