@@ -22,7 +22,11 @@ namespace {
 // A CTA takes the new rows of one (page, KV head): a thread keeps a pair of dimensions and walks the rows, so that the page's bounds
 // need no atomics.  They are formed again from the page's rows, old ones read back: a function of what the cache holds, whatever was
 // appended and given up before.
-constexpr int PA_THREADS = 256;
+//
+// What bounds it: memory for long prompts (2350 rows of 8 KV heads of 128, 58 MB, 11.3 us: 5.1 TB/s), for a token each the launch and four dependent loads
+// (a token's row, the table's entry, the row, the page's older rows; 3.2 us for 64 sequences).  A thread has the loads of PA_ROWS rows on their way
+// at once; CTAs of 128 are all resident from the start (of 256, 16.3 us with four rows, 13.2 with two; 128: 14.3 with one, 12.2 with four).
+constexpr int PA_THREADS = 128, PA_ROWS = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedAppendArgs a) {
@@ -89,14 +93,28 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
                     const int x0 = kp[(long long)r * a.hd + d0], x1 = kp[(long long)r * a.hd + d1];
                     mx0 = max(mx0, x0); mn0 = min(mn0, x0); mx1 = max(mx1, x1); mn1 = min(mn1, x1);
                 }
-            for (int r = g; r < count; r += groups) {
-                int64_t x0 = k[r * a.k_ld + d0], x1 = k[r * a.k_ld + d1];
-                const int64_t y0 = v[r * a.v_ld + d0], y1 = v[r * a.v_ld + d1];
-                paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, logical * P + first + r, i, x0, x1);
-                bad = bad || x0 != (int32_t)x0 || x1 != (int32_t)x1 || y0 != (int32_t)y0 || y1 != (int32_t)y1;
-                const long long to = (long long)(first + r) * a.hd;
-                kp[to + d0] = (int32_t)x0; kp[to + d1] = (int32_t)x1; vp[to + d0] = (int32_t)y0; vp[to + d1] = (int32_t)y1;
-                mx0 = max(mx0, (int32_t)x0); mn0 = min(mn0, (int32_t)x0); mx1 = max(mx1, (int32_t)x1); mn1 = min(mn1, (int32_t)x1);
+            for (int r0 = g; r0 < count; r0 += PA_ROWS * groups) {
+                int64_t x[PA_ROWS][2], y[PA_ROWS][2], c[PA_ROWS], n[PA_ROWS];
+#pragma unroll
+                for (int u = 0; u < PA_ROWS; u++) {
+                    const int r = min(r0 + u * groups, count - 1);
+                    const T *kr = k + r * a.k_ld, *vr = v + r * a.v_ld;
+                    x[u][0] = __ldg(kr + d0); x[u][1] = __ldg(kr + d1); y[u][0] = __ldg(vr + d0); y[u][1] = __ldg(vr + d1);
+                    const long long turn = (logical * P + first + r) * half + i;
+                    c[u] = a.rope ? __ldg(a.cos + turn) : 0; n[u] = a.rope ? __ldg(a.sin + turn) : 0;
+                }
+#pragma unroll
+                for (int u = 0; u < PA_ROWS; u++) {
+                    const int r = r0 + u * groups;
+                    if (r >= count) break;
+                    int64_t x0 = x[u][0], x1 = x[u][1];
+                    const int64_t y0 = y[u][0], y1 = y[u][1];
+                    if (a.rope) { x0 = (x[u][0] * c[u] - x[u][1] * n[u]) >> a.fa; x1 = (x[u][0] * n[u] + x[u][1] * c[u]) >> a.fa; }
+                    bad = bad || x0 != (int32_t)x0 || x1 != (int32_t)x1 || y0 != (int32_t)y0 || y1 != (int32_t)y1;
+                    const long long to = (long long)(first + r) * a.hd;
+                    kp[to + d0] = (int32_t)x0; kp[to + d1] = (int32_t)x1; vp[to + d0] = (int32_t)y0; vp[to + d1] = (int32_t)y1;
+                    mx0 = max(mx0, (int32_t)x0); mn0 = min(mn0, (int32_t)x0); mx1 = max(mx1, (int32_t)x1); mn1 = min(mn1, (int32_t)x1);
+                }
             }
         }
         if (a.bounds) {
@@ -471,7 +489,11 @@ __device__ __forceinline__ bool rank_pages(const PagedSelectArgs &a, const int *
         if (page >= 0)
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                          ::"r"(to_at + lane * ld), "l"(a.bounds + ((long long)page * a.Hkv + kv) * 2 * a.hd), "r"(8 * a.hd), "r"(bar_at) : "memory");
-        if (!tl_wait(bar_at, pass, abort_flag)) return false;
+        if (!tl_wait(bar_at, pass, abort_flag)) {
+            volatile int patient = 0;              // copies under way end first
+            tl_wait_slow(bar_at, pass, &patient);
+            return false;
+        }
         const int4 *row = reinterpret_cast<const int4 *>(stage + g * ld) + t;
         long long best = INT64_MIN;
         for (int h0 = 0; h0 < rep; h0 += HEADS) {
@@ -565,7 +587,7 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const Paged
     const bool ok = s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort)
                   : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort)
                              : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort);
-    if (!ok) { volatile int patient = 0; tl_wait_slow(tl_u32(&s_bar[tid >> 5]), 0, &patient); atomicOr(a.flags, FLAG_GAVE_UP); }      // (a copy under way ends first)
+    if (!ok) atomicOr(a.flags, FLAG_GAVE_UP);
     if (bad) atomicOr(a.flags, 16);
     if (blocks > 1) cluster.sync();
     else __syncthreads();
