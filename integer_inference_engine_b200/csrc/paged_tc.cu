@@ -251,8 +251,9 @@ __device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap *map, int
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(bar), "l"(policy) : "memory");
 }
 
-// 128-byte chunks of a row, ring slots, TMEM columns, those of the scores (behind the outputs, or over their second buffer)
-struct TcShape { int chunks, slots, columns, score_at; };
+// 128-byte chunks of a row, ring slots, TMEM columns, those of the scores (behind the outputs, or over their second buffer); whether no pair can be cut, so
+// that no launch stands in front
+struct TcShape { int chunks, slots, columns, score_at; bool alone; };
 
 struct TcBars {
     uint64_t full[PT_MAX_SLOTS], empty[PT_MAX_SLOTS], meta[PT_META];
@@ -597,7 +598,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tl_u32(&s.tmem)), "r"(sh.columns));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (warp == 3) tc_share(a, s.run);
+    if (warp == 3) {
+        if (sh.alone) asm volatile("griddepcontrol.wait;" ::: "memory");       // (else what lies in front has ended: the clearing kernel waited for it)
+        tc_share(a, s.run);
+    }
     tc_before();
     __syncthreads();
     tc_after();
@@ -958,8 +962,6 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     if (sms <= 0) return cudaErrorInvalidDevice;
     const size_t fixed = 1024 + 2 * (size_t)chunks * padded * 1024 + PT_SETS * PT_PROBS, room = 227 * 1024 - sizeof(TcBars) - 64;
     const int slots = (int)std::min<size_t>(PT_MAX_SLOTS, (room - fixed) / PT_SLOT);
-    // outputs: two buffers of 64 columns a chunk; scores: two of 64, behind them or, at four chunks, over the end of the second
-    const TcShape sh = {chunks, slots, chunks == 1 ? 256 : 512, chunks == 4 ? 384 : 128 * chunks};
     const size_t smem = fixed + (size_t)slots * PT_SLOT;
     static std::atomic<unsigned long long> configured;             // devices, a bit each
     const unsigned long long bit = device < 64 ? 1ULL << device : 0;
@@ -971,17 +973,24 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     }
     const long long most = (long long)a.B * a.Hkv * tc_head_groups(a) * tc_tiles_most(a);
     const unsigned ctas = (unsigned)std::min<long long>(std::min(sms, PT_MOST_CTAS), std::max<long long>(1, most));
-    const TcWork w = tc_work(a, (int)ctas);
-    e = launch_behind(paged_clear_kernel, ctas, 128, 0, s, w.notes, w.acc, PT_HEADS * a.hd);
-    if (e != cudaSuccess) return e;
+    // few tiles a CTA, and tc_share deals out whole pairs whatever the lengths: nothing to clear (1 x 300 keys 18.8 us; with the launch in front 19.8)
+    const long long pairs = (long long)a.B * a.Hkv * tc_head_groups(a);
+    const bool alone = (pairs + ctas - 1) / ctas * tc_tiles_most(a) <= 4;
+    // outputs: two buffers of 64 columns a chunk; scores: two of 64, behind them or, at four chunks, over the end of the second
+    const TcShape sh = {chunks, slots, chunks == 1 ? 256 : 512, chunks == 4 ? 384 : 128 * chunks, alone};
+    if (!alone) {
+        const TcWork w = tc_work(a, (int)ctas);
+        e = launch_behind(paged_clear_kernel, ctas, 128, 0, s, w.notes, w.acc, PT_HEADS * a.hd);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(PT_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeCooperative; attr[0].val.cooperative = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeCooperative; attr[1].val.cooperative = 1;
+    cfg.attrs = attr; cfg.numAttrs = alone ? 1 : 2;
     e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<AT16, SMALL, N>, a, kmap, vmap, sh);
-    note_launch(2);
+    note_launch(alone ? 1 : 2);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

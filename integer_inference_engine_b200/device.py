@@ -204,10 +204,15 @@ def _paged_table(table: torch.Tensor, name: str, each: torch.Tensor) -> tuple:
     return shape
 
 
-def _rows_apart(t: torch.Tensor) -> bool:
-    """Whether a matrix is rows of adjacent values that do not overlap (any distance apart)."""
-    rows, columns = t.shape
-    return (rows == 0 or t.stride(1) == 1) and (rows < 2 or t.stride(0) >= columns)
+def _row_distance(t: torch.Tensor, shape) -> int:
+    """Distance of the rows of a matrix, of adjacent values each; -1 where they are not adjacent or overlap."""
+    rows, columns = shape
+    if t.is_contiguous():
+        return columns
+    apart, beside = t.stride()
+    if (beside != 1 and rows > 0) or (rows > 1 and apart < columns):
+        return -1
+    return max(apart, columns)
 
 
 def _paged_rope(rope: int, cos, sin, head_dim: int) -> tuple:
@@ -222,11 +227,14 @@ def _paged_rope(rope: int, cos, sin, head_dim: int) -> tuple:
     return cos.data_ptr(), sin.data_ptr(), cos.shape[0]
 
 
-def _paged_query(q: torch.Tensor, n_seqs: int, n_kv: int, head_dim: int) -> int:
-    """Query heads of q [sequences, heads * head_dim]."""
-    if q.dtype != torch.int64 or q.dim() != 2 or q.shape[0] != n_seqs or q.shape[1] == 0 or q.shape[1] % (n_kv * head_dim) or not _rows_apart(q):
-        raise ValueError("q must be int64 [sequences, heads * head_dim], heads a multiple of the KV heads, columns adjacent")
-    return q.shape[1] // head_dim
+def _paged_query(q: torch.Tensor, n_seqs: int, n_kv: int, head_dim: int) -> tuple:
+    """Query heads of q [sequences, heads * head_dim], and the distance of its rows."""
+    shape = q.shape
+    if q.dtype == torch.int64 and len(shape) == 2 and shape[0] == n_seqs and shape[1] > 0 and shape[1] % (n_kv * head_dim) == 0:
+        apart = _row_distance(q, shape)
+        if apart >= 0:
+            return shape[1] // head_dim, apart
+    raise ValueError("q must be int64 [sequences, heads * head_dim], heads a multiple of the KV heads, columns adjacent")
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
@@ -244,11 +252,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages:
     outside the cache (it is left out) bit 4 of :func:`read_flags`."""
     n_pages, n_kv, page_rows, head_dim = _paged_pool(kpages, vpages)
     B, per_seq = _paged_table(table, "start", start)
-    if k.dtype not in (torch.int64, torch.int32) or v.dtype != k.dtype or k.dim() != 2 or k.shape != v.shape or k.shape[1] != n_kv * head_dim:
+    narrow, width, shape = k.dtype == torch.int32, n_kv * head_dim, k.shape
+    if not (narrow or k.dtype == torch.int64) or v.dtype != k.dtype or len(shape) != 2 or shape != v.shape or shape[1] != width:
         raise ValueError("k and v must be int64 or int32 [rows, n_kv * head_dim] of one shape")
-    if not (_rows_apart(k) and _rows_apart(v)):
+    k_ld, v_ld = _row_distance(k, shape), _row_distance(v, shape)
+    if k_ld < 0 or v_ld < 0:
         raise ValueError("the columns of k and v must be adjacent and their rows must not overlap")
-    if rows is None and k.shape[0] < B:
+    if rows is None and shape[0] < B:
         raise ValueError("without rows, k and v need a row per sequence")
     if rows is not None and (rows.dtype != torch.int32 or rows.shape != (B + 1,) or not rows.is_contiguous()):
         raise ValueError("rows must be a contiguous int32 vector with one entry more than table has rows")
@@ -258,7 +268,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages:
     lib = qk_cuda._lib()
     _on_current_device("k v kpages vpages table start rows bounds cos sin", k, v, kpages, vpages, table, start, rows, bounds, cos if rope else None, sin if rope else None)
     with _CUDA_LOCK:
-        rc = lib.iie_paged_append_dev(k.data_ptr(), v.data_ptr(), int(k.dtype == torch.int32), max(k.stride(0), k.shape[1]), max(v.stride(0), v.shape[1]), k.shape[0],
+        rc = lib.iie_paged_append_dev(k.data_ptr(), v.data_ptr(), narrow, k_ld, v_ld, shape[0],
                                       kpages.data_ptr(), vpages.data_ptr(), n_pages, page_rows, table.data_ptr(), per_seq, start.data_ptr(),
                                       rows.data_ptr() if rows is not None else None, B, cos_p, sin_p, rope_rows, int(rope), n_kv, head_dim, int(fa),
                                       bounds.data_ptr() if bounds is not None else None, _stream_ptr())
@@ -278,7 +288,7 @@ def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     int64, the bytes :func:`attention_decode` gives over the same keys."""
     n_pages, n_kv, page_rows, head_dim = _paged_pool(kpages, vpages)
     B, per_seq = _paged_table(table, "lengths", lengths)
-    n_heads = _paged_query(q, B, n_kv, head_dim)
+    n_heads, q_ld = _paged_query(q, B, n_kv, head_dim)
     if pages is not None and (pages.dtype != torch.int32 or pages.dim() != 3 or pages.shape[:2] != (B, n_kv) or pages.shape[2] == 0 or not pages.is_contiguous()):
         raise ValueError("pages must be a contiguous int32 [sequences, n_kv, n] with n > 0")
     if max_length is None:
@@ -302,7 +312,7 @@ def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
         raise ValueError("a shape that paged attention does not take")
     work = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)      # the stream's own: calls on other streams have theirs
     with _CUDA_LOCK:
-        rc = lib.iie_paged_attn_dev(q.data_ptr(), max(q.stride(0), q.shape[1]), kpages.data_ptr(), vpages.data_ptr(), n_pages, page_rows, table.data_ptr(), per_seq, lengths.data_ptr(), B,
+        rc = lib.iie_paged_attn_dev(q.data_ptr(), q_ld, kpages.data_ptr(), vpages.data_ptr(), n_pages, page_rows, table.data_ptr(), per_seq, lengths.data_ptr(), B,
                                     int(max_length), pages.data_ptr() if pages is not None else None, picked, int(window), cos_p, sin_p, rope_rows, int(rope),
                                     n_heads, n_kv, head_dim, int(fa), int(inv_sqrt), work.data_ptr(), need, out.data_ptr(), _stream_ptr())
     if rc != 0:
@@ -322,7 +332,7 @@ def paged_select(q: torch.Tensor, bounds: torch.Tensor, table: torch.Tensor, len
         raise ValueError("bounds must be a contiguous int32 [pages, n_kv, 2, head_dim]")
     n_pages, n_kv, _, head_dim = bounds.shape
     B, per_seq = _paged_table(table, "lengths", lengths)
-    n_heads = _paged_query(q, B, n_kv, head_dim)
+    n_heads, q_ld = _paged_query(q, B, n_kv, head_dim)
     if page_rows <= 0 or n_select <= 0 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > n_select:
         raise ValueError("page_rows and n_select must be positive, keep_first + keep_last at most n_select")
     if window < 0:
@@ -336,7 +346,7 @@ def paged_select(q: torch.Tensor, bounds: torch.Tensor, table: torch.Tensor, len
     _on_current_device("q bounds table lengths out cos sin", q, bounds, table, lengths, out, cos if rope else None, sin if rope else None)
     score = q.new_empty((B, n_kv, per_seq))
     with _CUDA_LOCK:
-        rc = lib.iie_paged_select_dev(q.data_ptr(), max(q.stride(0), q.shape[1]), bounds.data_ptr(), n_pages, int(page_rows), table.data_ptr(), per_seq, lengths.data_ptr(), B, int(n_select),
+        rc = lib.iie_paged_select_dev(q.data_ptr(), q_ld, bounds.data_ptr(), n_pages, int(page_rows), table.data_ptr(), per_seq, lengths.data_ptr(), B, int(n_select),
                                       int(keep_first), int(keep_last), int(window), cos_p, sin_p, rope_rows, int(rope), n_heads, n_kv, head_dim, int(fa),
                                       score.data_ptr(), out.data_ptr(), _stream_ptr())
     if rc != 0:
