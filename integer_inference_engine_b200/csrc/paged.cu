@@ -462,8 +462,10 @@ __global__ void __launch_bounds__(PS_THREADS) paged_pick_kernel(const PagedSelec
 // into the first CTA's shared memory, and that one picks.  A warp has the bounds of eight pages copied into shared memory (a page's 8 hd bytes lie
 // side by side; a gap behind each keeps the banks apart); four lanes share a page, a lane takes every fourth group of four dimensions of eight
 // heads: 32 x 32 -> 64-bit multiply-adds (four clocks a warp) of a query value with the bound that its sign selects (four clocks on the
-// other pipe).  What bounds it: those, 4.3 us for the 39 MB of 38500 pages of two bounds of 128 and 8 heads on 148 SMs; memory alone 6.  (Loads
-// into registers instead, two pages a lane: four round trips a page, 20 us.)  A query beyond int32 takes 64-bit products.
+// other pipe).  What bounds it: those, and the longest sequence.  Eight sequences of up to 2000 pages (4 KV heads of two bounds of 128, 38500 pages, 39 MB) take 26 us:
+// 2 for the query, 16 for the four rounds of the longest (3 of each round's 4 are multiply-adds; memory alone would take 6 in all), 7 to pick.  (A page's
+// bounds copied as halves, the next ones' while the others are multiplied: 21 for the rounds, four times as many copies.  Loads into registers instead, two
+// pages a lane: four round trips a page, 20.)  A query beyond int32 takes 64-bit products.
 constexpr int PR_PAGES = 8;                        // pages of a warp at a time
 constexpr int PR_GAP = 64;
 constexpr int PR_MOST = 8192;                      // pages of a sequence: 64 KB of scores

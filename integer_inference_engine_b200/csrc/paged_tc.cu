@@ -13,9 +13,14 @@
 // Tiles of 128 keys of all sequences and KV heads form one list that one CTA per SM share evenly, whatever the lengths.  The softmax floors e
 // and p, which takes the maximum and then the normaliser of all of a pair's keys (pair: a sequence's KV head with up to eight query heads) in
 // front of its values: a CTA takes the scores of all its tiles (in memory, as 32-bit distances below the maximum of 32 keys; one beyond
-// `clip` has no weight, so nothing is lost), the normalisers, then the values.  Pairs that lie in one CTA need nobody else; those cut
-// between CTAs (at most one begins in each) exchange maximum, normaliser and output sums in memory, in a cell of the CTA where they
-// begin.  The launch is cooperative, every wait is bounded, and integers are added in any order.  A small kernel in front clears the cells.
+// `clip` has no weight, so nothing is lost), the normalisers, then the values.  Pairs that lie in one CTA need nobody else.  Of those cut between CTAs
+// (at most one begins in each) every CTA tells the others its maximum and its normaliser, and the output sums are added up in memory with a count of their
+// parts.  The launch is cooperative, every wait is bounded, and integers are added in any order.  A small kernel in front clears what is told.
+//
+// What bounds it: memory where there is much of it, 122 us for 64 sequences of up to 4096 keys (4 KV heads of 128, 8 query heads each; 640 MB: 5.2 TB/s), 63 us for
+// 278 MB of three of up to 30000.  Beside that a call pays 3 us until the share is planned, 3 us until the first query columns are written, 6 to 9 us
+// between keys and values (a microsecond or two for an exchange, twice, and the exponentials: 24 clocks for a warp's 32, 0.13 us for a tile of eight heads),
+// 2 us for the outputs: 19 us for one sequence of 300 keys, 24 for one of 4096.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -77,7 +82,8 @@ __host__ __device__ inline TcWork tc_work(const PagedAttnArgs &a, int ctas, size
     w.z = w.top + pairs * PT_HEADS;
     w.notes = reinterpret_cast<TcNotes *>(w.z + pairs * PT_WORKERS * PT_HEADS);
     w.acc = reinterpret_cast<unsigned long long *>(w.notes + 2 * ctas);
-    if (bytes) *bytes = (size_t)tiles * room * (PT_KEYS * 4 + 4 * 8) + (size_t)pairs * (PT_WORKERS + 1) * PT_HEADS * 8 + (size_t)ctas * (2 * sizeof(TcNotes) + (size_t)PT_HEADS * a.hd * 8);
+    if (bytes)
+        *bytes = (size_t)tiles * room * (PT_KEYS * 4 + 4 * 8) + (size_t)pairs * (PT_WORKERS + 1) * PT_HEADS * 8 + (size_t)ctas * (2 * sizeof(TcNotes) + (size_t)PT_HEADS * a.hd * 8);
     return w;
 }
 
@@ -114,11 +120,13 @@ struct TcWalk {
     }
 };
 
-// One warp: the CTA's share of the list, as up to three runs: two pairs that it has in common with other CTAs, and whole pairs.  A pair that is cut costs its CTAs an exchange, some six microseconds or four tiles; a second pair costs other query columns.
+// One warp: the CTA's share of the list, as up to three runs: two pairs that it has in common with other CTAs, and whole pairs.  A pair that is cut costs its
+// CTAs an exchange, some six microseconds or four tiles; a second pair costs other query columns.
 //  * Whole pairs, dealt out in order, where the longest pairs so dealt make a CTA no more than four tiles above the average.
 //  * Else each pair has CTAs of its own in proportion to its tiles, where there are enough CTAs and no part is more than two tiles above it.
 //  * Else the list is cut evenly: a CTA has the end of a pair, whole ones, the beginning of another.  (Cut pairs in an order that has two neighbours at
-//    the same one first, normalised between tiles as soon as the maxima are in, came to the same: what is looked up between tiles holds them up.)
+//    the same one first, normalised between tiles as soon as the maxima are in, were no faster: the registers and the code that this takes cost the
+//    tiles what it hides.)
 enum { RUN_WHOLE = 2, RUNS };
 __device__ __noinline__ int tc_count(const PagedAttnArgs &a, int b) {
     PagedSpan s;
@@ -133,7 +141,8 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
     int sum = 0, some = 0, longest = 0;
 #pragma unroll 1
     for (int b = lane; b - lane < a.B; b += 32) { const int c = count(b); sum += c; some += c > 0; longest = max(longest, c); }
-    const int total = __reduce_add_sync(0xffffffffu, sum) * per_seq, pairs = __reduce_add_sync(0xffffffffu, some) * per_seq, most = __reduce_max_sync(0xffffffffu, longest);      // (total * 256 fits 32 bits: paged_tc_ok)
+    const int total = __reduce_add_sync(0xffffffffu, sum) * per_seq, pairs = __reduce_add_sync(0xffffffffu, some) * per_seq;       // (total * 256 fits 32 bits: paged_tc_ok)
+    const int most = __reduce_max_sync(0xffffffffu, longest);
     const int average = total / ctas;
     // CTAs of a pair of c tiles that has its own, and the tiles of one
     auto parts = [&](int c) { return c == 0 ? 0 : max(1, min(c, (int)((uint32_t)c * ctas / total))); };
@@ -147,7 +156,8 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
         if ((int)__reduce_add_sync(0xffffffffu, ps) * per_seq <= ctas && (int)__reduce_max_sync(0xffffffffu, pl) <= average + 2) way = OWN_CTAS;
     }
     // the share in units of the way, and where in the list its first and last unit are
-    const int all = way == EVEN ? total : pairs, from = way == OWN_CTAS ? me : (int)((uint32_t)all * me / ctas), to = way == OWN_CTAS ? me + 1 : (int)((uint32_t)all * (me + 1) / ctas);
+    const int all = way == EVEN ? total : pairs;
+    const int from = way == OWN_CTAS ? me : (int)((uint32_t)all * me / ctas), to = way == OWN_CTAS ? me + 1 : (int)((uint32_t)all * (me + 1) / ctas);
     int at[2] = {-1, -1}, in[2] = {0, 0}, first[2] = {0, 0};       // sequence, unit in it, its first tile
     int before = 0, tiles_before = 0;              // units and tiles per pair of the sequences in front
 #pragma unroll 1
@@ -328,7 +338,8 @@ __device__ __forceinline__ TcBoxes tc_boxes(const PagedAttnArgs &a, const TcLook
 // IN_BOX: groups of eight rows that a box brings.  `turn`: chunks requested so far, by both warps; `tile`: tiles.  (Asking the values into L2 ahead
 // of the ring, too, while the normalisers are exchanged, was slower by a fifth: every other access waits behind them.)
 template <int IN_BOX, bool KEYS>
-__device__ __forceinline__ bool tc_produce(const PagedAttnArgs &a, TcWalk w, const CUtensorMap *map, TcBars &s, uint32_t ring, const TcShape &sh, int me, TcRing &at, int &turn, int &tile, volatile int *abort_flag) {
+__device__ __forceinline__ bool tc_produce(const PagedAttnArgs &a, TcWalk w, const CUtensorMap *map, TcBars &s, uint32_t ring, const TcShape &sh, int me, TcRing &at, int &turn,
+                                           int &tile, volatile int *abort_flag) {
     const int lane = threadIdx.x & 31, groups = tc_head_groups(a), per_seq = a.Hkv * groups;
     constexpr uint32_t ALL = IN_BOX == 1 ? 0xFFFFu : 0x5555u;
     if (w.left == 0) return true;
@@ -371,7 +382,8 @@ __device__ __forceinline__ bool tc_produce(const PagedAttnArgs &a, TcWalk w, con
     return true;
 }
 template <int IN_BOX>
-__device__ __forceinline__ void tc_producer(const PagedAttnArgs &a, const CUtensorMap *kmap, const CUtensorMap *vmap, TcBars &s, uint32_t ring, const TcShape &sh, int me, volatile int *abort_flag) {
+__device__ __forceinline__ void tc_producer(const PagedAttnArgs &a, const CUtensorMap *kmap, const CUtensorMap *vmap, TcBars &s, uint32_t ring, const TcShape &sh, int me,
+                                            volatile int *abort_flag) {
     TcRing at;
     int turn = 0, tile = 0;
     bool ok = true;
@@ -569,7 +581,8 @@ __device__ __noinline__ unsigned long long tc_normalise(const PagedAttnArgs &a, 
 // AT16: fa = 16; SMALL: beside that every sum of exponentials at most 2^31; N: heads that a warp's lanes are dealt to, and keys of a lane (of four heads in a layout
 // for eight, half of the lanes' exponentials would be for nothing)
 template <bool AT16, bool SMALL, int N>
-__global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcShape sh) {
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                                                                  const __grid_constant__ TcShape sh) {
     using Exp = std::conditional_t<AT16, TcExp16, TcExp>;
     using Quotient = std::conditional_t<SMALL, SoftmaxQuotient16, SoftmaxQuotient>;
     extern __shared__ unsigned char pt_raw[];
@@ -618,61 +631,61 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             bool ok = true, fresh = true;
             int queries = 0, i = 0;
             for (int u = 0; u < RUNS; u++) {       // scores
-            TcWalk v = s.run[u];
-            for (fresh = true; ok && v.left > 0; i++) {
-                if (i >= 2) ok = tc_wait(tl_u32(&s.score_free[i & 1]), ((i >> 1) & 1) ^ 1, abort_flag);
-                if (ok && fresh) { ok = tc_wait(tl_u32(&s.query_full), queries & 1, abort_flag); queries++; }
-                const uint32_t d = score_at + (i & 1) * 64;
-                uint32_t q = tc_desc(tl_u32(smem));
-                for (int c = 0; ok && c < sh.chunks; c++, q += (uint32_t)padded * 64) {
-                    ok = tc_wait(tl_u32(&s.full[at.slot]), at.pass, abort_flag);
-                    if (!ok) break;
-                    tc_after();
-                    const uint32_t keys = tc_desc(ring + at.slot * PT_SLOT), q3 = q + (operand >> 4);
+                TcWalk v = s.run[u];
+                for (fresh = true; ok && v.left > 0; i++) {
+                    if (i >= 2) ok = tc_wait(tl_u32(&s.score_free[i & 1]), ((i >> 1) & 1) ^ 1, abort_flag);
+                    if (ok && fresh) { ok = tc_wait(tl_u32(&s.query_full), queries & 1, abort_flag); queries++; }
+                    const uint32_t d = score_at + (i & 1) * 64;
+                    uint32_t q = tc_desc(tl_u32(smem));
+                    for (int c = 0; ok && c < sh.chunks; c++, q += (uint32_t)padded * 64) {
+                        ok = tc_wait(tl_u32(&s.full[at.slot]), at.pass, abort_flag);
+                        if (!ok) break;
+                        tc_after();
+                        const uint32_t keys = tc_desc(ring + at.slot * PT_SLOT), q3 = q + (operand >> 4);
 #pragma unroll
-                    for (int k = 0; k < 8; k += 2) {       // 32 bytes of the rows
-                        tc_mma<up, up>(d, keys + k, q + k, lower_i, (c | k) != 0);
-                        tc_mma<up, up>(d, keys + k, q3 + k, upper_i, 1);
+                        for (int k = 0; k < 8; k += 2) {       // 32 bytes of the rows
+                            tc_mma<up, up>(d, keys + k, q + k, lower_i, (c | k) != 0);
+                            tc_mma<up, up>(d, keys + k, q3 + k, upper_i, 1);
+                        }
+                        tl_commit(tl_u32(&s.empty[at.slot]));
+                        at.step(sh.slots);
                     }
-                    tl_commit(tl_u32(&s.empty[at.slot]));
-                    at.step(sh.slots);
+                    if (ok) tl_commit(tl_u32(&s.score_full[i % PT_SETS]));
+                    fresh = v.t + 1 == v.nt;
+                    v.next(a, per_seq);
                 }
-                if (ok) tl_commit(tl_u32(&s.score_full[i % PT_SETS]));
-                fresh = v.t + 1 == v.nt;
-                v.next(a, per_seq);
-            }
             }
             for (int k = max(0, i - 2); ok && k < i; k++) ok = tc_wait(tl_u32(&s.score_free[k & 1]), (k >> 1) & 1, abort_flag);      // (outputs take the scores' columns)
             int seg = 0;
             i = 0;
             for (int u = 0; u < RUNS; u++) {       // values
-            TcWalk v = s.run[tc_value_run(u)];
-            for (; ok && v.left > 0; i++) {
-                ok = tc_wait(tl_u32(&s.prob_full[i % PT_SETS]), (i / PT_SETS) & 1, abort_flag);
-                if (ok && v.seg == 0 && seg >= 2) ok = tc_wait(tl_u32(&s.out_free[seg & 1]), ((seg >> 1) & 1) ^ 1, abort_flag);
-                const uint32_t p = tc_desc(tl_u32(probs) + (i % PT_SETS) * PT_PROBS);
-                uint32_t d = tmem + (seg & 1) * buffer;
-                for (int c = 0; ok && c < sh.chunks; c++, d += 64) {
-                    ok = tc_wait(tl_u32(&s.full[at.slot]), at.pass, abort_flag);
-                    if (!ok) break;
-                    tc_after();
-                    const uint32_t values = tc_desc(ring + at.slot * PT_SLOT);
+                TcWalk v = s.run[tc_value_run(u)];
+                for (; ok && v.left > 0; i++) {
+                    ok = tc_wait(tl_u32(&s.prob_full[i % PT_SETS]), (i / PT_SETS) & 1, abort_flag);
+                    if (ok && v.seg == 0 && seg >= 2) ok = tc_wait(tl_u32(&s.out_free[seg & 1]), ((seg >> 1) & 1) ^ 1, abort_flag);
+                    const uint32_t p = tc_desc(tl_u32(probs) + (i % PT_SETS) * PT_PROBS);
+                    uint32_t d = tmem + (seg & 1) * buffer;
+                    for (int c = 0; ok && c < sh.chunks; c++, d += 64) {
+                        ok = tc_wait(tl_u32(&s.full[at.slot]), at.pass, abort_flag);
+                        if (!ok) break;
+                        tc_after();
+                        const uint32_t values = tc_desc(ring + at.slot * PT_SLOT);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {          // 32 keys
-                        tc_mma<up, pp>(d, values + 256 * k, p + 64 * k, plain, (v.seg | k) != 0);
-                        tc_mma<up, pp>(d + 32, values + 256 * k, p + 64 * k, last_byte, (v.seg | k) != 0);
+                        for (int k = 0; k < 4; k++) {          // 32 keys
+                            tc_mma<up, pp>(d, values + 256 * k, p + 64 * k, plain, (v.seg | k) != 0);
+                            tc_mma<up, pp>(d + 32, values + 256 * k, p + 64 * k, last_byte, (v.seg | k) != 0);
+                        }
+                        tl_commit(tl_u32(&s.empty[at.slot]));
+                        at.step(sh.slots);
                     }
-                    tl_commit(tl_u32(&s.empty[at.slot]));
-                    at.step(sh.slots);
+                    const bool last = v.ends_segment();
+                    if (ok) {
+                        tl_commit(tl_u32(&s.prob_free[i % PT_SETS]));
+                        if (last) tl_commit(tl_u32(&s.out_full[seg & 1]));
+                    }
+                    if (last) seg++;
+                    v.next(a, per_seq);
                 }
-                const bool last = v.ends_segment();
-                if (ok) {
-                    tl_commit(tl_u32(&s.prob_free[i % PT_SETS]));
-                    if (last) tl_commit(tl_u32(&s.out_full[seg & 1]));
-                }
-                if (last) seg++;
-                v.next(a, per_seq);
-            }
             }
             if (*abort_flag) {                     // products under way end before their TMEM is given back
                 tl_commit(tl_u32(&s.drain));
@@ -739,7 +752,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         for (int u = 0; u < RUNS; u++) {
             TcWalk v = s.run[u];
             for (bool fresh = true; ok && v.left > 0; i++) {
-                if (fresh) {                       // the columns are free once the tile in front has been multiplied (every set has waited for one of the last four tiles: no phase is mistaken)
+                if (fresh) {                       // the columns are free once the tile in front has been multiplied (a set has waited for one of the last four: no phase is mistaken)
                     if (i > 0 && !tl_wait(tl_u32(&s.score_full[(i - 1) % PT_SETS]), ((i - 1) / PT_SETS) & 1, abort_flag)) { ok = false; break; }
                     const long long most = largest;
                     largest = INT64_MIN;
@@ -851,7 +864,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
                 for (int h = 0; h < HELD; h++) {
                     if (!pending.ends || h0 + h >= pending.heads) continue;
                     if (!whole) {                  // added up in memory: who adds the last part finds the sum
-                        const unsigned long long part = carry[h] + (1ULL << PT_COUNT), all = atomicAdd(acc + (h0 + h) * a.hd + d, part) + part, parts = (all + (1ULL << (PT_COUNT - 1))) >> PT_COUNT;
+                        const unsigned long long part = carry[h] + (1ULL << PT_COUNT), all = atomicAdd(acc + (h0 + h) * a.hd + d, part) + part;
+                        const unsigned long long parts = (all + (1ULL << (PT_COUNT - 1))) >> PT_COUNT;
                         if (((parts ^ pending.parts) & 0xFF) != 0) continue;
                         carry[h] = all - (parts << PT_COUNT);
                     }
@@ -869,57 +883,57 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         };
         i = 0;
         for (int u = 0; u < RUNS; u++) {
-        const int run = tc_value_run(u);
-        TcWalk v = s.run[run];
-        for (bool fresh = true; ok && v.left > 0; i++) {
-            if (fresh) {
-                unsigned long long z = 0;
-                top = 0;
-                if (v.t == 0 && v.rest() == v.nt) {
-                    const long long pair = (long long)v.b * per_seq + v.pair_of;
-                    top = __ldcg(work.top + pair * PT_HEADS + g);
+            const int run = tc_value_run(u);
+            TcWalk v = s.run[run];
+            for (bool fresh = true; ok && v.left > 0; i++) {
+                if (fresh) {
+                    unsigned long long z = 0;
+                    top = 0;
+                    if (v.t == 0 && v.rest() == v.nt) {
+                        const long long pair = (long long)v.b * per_seq + v.pair_of;
+                        top = __ldcg(work.top + pair * PT_HEADS + g);
 #pragma unroll
-                    for (int w = 0; w < PT_WORKERS / LANES; w++) z += __ldcg(work.z + (pair * PT_WORKERS + LANES * w + t) * PT_HEADS + g);
+                        for (int w = 0; w < PT_WORKERS / LANES; w++) z += __ldcg(work.z + (pair * PT_WORKERS + LANES * w + t) * PT_HEADS + g);
 #pragma unroll
-                    for (int d = 1; d < LANES; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
-                } else {
-                    if (!tl_wait(tl_u32(&s.known[run]), 1, abort_flag)) { ok = false; break; }
-                    top = s.top[run][g]; z = s.z[run][g];
+                        for (int d = 1; d < LANES; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+                    } else {
+                        if (!tl_wait(tl_u32(&s.known[run]), 1, abort_flag)) { ok = false; break; }
+                        top = s.top[run][g]; z = s.z[run][g];
+                    }
+                    quotient = Quotient(g < heads_most ? z : 0, a.fa);
                 }
-                quotient = Quotient(g < heads_most ? z : 0, a.fa);
-            }
-            if (i % PT_SETS == set) {
-                uint32_t p[N];
-                unsigned long long base;
-                tc_distances<N>(work.dist + g * PT_KEYS + quarter * 32 + N * t, work.base + quarter * N + g, v.tile, p, base);
-                const uint32_t above = (uint32_t)tc_min(top - base, a.clip) << Exp::SHIFT;
+                if (i % PT_SETS == set) {
+                    uint32_t p[N];
+                    unsigned long long base;
+                    tc_distances<N>(work.dist + g * PT_KEYS + quarter * 32 + N * t, work.base + quarter * N + g, v.tile, p, base);
+                    const uint32_t above = (uint32_t)tc_min(top - base, a.clip) << Exp::SHIFT;
 #pragma unroll
-                for (int e = 0; e < N; e++) p[e] = g < heads_most ? (uint32_t)quotient(tc_weight(exp2, above, p[e])) : 0u;
-                if (i >= PT_SETS && !tl_wait(tl_u32(&s.prob_free[set]), ((i / PT_SETS) & 1) ^ 1, abort_flag)) { ok = false; break; }
-                unsigned char *to = probs + set * PT_PROBS + (quarter * 32 + t) * 32 + g;
+                    for (int e = 0; e < N; e++) p[e] = g < heads_most ? (uint32_t)quotient(tc_weight(exp2, above, p[e])) : 0u;
+                    if (i >= PT_SETS && !tl_wait(tl_u32(&s.prob_free[set]), ((i / PT_SETS) & 1) ^ 1, abort_flag)) { ok = false; break; }
+                    unsigned char *to = probs + set * PT_PROBS + (quarter * 32 + t) * 32 + g;
 #pragma unroll
-                for (int e = 0; e < N; e++) {      // key t + LANES e: byte b at 8 b + g, the halves of 32 bytes swapped in every second group of four rows
-                    const int at = LANES * 32 * e, swap = (((t + LANES * e) >> 2) & 1) * 16;
-                    to[at + swap] = (unsigned char)p[e];
-                    to[at + 8 + swap] = (unsigned char)(p[e] >> 8);
-                    to[at + 16 - swap] = (unsigned char)(p[e] >> 16);
+                    for (int e = 0; e < N; e++) {      // key t + LANES e: byte b at 8 b + g, the halves of 32 bytes swapped in every second group of four rows
+                        const int at = LANES * 32 * e, swap = (((t + LANES * e) >> 2) & 1) * 16;
+                        to[at + swap] = (unsigned char)p[e];
+                        to[at + 8 + swap] = (unsigned char)(p[e] >> 8);
+                        to[at + 16 - swap] = (unsigned char)(p[e] >> 16);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tl_arrive(tl_u32(&s.prob_full[set]));
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) tl_arrive(tl_u32(&s.prob_full[set]));
+                // (sums are read out behind the next tile's probabilities, so that the products go on meanwhile)
+                if (pending.tiles && (i % PT_SETS == set) && !read_out()) { ok = false; break; }
+                if (v.ends_segment()) {
+                    if (pending.tiles && !read_out()) { ok = false; break; }
+                    const int group = v.pair_of % groups, kv = v.pair_of / groups;
+                    pending.tiles = v.part + 1; pending.nt = v.nt; pending.ends = v.ends_part(); pending.owner = v.owner; pending.parts = v.parts;
+                    pending.heads = min(heads_most, a.H / a.Hkv - group * heads_most);
+                    pending.out = a.out + ((long long)v.b * a.H + kv * (a.H / a.Hkv) + group * heads_most) * a.hd;
+                }
+                fresh = v.t + 1 == v.nt;
+                v.next(a, per_seq);
             }
-            // (sums are read out behind the next tile's probabilities, so that the products go on meanwhile)
-            if (pending.tiles && (i % PT_SETS == set) && !read_out()) { ok = false; break; }
-            if (v.ends_segment()) {
-                if (pending.tiles && !read_out()) { ok = false; break; }
-                const int group = v.pair_of % groups, kv = v.pair_of / groups;
-                pending.tiles = v.part + 1; pending.nt = v.nt; pending.ends = v.ends_part(); pending.owner = v.owner; pending.parts = v.parts;
-                pending.heads = min(heads_most, a.H / a.Hkv - group * heads_most);
-                pending.out = a.out + ((long long)v.b * a.H + kv * (a.H / a.Hkv) + group * heads_most) * a.hd;
-            }
-            fresh = v.t + 1 == v.nt;
-            v.next(a, per_seq);
-        }
         }
         if (ok && pending.tiles) read_out();
     }
@@ -948,7 +962,7 @@ int tc_sms(int device) {
     if (device >= 0 && device < 64) known[device] = n;
     return n;
 }
-constexpr int PT_MOST_CTAS = 256;                  // cells in the scratch
+constexpr int PT_MOST_CTAS = 256;                  // that the scratch has room for
 
 template <bool AT16, bool SMALL, int N>
 cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
