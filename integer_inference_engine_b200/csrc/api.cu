@@ -1783,7 +1783,7 @@ extern "C" int iie_apply_dev(long long h, const int64_t *x_dev, long long T, int
 extern "C" int iie_flags_read_clear(void *stream) {
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     if (!init()) return -1;
-    if (stream && cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return -1;
+    if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return -1;      // (null: the default stream)
     return read_flags_clear();
 }
 

@@ -354,6 +354,23 @@ def test_what_lies_outside_the_cache_is_flagged_and_left_out():
         assert device.read_flags() == 4
 
 
+def test_flags_wait_for_the_default_stream():
+    import torch
+
+    from integer_inference_engine_b200 import device
+    k = torch.zeros((1, 64), dtype=torch.int64, device="cuda")
+    pages, table = torch.zeros((2, 1, 16, 64), dtype=torch.int32, device="cuda"), torch.zeros((1, 2), dtype=torch.int32, device="cuda")
+    inside, outside = (torch.tensor([n], dtype=torch.int32, device="cuda") for n in (3, 40))
+    busy = torch.zeros((4096, 4096), device="cuda")
+    device.paged_append(k, k, pages, pages.clone(), table, inside)
+    device.read_flags()
+    for _ in range(3):
+        for _ in range(20):
+            busy = busy @ busy                     # some milliseconds in front of the call whose flag is read
+        device.paged_append(k, k, pages, pages, table, outside)
+        assert device.read_flags() == 16 and device.read_flags() == 0
+
+
 def test_no_sequences():
     import torch
 
