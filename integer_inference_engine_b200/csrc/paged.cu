@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
                 for (int u = 0; u < PA_ROWS; u++) {
                     const int r = min(r0 + u * groups, count - 1);
                     const T *kr = k + r * a.k_ld, *vr = v + r * a.v_ld;
-                    x[u][0] = __ldg(kr + d0); x[u][1] = __ldg(kr + d1); y[u][0] = __ldg(vr + d0); y[u][1] = __ldg(vr + d1);
+                    x[u][0] = kr[d0]; x[u][1] = kr[d1]; y[u][0] = vr[d0]; y[u][1] = vr[d1];
                     const long long turn = (logical * P + first + r) * half + i;
-                    c[u] = a.rope ? __ldg(a.cos + turn) : 0; n[u] = a.rope ? __ldg(a.sin + turn) : 0;
+                    c[u] = a.rope ? a.cos[turn] : 0; n[u] = a.rope ? a.sin[turn] : 0;
                 }
 #pragma unroll
                 for (int u = 0; u < PA_ROWS; u++) {

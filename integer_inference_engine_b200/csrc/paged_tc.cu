@@ -319,7 +319,7 @@ __device__ __forceinline__ TcLook tc_look(const PagedAttnArgs &a, const TcWalk &
     const int from = max(w.s.lo - pos, 0), to = min(w.s.len - pos, 8);
     if (from >= to) return x;
     x.rows = ((1u << to) - 1) & ~((1u << from) - 1);
-    x.page = __ldg(a.table + (long long)w.b * a.table_ld + logical);
+    x.page = a.table[(long long)w.b * a.table_ld + logical];
     return x;
 }
 __device__ __forceinline__ TcBoxes tc_boxes(const PagedAttnArgs &a, const TcLook &look, int kv, int box) {

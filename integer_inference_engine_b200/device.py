@@ -303,6 +303,8 @@ def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
         out = q.new_empty((B, n_heads * head_dim))
     elif out.dtype != torch.int64 or out.shape != (B, n_heads * head_dim) or not out.is_contiguous():
         raise ValueError("out must be a contiguous int64 [sequences, heads * head_dim]")
+    elif q.data_ptr() < out.data_ptr() + 8 * out.numel() and out.data_ptr() < q.data_ptr() + 8 * ((B - 1) * q_ld + n_heads * head_dim):
+        raise ValueError("out must not overlap q: other heads' queries are read while an output is written")
     cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
     lib = qk_cuda._lib()
     _on_current_device("q kpages vpages table lengths pages out cos sin", q, kpages, vpages, table, lengths, pages, out, cos if rope else None, sin if rope else None)

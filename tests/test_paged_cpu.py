@@ -57,6 +57,18 @@ def test_refused(case):
         call(name, {**good(), **change}, **dict(kw))
 
 
+def test_an_output_over_the_queries_is_refused():
+    """In place, one row on, and as columns of the matrix that holds the queries; beside them the path is taken (and finds no GPU, or tensors of another device)."""
+    w, wide = good(), torch.zeros(4, 256, dtype=I64)
+    for q, out in ((wide[:3], wide[:3]), (wide[:3], wide[1:]), (wide[1:], wide[:3])):
+        with pytest.raises(ValueError, match="overlap"):
+            call("attention", {**w, "q": q}, out=out)
+    both = torch.zeros(6, 256, dtype=I64)
+    with pytest.raises((ValueError, qk_cuda.CudaUnavailableError)) as e:
+        call("attention", {**w, "q": both[:3]}, out=both[3:])
+    assert "overlap" not in str(e.value)
+
+
 @pytest.mark.parametrize("name", ["append", "attention", "select"])
 def test_tensors_of_another_device_are_refused(name):
     """Good arguments on the CPU: without a GPU there is no path, with one they lie on the wrong device."""
