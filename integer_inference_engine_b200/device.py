@@ -176,17 +176,21 @@ def attention_decode_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc
     return out
 
 
+_I32, _I64 = torch.int32, torch.int64
+
+
 def _on_current_device(names: str, *tensors) -> None:
     """Every tensor given lies on the current device, where the kernels run."""
     here = torch.cuda.current_device()
-    for i, t in enumerate(tensors):
+    for t in tensors:
         if t is not None and t.get_device() != here:
-            raise ValueError(f"{names.split()[i]} lies on {t.device}, the current device is cuda:{here}")
+            name = next(n for n, u in zip(names.split(), tensors) if u is t)
+            raise ValueError(f"{name} lies on {t.device}, the current device is cuda:{here}")
 
 
 def _paged_pool(kpages: torch.Tensor, vpages: torch.Tensor) -> tuple:
     shape = kpages.shape
-    if len(shape) != 4 or shape != vpages.shape or kpages.dtype != torch.int32 or vpages.dtype != torch.int32:
+    if len(shape) != 4 or shape != vpages.shape or kpages.dtype != _I32 or vpages.dtype != _I32:
         raise ValueError("kpages and vpages must be int32 [pages, n_kv, page rows, head_dim] of one shape")
     if not (kpages.is_contiguous() and vpages.is_contiguous()) or 0 in shape:
         raise ValueError("kpages and vpages must be contiguous and not empty")
@@ -197,9 +201,9 @@ def _paged_pool(kpages: torch.Tensor, vpages: torch.Tensor) -> tuple:
 
 def _paged_table(table: torch.Tensor, name: str, each: torch.Tensor) -> tuple:
     shape = table.shape
-    if len(shape) != 2 or table.dtype != torch.int32 or not table.is_contiguous() or shape[1] == 0:
+    if len(shape) != 2 or table.dtype != _I32 or not table.is_contiguous() or shape[1] == 0:
         raise ValueError("table must be a contiguous int32 [sequences, pages of a sequence]")
-    if each.dtype != torch.int32 or each.shape != shape[:1] or not each.is_contiguous():
+    if each.dtype != _I32 or each.shape != shape[:1] or not each.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector with an entry per row of table")
     return shape
 
@@ -221,16 +225,17 @@ def _paged_rope(rope: int, cos, sin, head_dim: int) -> tuple:
         raise ValueError("rope is 0 (none), 1 (pairs 2i, 2i + 1) or 2 (pairs i, i + head_dim / 2)")
     if rope == 0:
         return None, None, 0
-    if cos is None or sin is None or cos.dtype != torch.int64 or sin.dtype != torch.int64 or cos.dim() != 2 or cos.shape[1] != head_dim // 2 or cos.shape != sin.shape \
-            or not (cos.is_contiguous() and sin.is_contiguous()):
-        raise ValueError("cos and sin must be contiguous int64 [positions, head_dim / 2] of one shape")
-    return cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    if cos is not None and sin is not None and cos.dtype == _I64 and sin.dtype == _I64:
+        shape = cos.shape
+        if len(shape) == 2 and shape[1] == head_dim // 2 and shape == sin.shape and cos.is_contiguous() and sin.is_contiguous():
+            return cos.data_ptr(), sin.data_ptr(), shape[0]
+    raise ValueError("cos and sin must be contiguous int64 [positions, head_dim / 2] of one shape")
 
 
 def _paged_query(q: torch.Tensor, n_seqs: int, n_kv: int, head_dim: int) -> tuple:
     """Query heads of q [sequences, heads * head_dim], and the distance of its rows."""
     shape = q.shape
-    if q.dtype == torch.int64 and len(shape) == 2 and shape[0] == n_seqs and shape[1] > 0 and shape[1] % (n_kv * head_dim) == 0:
+    if q.dtype == _I64 and len(shape) == 2 and shape[0] == n_seqs and shape[1] > 0 and shape[1] % (n_kv * head_dim) == 0:
         apart = _row_distance(q, shape)
         if apart >= 0:
             return shape[1] // head_dim, apart
@@ -252,23 +257,23 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages:
     outside the cache (it is left out) bit 4 of :func:`read_flags`."""
     n_pages, n_kv, page_rows, head_dim = _paged_pool(kpages, vpages)
     B, per_seq = _paged_table(table, "start", start)
-    narrow, width, shape = k.dtype == torch.int32, n_kv * head_dim, k.shape
-    if not (narrow or k.dtype == torch.int64) or v.dtype != k.dtype or len(shape) != 2 or shape != v.shape or shape[1] != width:
+    kind, width, shape = k.dtype, n_kv * head_dim, k.shape
+    if kind not in (_I64, _I32) or v.dtype != kind or len(shape) != 2 or shape != v.shape or shape[1] != width:
         raise ValueError("k and v must be int64 or int32 [rows, n_kv * head_dim] of one shape")
     k_ld, v_ld = _row_distance(k, shape), _row_distance(v, shape)
     if k_ld < 0 or v_ld < 0:
         raise ValueError("the columns of k and v must be adjacent and their rows must not overlap")
     if rows is None and shape[0] < B:
         raise ValueError("without rows, k and v need a row per sequence")
-    if rows is not None and (rows.dtype != torch.int32 or rows.shape != (B + 1,) or not rows.is_contiguous()):
+    if rows is not None and (rows.dtype != _I32 or rows.shape != (B + 1,) or not rows.is_contiguous()):
         raise ValueError("rows must be a contiguous int32 vector with one entry more than table has rows")
-    if bounds is not None and (bounds.dtype != torch.int32 or bounds.shape != (n_pages, n_kv, 2, head_dim) or not bounds.is_contiguous()):
+    if bounds is not None and (bounds.dtype != _I32 or bounds.shape != (n_pages, n_kv, 2, head_dim) or not bounds.is_contiguous()):
         raise ValueError("bounds must be a contiguous int32 [pages, n_kv, 2, head_dim]")
     cos_p, sin_p, rope_rows = _paged_rope(rope, cos, sin, head_dim)
     lib = qk_cuda._lib()
     _on_current_device("k v kpages vpages table start rows bounds cos sin", k, v, kpages, vpages, table, start, rows, bounds, cos if rope else None, sin if rope else None)
     with _CUDA_LOCK:
-        rc = lib.iie_paged_append_dev(k.data_ptr(), v.data_ptr(), narrow, k_ld, v_ld, shape[0],
+        rc = lib.iie_paged_append_dev(k.data_ptr(), v.data_ptr(), kind == _I32, k_ld, v_ld, shape[0],
                                       kpages.data_ptr(), vpages.data_ptr(), n_pages, page_rows, table.data_ptr(), per_seq, start.data_ptr(),
                                       rows.data_ptr() if rows is not None else None, B, cos_p, sin_p, rope_rows, int(rope), n_kv, head_dim, int(fa),
                                       bounds.data_ptr() if bounds is not None else None, _stream_ptr())
