@@ -128,6 +128,7 @@ struct TcWalk {
 //    the same one first, normalised between tiles as soon as the maxima are in, were no faster: the registers and the code that this takes cost the
 //    tiles what it hides.)
 enum { RUN_WHOLE = 2, RUNS };
+constexpr int PT_PAIR = 1;                         // what a pair costs beside its tiles, in tiles (64 x 4096 keys: 121 us with none, 118.3, 119.0 with two, 120.5 with three)
 __device__ __noinline__ int tc_count(const PagedAttnArgs &a, int b) {
     PagedSpan s;
     if (b >= a.B) return 0;
@@ -156,13 +157,13 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
         if ((int)__reduce_add_sync(0xffffffffu, ps) * per_seq <= ctas && (int)__reduce_max_sync(0xffffffffu, pl) <= average + 2) way = OWN_CTAS;
     }
     // the share in units of the way, and where in the list its first and last unit are
-    const int all = way == EVEN ? total : pairs;
+    const int all = way == EVEN ? total + PT_PAIR * pairs : pairs;
     const int from = way == OWN_CTAS ? me : (int)((uint32_t)all * me / ctas), to = way == OWN_CTAS ? me + 1 : (int)((uint32_t)all * (me + 1) / ctas);
     int at[2] = {-1, -1}, in[2] = {0, 0}, first[2] = {0, 0};       // sequence, unit in it, its first tile
     int before = 0, tiles_before = 0;              // units and tiles per pair of the sequences in front
 #pragma unroll 1
     for (int b0 = 0; b0 < a.B && from < to && (at[0] < 0 || at[1] < 0); b0 += 32) {
-        const int c = count(b0 + lane), mine = way == EVEN ? c : way == OWN_CTAS ? parts(c) : (int)(c > 0);
+        const int c = count(b0 + lane), mine = way == EVEN ? (c > 0) * (c + PT_PAIR) : way == OWN_CTAS ? parts(c) : (int)(c > 0);
         int upto = mine, tiles = c;
 #pragma unroll 1
         for (int d = 1; d < 32; d <<= 1) {
@@ -206,21 +207,27 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
         w.left = first[1] + (in[1] + 1) * e.nt - w.tile;
         run[RUN_WHOLE] = w;
     } else {
-        auto owner = [&](int tile) { return (int)((((uint32_t)tile + 1) * ctas - 1) / total); };
-        w.pair_of = in[0] / w.nt; w.t = in[0] - w.pair_of * w.nt;
-        w.left = to - from; w.tile = from;
-        w.owner = owner(w.tile - w.t); w.parts = owner(w.tile - w.t + w.nt - 1) - w.owner + 1;
-        if (w.rest() < w.nt) {
+        // a pair's units: PT_PAIR without a tile, then one a tile; a CTA has the tiles whose units it has
+        auto owner = [&](int unit) { return (int)((((uint32_t)unit + 1) * ctas - 1) / all); };
+        const int units = w.nt + PT_PAIR, units_e = e.nt + PT_PAIR;
+        w.pair_of = in[0] / units;
+        const int begins = from - (in[0] - w.pair_of * units) + PT_PAIR;       // unit of its first tile
+        w.t = max(0, from - begins);
+        w.tile = first[0] + w.pair_of * w.nt + w.t;
+        w.owner = owner(begins); w.parts = owner(begins + w.nt - 1) - w.owner + 1;
+        e.pair_of = in[1] / units_e;
+        const int begins_e = to - 1 - (in[1] - e.pair_of * units_e) + PT_PAIR;
+        e.left = max(0, to - begins_e);            // (none where the share ends in front of its first tile)
+        e.tile = first[1] + e.pair_of * e.nt;
+        e.owner = owner(begins_e); e.parts = owner(begins_e + e.nt - 1) - e.owner + 1;
+        w.left = e.tile + e.left - w.tile;
+        if (w.left > 0 && w.rest() < w.nt) {
             run[0] = w;
             run[0].left = w.rest();
             w.skip(a, per_seq, w.rest());
         }
         if (w.left > 0) {
-            e.pair_of = in[1] / e.nt;
-            e.left = in[1] - e.pair_of * e.nt + 1;
-            e.tile = to - e.left;
-            e.owner = owner(e.tile); e.parts = owner(e.tile + e.nt - 1) - e.owner + 1;
-            if (e.left < e.nt) { run[1] = e; w.left -= e.left; }
+            if (e.left > 0 && e.left < e.nt) { run[1] = e; w.left -= e.left; }
             run[RUN_WHOLE] = w;
         }
     }
