@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(256) paged_rank_kernel(const PagedSelectArgs a
 // Pages that always count apart, the rest by radix selection from the highest bit in which scores differ: eight bits a pass, until a bin ends
 // where the selection does (two passes as a rule; from the top byte, which nearly all share, every count would hit one bin).  Equal scores: the
 // lowest pages.  Then the pages in order.
-constexpr int PS_THREADS = 256;
+constexpr int PS_THREADS = 256, PK_HELD = 8192;    // scores that shared memory has room for
 struct PickScratch {
     int hist[256], scan[2][PS_THREADS / 32], digit, left, count;
     unsigned long long ends[2][PS_THREADS / 32];
@@ -447,36 +447,49 @@ __device__ __forceinline__ void pick_rest(const PagedSelectArgs &a, int first, i
         else if (n <= a.n_sel) out[i] = first + i;
 }
 
-__global__ void __launch_bounds__(PS_THREADS) paged_pick_kernel(const PagedSelectArgs a) {
+__global__ void __launch_bounds__(PS_THREADS) paged_pick_kernel(const PagedSelectArgs a, const bool held) {
     pdl_enter();
     __shared__ PickScratch s;
     const int kv = blockIdx.x, b = blockIdx.y;
     int first, n, *out;
     const bool rank = pick_begin(a, b, kv, first, n, out);
     pick_rest(a, first, n, out);
+    if (!rank) return;
+    extern __shared__ long long pk_score[];
     const long long *score = a.score + ((long long)b * a.Hkv + kv) * a.table_ld;
-    if (rank) pick_pages(a, s, first, n, out, [&](int i) { return score[i]; });
+    if (held) {                                    // (a pass over them in memory costs a microsecond)
+        for (int i = threadIdx.x; i < n; i += 8 * PS_THREADS) {
+            long long x[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) x[u] = score[min(i + u * PS_THREADS, n - 1)];
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                if (i + u * PS_THREADS < n) pk_score[i + u * PS_THREADS] = x[u];
+        }
+        __syncthreads();
+        score = pk_score;
+    }
+    pick_pages(a, s, first, n, out, [&](int i) { return score[i]; });
 }
 
-// Both in one launch where head dimension and page count allow: a cluster of CTAs per (sequence, KV head) ranks the pages, 64 at a time each,
+// Both in one launch where head dimension and page count allow (up to 1024: two turns of a cluster): a cluster of CTAs per (sequence, KV head) ranks the pages, 64 at a time each,
 // into the first CTA's shared memory, and that one picks.  A warp has the bounds of eight pages copied into shared memory (a page's 8 hd bytes lie
 // side by side; a gap behind each keeps the banks apart); four lanes share a page, a lane takes every fourth group of four dimensions of eight
 // heads: 32 x 32 -> 64-bit multiply-adds (four clocks a warp) of a query value with the bound that its sign selects (four clocks on the
-// other pipe).  What bounds it: those, and the longest sequence.  Eight sequences of up to 2000 pages (4 KV heads of two bounds of 128, 38500 pages, 39 MB) take 26 us:
-// 2 for the query, 16 for the four rounds of the longest (3 of each round's 4 are multiply-adds; memory alone would take 6 in all), 7 to pick.  (A page's
-// bounds copied as halves, the next ones' while the others are multiplied: 21 for the rounds, four times as many copies.  Loads into registers instead, two
-// pages a lane: four round trips a page, 20.)  A query beyond int32 takes 64-bit products.
+// other pipe).  What bounds it: those, 4 us a turn of 64 pages for two CTAs of an SM (3 of them multiply-adds), the query's 2 and picking's 3 to 7: 8.8 us for a sequence
+// of 500 pages (4 KV heads of two bounds of 128, 8 query heads each).  (A page's bounds copied as halves, the next ones' while the others are multiplied: a third
+// slower, four times as many copies.  Loads into registers instead, two pages a lane: four round trips a page, twice the time.)  A query beyond int32 takes
+// 64-bit products.
 constexpr int PR_PAGES = 8;                        // pages of a warp at a time
 constexpr int PR_GAP = 64;
-constexpr int PR_MOST = 8192;                      // pages of a sequence: 64 KB of scores
+constexpr int PR_CLUSTER = 8, PR_TURN = PR_PAGES * (PS_THREADS / 32), PR_MOST = 2 * PR_CLUSTER * PR_TURN;     // CTAs of a cluster; pages of one at a time; of a list for this form
 __host__ __device__ inline int rank_heads(int rep) { return rep <= 4 ? 4 : (rep + 7) / 8 * 8; }
 __host__ __device__ inline size_t rank_stage(int hd) { return (size_t)PR_PAGES * (8 * hd + PR_GAP); }       // of a warp
 template <bool WIDE, int HEADS>                   // HEADS at a time: the queries are padded with zeros to a multiple
 __device__ __forceinline__ bool rank_pages(const PagedSelectArgs &a, const int *q32, const int64_t *q64, unsigned char *stage, uint64_t *bar, int rep, int b, int kv, int first, int n, long long *to, int block,
-                                           int blocks, bool &bad, volatile int *abort_flag) {
+                                           int blocks, uint32_t &pass, bool &bad, volatile int *abort_flag) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, g = lane >> 2, ld = 8 * a.hd + PR_GAP;
     const uint32_t bar_at = tl_u32(bar), to_at = tl_u32(stage);
-    uint32_t pass = 0;
     const int step = blocks * (PS_THREADS / 32) * PR_PAGES;
     for (int p0 = (block * (PS_THREADS / 32) + warp) * PR_PAGES; p0 < n; p0 += step, pass ^= 1) {
         // the warp's pages; one outside the pool counts as lowest
@@ -541,6 +554,25 @@ __device__ __forceinline__ bool rank_pages(const PagedSelectArgs &a, const int *
     }
     return true;
 }
+// The queries of a KV head, rotated, as int64 and as int32: whether one of the thread's is beyond that.
+__device__ __forceinline__ bool rank_queries(const PagedSelectArgs &a, int b, int kv, int rep, int padded, int64_t *q64, int *q32) {
+    const int half = a.hd / 2;
+    bool wide = false;
+    const long long pos = a.lengths[b] - 1;
+    for (int idx = threadIdx.x; idx < padded * half; idx += PS_THREADS) {
+        const int h = idx / half, i = idx - h * half, d0 = a.rope == 2 ? i : 2 * i, d1 = a.rope == 2 ? i + half : 2 * i + 1;
+        int64_t x0 = 0, x1 = 0;
+        if (h < rep) {
+            const int64_t *src = a.q + b * a.q_ld + (long long)(kv * rep + h) * a.hd;
+            x0 = src[d0]; x1 = src[d1];
+            paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, pos, i, x0, x1);
+        }
+        q64[h * a.hd + d0] = x0; q64[h * a.hd + d1] = x1;
+        q32[h * a.hd + d0] = (int)x0; q32[h * a.hd + d1] = (int)x1;
+        wide = wide || x0 != (int)x0 || x1 != (int)x1;
+    }
+    return wide;
+}
 __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const PagedSelectArgs a) {
     pdl_enter();
     extern __shared__ __align__(16) int64_t pr_q[];                // queries [rep][hd] as int64, then as int32; the warps' pages; scores
@@ -548,7 +580,7 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const Paged
     __shared__ __align__(8) uint64_t s_bar[PS_THREADS / 32];
     __shared__ int s_wide, s_abort;
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, rep = a.H / a.Hkv, half = a.hd / 2, block = blockIdx.x, blocks = gridDim.x, kv = blockIdx.y, b = blockIdx.z;
+    const int tid = threadIdx.x, rep = a.H / a.Hkv, block = blockIdx.x, blocks = gridDim.x, kv = blockIdx.y, b = blockIdx.z;
     const int padded = rank_heads(rep);
     int *q32 = reinterpret_cast<int *>(pr_q + padded * a.hd);
     unsigned char *stage = reinterpret_cast<unsigned char *>(q32 + padded * a.hd);
@@ -567,33 +599,107 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const Paged
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    bool wide = false, bad = false;
-    const long long pos = a.lengths[b] - 1;
-    for (int idx = tid; idx < padded * half; idx += PS_THREADS) {
-        const int h = idx / half, i = idx - h * half, d0 = a.rope == 2 ? i : 2 * i, d1 = a.rope == 2 ? i + half : 2 * i + 1;
-        int64_t x0 = 0, x1 = 0;
-        if (h < rep) {
-            const int64_t *src = a.q + b * a.q_ld + (long long)(kv * rep + h) * a.hd;
-            x0 = src[d0]; x1 = src[d1];
-            paged_rotate(a.cos, a.sin, a.rope, a.hd, a.fa, pos, i, x0, x1);
-        }
-        pr_q[h * a.hd + d0] = x0; pr_q[h * a.hd + d1] = x1;
-        q32[h * a.hd + d0] = (int)x0; q32[h * a.hd + d1] = (int)x1;
-        wide = wide || x0 != (int)x0 || x1 != (int)x1;
-    }
+    bool bad = false;
+    uint32_t pass = 0;
+    const bool wide = rank_queries(a, b, kv, rep, padded, pr_q, q32);
     if (wide) s_wide = 1;
     if (blocks > 1) cluster.sync();                                // (the first CTA has started)
     else __syncthreads();
     long long *to = blocks > 1 ? cluster.map_shared_rank(score, 0) : score;
     unsigned char *mine = stage + (tid >> 5) * rank_stage(a.hd);
-    const bool ok = s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort)
-                  : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort)
-                             : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, bad, &s_abort);
+    const bool ok = s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, pass, bad, &s_abort)
+                  : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, pass, bad, &s_abort)
+                             : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, pass, bad, &s_abort);
     if (!ok) atomicOr(a.flags, FLAG_GAVE_UP);
     if (bad) atomicOr(a.flags, 16);
     if (blocks > 1) cluster.sync();
     else __syncthreads();
     if (block == 0) pick_pages(a, s, first, n, out, [&](int i) { return score[i]; });
+}
+
+// Longer lists, in a launch of their own: the pages of all sequences and KV heads shared evenly, each pair of them by CTAs in proportion to its pages
+// (whole groups of eight), two CTAs an SM.  Against clusters, both in one call alone: 1 x 1000 pages 13.5 and 12.5 us, 1 x 2000 15.9 and 19.6, 8 x up to 2000 27.4 and 29.7,
+// 1 x 8000 33.5 and 60.6.  Of the 27: plan 2, the part's place and query 2, ranking 12 to 15 (multiply-adds 8 of them), launch between 1, picking 5.
+__global__ void __launch_bounds__(PS_THREADS, 2) paged_rank_even_kernel(const PagedSelectArgs a) {
+    pdl_enter();
+    extern __shared__ __align__(16) int64_t pr_q[];                // queries as int64, then as int32; the warps' pages
+    __shared__ __align__(8) uint64_t s_bar[PS_THREADS / 32];
+    __shared__ int s_wide, s_abort, s_b, s_kv, s_from, s_count, s_first;
+    __shared__ long long s_units;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rep = a.H / a.Hkv, padded = rank_heads(rep), ctas = gridDim.x;
+    int *q32 = reinterpret_cast<int *>(pr_q + padded * a.hd);
+    unsigned char *mine = reinterpret_cast<unsigned char *>(q32 + padded * a.hd) + warp * rank_stage(a.hd);
+    if (tid == 0) {
+        s_abort = 0;
+        for (int w = 0; w < PS_THREADS / 32; w++) tl_init(tl_u32(&s_bar[w]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // pages of a sequence that are ranked; the first visible one
+    auto pages = [&](int b, int &first) {
+        PagedSpan s;
+        first = 0;
+        if (b >= a.B) return 0;
+        if (!paged_span(a, b, s)) { if (blockIdx.x == 0) atomicOr(a.flags, 16); return 0; }
+        first = s.lo / a.P;
+        const int n = s.len > 0 ? (s.len - 1) / a.P - first + 1 : 0;
+        return n > a.n_sel ? n : 0;
+    };
+    auto added = [&](long long x) {
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+        return x;
+    };
+    int quota = 1, first0 = 0, n0 = 0, first;                      // of warp 0: pages of a CTA on average; those of the first 32 sequences
+    // pages of a part, parts
+    auto parts_most = [&](int n) { return max(1, n / quota); };
+    auto size = [&](int n) { const int p = parts_most(n); return ((n + p - 1) / p + PR_PAGES - 1) / PR_PAGES * PR_PAGES; };
+    auto parts = [&](int n) { return n == 0 ? 0 : (n + size(n) - 1) / size(n); };
+    if (warp == 0) {
+        n0 = pages(lane, first0);
+        long long total = n0, units = 0;
+        for (int b = lane + 32; b - lane < a.B; b += 32) total += pages(b, first);
+        total = added(total) * a.Hkv;
+        quota = (int)max(1LL, min((total + ctas - 1) / ctas, (long long)INT32_MAX));
+        units = parts(n0);
+        for (int b = lane + 32; b - lane < a.B; b += 32) units += parts(pages(b, first));
+        units = added(units) * a.Hkv;
+        if (lane == 0) s_units = units;
+    }
+    __syncthreads();
+    const long long units = s_units;
+    uint32_t pass = 0;
+    bool bad = false, ok = true;
+    for (long long unit = blockIdx.x; unit < units; unit += ctas) {
+        if (warp == 0) {                                           // its sequence, KV head, pages
+            long long before = 0;
+            for (int b0 = 0; b0 < a.B; b0 += 32) {
+                first = first0;
+                const int n = b0 ? pages(b0 + lane, first) : n0, each = parts(n), own = each * a.Hkv;
+                long long upto = own;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) { const long long o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
+                const int in = (int)max(-1LL, min(unit - (before + upto - own), 1LL << 30));
+                if (in >= 0 && in < own) {
+                    const int kv = in / each, at = (in - kv * each) * size(n);
+                    s_b = b0 + lane; s_kv = kv; s_from = at; s_count = min(size(n), n - at); s_first = first;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
+                if (before > unit) break;
+            }
+        }
+        if (tid == 0) s_wide = 0;
+        __syncthreads();
+        const int b = s_b, kv = s_kv, from = s_first + s_from, n = s_count;
+        if (rank_queries(a, b, kv, rep, padded, pr_q, q32)) s_wide = 1;
+        long long *to = a.score + ((long long)b * a.Hkv + kv) * a.table_ld + s_from;
+        __syncthreads();
+        ok = ok && (s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, 0, 1, pass, bad, &s_abort)
+                    : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, 0, 1, pass, bad, &s_abort)
+                               : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, 0, 1, pass, bad, &s_abort));
+        __syncthreads();
+    }
+    if (!ok) atomicOr(a.flags, FLAG_GAVE_UP);
+    if (bad) atomicOr(a.flags, 16);
 }
 
 // a device's first launch of a kernel sets its attributes
@@ -652,16 +758,16 @@ cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s) {
 
 cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
     const int rep = a.H / a.Hkv;
-    const size_t fused = (size_t)rank_heads(rep) * a.hd * 12 + PS_THREADS / 32 * rank_stage(a.hd) + (size_t)a.table_ld * 8;
-    if (a.hd % 16 == 0 && a.table_ld <= PR_MOST && fused <= 220 * 1024 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0) {
+    const size_t rank = (size_t)rank_heads(rep) * a.hd * 12 + PS_THREADS / 32 * rank_stage(a.hd), fused = rank + (size_t)a.table_ld * 8;
+    const bool staged = a.hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0 && rank <= 215 * 1024;
+    if (staged && a.table_ld <= PR_MOST) {
         static std::atomic<unsigned long long> configured;
         cudaError_t e = paged_once(configured, [] {
             const cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
             return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         });
         if (e != cudaSuccess) return e;
-        // a cluster of up to eight, a round of 64 pages for each
-        const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>(8, (a.table_ld + 63) / (PR_PAGES * (PS_THREADS / 32))));
+        const unsigned blocks = (unsigned)std::min<long long>(PR_CLUSTER, (a.table_ld + PR_TURN - 1) / PR_TURN);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(blocks, (unsigned)a.Hkv, (unsigned)a.B); cfg.blockDim = dim3(PS_THREADS); cfg.dynamicSmemBytes = fused; cfg.stream = s;
         cudaLaunchAttribute attr[2];
@@ -673,13 +779,23 @@ cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
         note_launch();
         return e != cudaSuccess ? e : cudaGetLastError();
     }
-    const size_t smem = (size_t)rep * a.hd * 8;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(paged_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
-    launch_behind(paged_rank_kernel, dim3((unsigned)((a.table_ld + 31) / 32), a.Hkv, a.B), 256, smem, s, a);
-    const cudaError_t e = launch_behind(paged_pick_kernel, dim3(a.Hkv, a.B), PS_THREADS, 0, s, a);
+    static std::atomic<unsigned long long> configured;
+    cudaError_t e = paged_once(configured, [] {
+        cudaError_t e = cudaFuncSetAttribute(paged_rank_even_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_rank_even_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PK_HELD * 8);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_pick_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    });
+    if (e != cudaSuccess) return e;
+    if (staged) {
+        const int sms = paged_sms();
+        if (sms <= 0) return cudaErrorInvalidDevice;
+        e = launch_behind(paged_rank_even_kernel, dim3(2 * sms), PS_THREADS, rank, s, a);
+    } else e = launch_behind(paged_rank_kernel, dim3((unsigned)((a.table_ld + 31) / 32), a.Hkv, a.B), 256, (size_t)rep * a.hd * 8, s, a);
+    if (e != cudaSuccess) return e;
+    const bool held = a.table_ld <= PK_HELD;
+    e = launch_behind(paged_pick_kernel, dim3(a.Hkv, a.B), PS_THREADS, held ? (size_t)a.table_ld * 8 : 0, s, a, held);
     note_launch(2);
     return e != cudaSuccess ? e : cudaGetLastError();
 }

@@ -55,6 +55,7 @@ cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s);
 bool paged_tc_ok(const PagedAttnArgs &a);
 size_t paged_tc_bytes(const PagedAttnArgs &a);
 cudaError_t launch_paged_tc(const PagedAttnArgs &a, cudaStream_t s);
+int paged_sms();                   // SMs of the current device (0: no device)
 
 struct PagedSelectArgs {
     const int64_t *q;

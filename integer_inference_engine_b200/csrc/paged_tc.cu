@@ -960,15 +960,6 @@ bool tc_map(CUtensorMap *map, const int32_t *pool, const PagedAttnArgs &a) {
                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// SMs of the current device: CTAs of a launch at most (one is resident on each, as a cooperative launch needs)
-int tc_sms(int device) {
-    static std::atomic<int> known[64];
-    if (device >= 0 && device < 64 && known[device] > 0) return known[device];
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return 0; }
-    if (device >= 0 && device < 64) known[device] = n;
-    return n;
-}
 constexpr int PT_MOST_CTAS = 256;                  // that the scratch has room for
 
 template <bool AT16, bool SMALL, int N>
@@ -979,7 +970,7 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return e;
-    const int sms = tc_sms(device);
+    const int sms = paged_sms();                   // one CTA is resident on each, as a cooperative launch needs
     if (sms <= 0) return cudaErrorInvalidDevice;
     const size_t fixed = 1024 + 2 * (size_t)chunks * padded * 1024 + PT_SETS * PT_PROBS, room = 227 * 1024 - sizeof(TcBars) - 64;
     const int slots = (int)std::min<size_t>(PT_MAX_SLOTS, (room - fixed) / PT_SLOT);
@@ -1016,6 +1007,16 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
 }
 
 }  // namespace
+
+int paged_sms() {
+    static std::atomic<int> known[64];
+    int device = 0, n = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) { cudaGetLastError(); return 0; }
+    if (device < 64 && known[device] > 0) return known[device];
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) { cudaGetLastError(); return 0; }
+    if (device < 64) known[device] = n;
+    return n;
+}
 
 // Rows that are whole 128-byte chunks (up to four), pages of whole groups of eight rows, probabilities of three bytes, a list whose place times the
 // CTAs fits 32 bits.

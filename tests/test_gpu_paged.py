@@ -291,6 +291,44 @@ def test_select_of_many_pages():
         assert np.array_equal(got.cpu().numpy(), po.select(q, bounds, table, [n], 1, n_select, 1, 1, 16, 0, None, None, 0))
 
 
+# lists of more than 1024 pages, ranked by all SMs together
+LONG = [
+    (12, 1, 128, 16, [20000, 16000, 1], 0, 2, 40, 3, 2, 18),
+    (4, 2, 64, 8, [12000, 0, 300, 9000], 5000, 2, 33, 1, 1, 62),
+    (8, 4, 80, 4, [5000, 4097, 130], 0, 1, 32, 0, 0, 18),
+    (2, 1, 32, 1, [1500, 0, 3, 40, 200] * 9, 0, 1, 30, 1, 1, 18),
+    (16, 8, 32, 1, [1100], 0, 0, 1100, 1, 1, 18),
+    (3, 1, 16, 2, [2600, 2500], 0, 1, 1, 0, 1, 18),
+]
+
+
+@pytest.mark.parametrize("shape", LONG, ids=[f"{c[0]}x{c[1]}x{c[2]}-p{c[3]}" for c in LONG])
+@pytest.mark.parametrize("flat", [False, True])
+def test_select_from_long_lists(shape, flat):
+    test_select(shape, flat)
+
+
+def test_select_from_a_long_list_with_a_page_outside():
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(12)
+    n, hd = 1500, 64
+    bounds = np.sort(rng.integers(-1000, 1000, size=(n, 2, 2, hd)), axis=2)[:, :, ::-1].astype(np.int32)
+    table = rng.permutation(n).astype(np.int32)[None].repeat(2, 0)
+    q = rng.integers(-1000, 1000, size=(2, 4 * hd), dtype=np.int64)
+    device.read_flags()
+    call = lambda t, lens: device.paged_select(dev(q), dev(bounds), dev(t), dev(np.array(lens, np.int32)), 1, 20, 0, 0).cpu().numpy()
+    good = call(table, [n, n - 7])
+    assert device.read_flags() == 0
+    best = good[0, 0, 0]
+    for wrong in (-1, n, 1 << 30):
+        other = table.copy()
+        other[0, best] = wrong                     # never chosen: the twenty best are others
+        got = call(other, [n, n - 7])
+        assert device.read_flags() == 16 and best not in got[0] and np.array_equal(got[1], good[1])
+    got = call(table, [n + 1, n - 7])              # a length beyond the table: none of its pages
+    assert device.read_flags() == 16 and (got[0] == -1).all() and np.array_equal(got[1], good[1])
+
+
 def test_rows_of_a_wider_matrix_and_a_given_output():
     import torch
 
