@@ -486,12 +486,12 @@ constexpr int PR_CLUSTER = 8, PR_TURN = PR_PAGES * (PS_THREADS / 32), PR_MOST = 
 __host__ __device__ inline int rank_heads(int rep) { return rep <= 4 ? 4 : (rep + 7) / 8 * 8; }
 __host__ __device__ inline size_t rank_stage(int hd) { return (size_t)PR_PAGES * (8 * hd + PR_GAP); }       // of a warp
 template <bool WIDE, int HEADS>                   // HEADS at a time: the queries are padded with zeros to a multiple
-__device__ __forceinline__ bool rank_pages(const PagedSelectArgs &a, const int *q32, const int64_t *q64, unsigned char *stage, uint64_t *bar, int rep, int b, int kv, int first, int n, long long *to, int block,
+__device__ __forceinline__ bool rank_pages(const PagedSelectArgs &a, const int *q32, const int64_t *q64, unsigned char *stage, uint64_t *bar, int rep, int b, int kv, int first, int n, long long *to, int turn, int block,
                                            int blocks, uint32_t &pass, bool &bad, volatile int *abort_flag) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, g = lane >> 2, ld = 8 * a.hd + PR_GAP;
+    const int lane = threadIdx.x & 31, t = lane & 3, g = lane >> 2, ld = 8 * a.hd + PR_GAP;
     const uint32_t bar_at = tl_u32(bar), to_at = tl_u32(stage);
     const int step = blocks * (PS_THREADS / 32) * PR_PAGES;
-    for (int p0 = (block * (PS_THREADS / 32) + warp) * PR_PAGES; p0 < n; p0 += step, pass ^= 1) {
+    for (int p0 = (block * (PS_THREADS / 32) + turn) * PR_PAGES; p0 < n; p0 += step, pass ^= 1) {
         // the warp's pages; one outside the pool counts as lowest
         int page = -1;
         if (lane < PR_PAGES && p0 + lane < n) {
@@ -607,9 +607,9 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const Paged
     else __syncthreads();
     long long *to = blocks > 1 ? cluster.map_shared_rank(score, 0) : score;
     unsigned char *mine = stage + (tid >> 5) * rank_stage(a.hd);
-    const bool ok = s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, pass, bad, &s_abort)
-                  : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, pass, bad, &s_abort)
-                             : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, block, blocks, pass, bad, &s_abort);
+    const bool ok = s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, tid >> 5, block, blocks, pass, bad, &s_abort)
+                  : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, tid >> 5, block, blocks, pass, bad, &s_abort)
+                             : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[tid >> 5], rep, b, kv, first, n, to, tid >> 5, block, blocks, pass, bad, &s_abort);
     if (!ok) atomicOr(a.flags, FLAG_GAVE_UP);
     if (bad) atomicOr(a.flags, 16);
     if (blocks > 1) cluster.sync();
@@ -618,8 +618,10 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const Paged
 }
 
 // Longer lists, in a launch of their own: the pages of all sequences and KV heads shared evenly, each pair of them by CTAs in proportion to its pages
-// (whole groups of eight), two CTAs an SM.  Against clusters, both in one call alone: 1 x 1000 pages 13.5 and 12.5 us, 1 x 2000 15.9 and 19.6, 8 x up to 2000 27.4 and 29.7,
-// 1 x 8000 33.5 and 60.6.  Of the 27: plan 2, the part's place and query 2, ranking 12 to 15 (multiply-adds 8 of them), launch between 1, picking 5.
+// (whole groups of eight), two CTAs an SM.  For lists of more than 1024 pages, or of more than 128 where the clusters would not all be resident at once.  Both forms, a call alone,
+// us (clusters first): 1 x 1000 pages 12.5 and 13.5, 1 x 2000 19.6 and 15.9, 1 x 8000 60.6 and 33.5; 8 x 500 13.9 and 19.4, 16 x 500 24.0 and 21.6, 32 x 1000 70.5 and 64.4; 64 x 200 38.6 and
+// 32.2, 150 x 120 45.1 and 53.1, 300 x 60 41.7 and 65.4; 8 x up to 2000 29.7 and 27.1: plan 2, the part's place and query 2, ranking 11 to 15 (multiply-adds 8 of them), the launch
+// between 1, picking 5.
 __global__ void __launch_bounds__(PS_THREADS, 2) paged_rank_even_kernel(const PagedSelectArgs a) {
     pdl_enter();
     extern __shared__ __align__(16) int64_t pr_q[];                // queries as int64, then as int32; the warps' pages
@@ -667,6 +669,7 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_rank_even_kernel(const Pa
     }
     __syncthreads();
     const long long units = s_units;
+    const int turn = (warp + 2 * ((blockIdx.x & 1) ^ (blockIdx.x >= ctas / 2))) & 7;      // (warps with a group more of an SM's two CTAs issue from different places)
     uint32_t pass = 0;
     bool bad = false, ok = true;
     for (long long unit = blockIdx.x; unit < units; unit += ctas) {
@@ -693,9 +696,9 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_rank_even_kernel(const Pa
         if (rank_queries(a, b, kv, rep, padded, pr_q, q32)) s_wide = 1;
         long long *to = a.score + ((long long)b * a.Hkv + kv) * a.table_ld + s_from;
         __syncthreads();
-        ok = ok && (s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, 0, 1, pass, bad, &s_abort)
-                    : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, 0, 1, pass, bad, &s_abort)
-                               : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, 0, 1, pass, bad, &s_abort));
+        ok = ok && (s_wide ? rank_pages<true, 4>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, turn, 0, 1, pass, bad, &s_abort)
+                    : rep <= 4 ? rank_pages<false, 4>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, turn, 0, 1, pass, bad, &s_abort)
+                               : rank_pages<false, 8>(a, q32, pr_q, mine, &s_bar[warp], rep, b, kv, from, n, to, turn, 0, 1, pass, bad, &s_abort));
         __syncthreads();
     }
     if (!ok) atomicOr(a.flags, FLAG_GAVE_UP);
@@ -760,14 +763,16 @@ cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
     const int rep = a.H / a.Hkv;
     const size_t rank = (size_t)rank_heads(rep) * a.hd * 12 + PS_THREADS / 32 * rank_stage(a.hd), fused = rank + (size_t)a.table_ld * 8;
     const bool staged = a.hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0 && rank <= 215 * 1024;
-    if (staged && a.table_ld <= PR_MOST) {
+    const int sms = paged_sms();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    const unsigned blocks = (unsigned)std::min<long long>(PR_CLUSTER, (a.table_ld + PR_TURN - 1) / PR_TURN);
+    if (staged && a.table_ld <= PR_MOST && (a.table_ld <= 2 * PR_TURN || (long long)blocks * a.Hkv * a.B <= 2 * sms)) {
         static std::atomic<unsigned long long> configured;
         cudaError_t e = paged_once(configured, [] {
             const cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
             return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         });
         if (e != cudaSuccess) return e;
-        const unsigned blocks = (unsigned)std::min<long long>(PR_CLUSTER, (a.table_ld + PR_TURN - 1) / PR_TURN);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(blocks, (unsigned)a.Hkv, (unsigned)a.B); cfg.blockDim = dim3(PS_THREADS); cfg.dynamicSmemBytes = fused; cfg.stream = s;
         cudaLaunchAttribute attr[2];
@@ -789,8 +794,6 @@ cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
     });
     if (e != cudaSuccess) return e;
     if (staged) {
-        const int sms = paged_sms();
-        if (sms <= 0) return cudaErrorInvalidDevice;
         e = launch_behind(paged_rank_even_kernel, dim3(2 * sms), PS_THREADS, rank, s, a);
     } else e = launch_behind(paged_rank_kernel, dim3((unsigned)((a.table_ld + 31) / 32), a.Hkv, a.B), 256, (size_t)rep * a.hd * 8, s, a);
     if (e != cudaSuccess) return e;

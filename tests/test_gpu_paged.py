@@ -291,7 +291,7 @@ def test_select_of_many_pages():
         assert np.array_equal(got.cpu().numpy(), po.select(q, bounds, table, [n], 1, n_select, 1, 1, 16, 0, None, None, 0))
 
 
-# lists of more than 1024 pages, ranked by all SMs together
+# lists of more than 1024 pages, and many of more than 128, ranked by all SMs together
 LONG = [
     (12, 1, 128, 16, [20000, 16000, 1], 0, 2, 40, 3, 2, 18),
     (4, 2, 64, 8, [12000, 0, 300, 9000], 5000, 2, 33, 1, 1, 62),
@@ -299,6 +299,7 @@ LONG = [
     (2, 1, 32, 1, [1500, 0, 3, 40, 200] * 9, 0, 1, 30, 1, 1, 18),
     (16, 8, 32, 1, [1100], 0, 0, 1100, 1, 1, 18),
     (3, 1, 16, 2, [2600, 2500], 0, 1, 1, 0, 1, 18),
+    (8, 4, 32, 1, [150, 7, 130, 0, 21] * 10, 0, 1, 20, 1, 1, 18),
 ]
 
 
