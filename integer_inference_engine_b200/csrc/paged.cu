@@ -672,24 +672,25 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_rank_even_kernel(const Pa
     const int turn = (warp + 2 * ((blockIdx.x & 1) ^ (blockIdx.x >= ctas / 2))) & 7;      // (warps with a group more of an SM's two CTAs issue from different places)
     uint32_t pass = 0;
     bool bad = false, ok = true;
+    int b0 = 0;                                                    // of warp 0: sequences searched so far, their parts
+    long long before = 0;
     for (long long unit = blockIdx.x; unit < units; unit += ctas) {
-        if (warp == 0) {                                           // its sequence, KV head, pages
-            long long before = 0;
-            for (int b0 = 0; b0 < a.B; b0 += 32) {
+        if (warp == 0)                                             // its sequence, KV head, pages; the search goes on where the last one ended
+            for (; b0 < a.B; b0 += 32) {
                 first = first0;
                 const int n = b0 ? pages(b0 + lane, first) : n0, each = parts(n), own = each * a.Hkv;
                 long long upto = own;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) { const long long o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
-                const int in = (int)max(-1LL, min(unit - (before + upto - own), 1LL << 30));
+                const long long in = unit - (before + upto - own);
                 if (in >= 0 && in < own) {
-                    const int kv = in / each, at = (in - kv * each) * size(n);
+                    const int kv = (int)in / each, at = ((int)in - kv * each) * size(n);
                     s_b = b0 + lane; s_kv = kv; s_from = at; s_count = min(size(n), n - at); s_first = first;
                 }
-                before += __shfl_sync(0xffffffffu, upto, 31);
-                if (before > unit) break;
+                const long long behind = before + __shfl_sync(0xffffffffu, upto, 31);
+                if (behind > unit) break;
+                before = behind;
             }
-        }
         if (tid == 0) s_wide = 0;
         __syncthreads();
         const int b = s_b, kv = s_kv, from = s_first + s_from, n = s_count;

@@ -300,6 +300,7 @@ LONG = [
     (16, 8, 32, 1, [1100], 0, 0, 1100, 1, 1, 18),
     (3, 1, 16, 2, [2600, 2500], 0, 1, 1, 0, 1, 18),
     (8, 4, 32, 1, [150, 7, 130, 0, 21] * 10, 0, 1, 20, 1, 1, 18),
+    (2, 1, 16, 1, [0] * 70 + [140, 129, 12] * 110, 0, 0, 11, 1, 1, 18),
 ]
 
 
