@@ -407,8 +407,8 @@ __device__ __forceinline__ void tc_producer(const PagedAttnArgs &a, const CUtens
 }
 
 // Query columns of one pair: column 8 h + s holds digit s - b of q_i at byte 4 i + b, bytes 0 .. 2 in one operand and byte 3 in the other.
-// A thread rotates one value and writes its word of the eight columns: little code, fetched once and run once, is what counts (a thread with four
-// values and columns, whole 16 bytes at a time, took 2.1 us instead of 1.1).
+// A thread rotates one value and writes its word of the eight columns; 3 us from the share to the last word, a round trip for queries and tables and code that is
+// fetched once and run once (a thread with four values and columns, 16 bytes at a time, took no less).
 __device__ __forceinline__ void tc_queries(const PagedAttnArgs &a, const TcWalk &w, int heads, int padded, unsigned char *lower, unsigned char *upper, int worker) {
     const int groups = tc_head_groups(a), kv = w.pair_of / groups, h0 = kv * (a.H / a.Hkv) + (w.pair_of % groups) * tc_group_heads(a), half = a.hd / 2;
     const int at_once = 32 * PT_WORKERS / a.hd, d = worker % a.hd;
