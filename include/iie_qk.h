@@ -237,7 +237,8 @@ int iie_paged_append_dev(const void *k_dev, const void *v_dev, int narrow, long 
  * lengths_dev[i] - 1, its key and value already in the cache; lengths_dev[i] = 0: no sequence, its output row is zero.  max_length bounds the
  * lengths.  window > 0: the last `window` keys.  selected_dev (nullable) [n_seqs][n_kv][n_selected]: only the rows of these logical pages
  * count, every entry as it stands, negative ones not at all.  Arithmetic of iie_attn_decode_dev over the keys that count.  work_dev: at
- * least iie_paged_attn_bytes (-1: bad argument) bytes.  The pools and work_dev start on 16 bytes; n_pages * n_kv * page_rows is below 2^31.  out_dev [n_seqs][n_heads * head_dim]. */
+ * least iie_paged_attn_bytes (-1: bad argument) bytes.  The pools and work_dev start on 16 bytes; n_pages * n_kv * page_rows is below 2^31.
+ * out_dev [n_seqs][n_heads * head_dim] overlaps none of the inputs. */
 long long iie_paged_attn_bytes(long long n_seqs, long long max_length, long long window, int n_selected, long long page_rows, int n_heads,
                                int n_kv, int head_dim, int fa);
 int iie_paged_attn_dev(const int64_t *q_dev, long long q_ld, const int32_t *kpages_dev, const int32_t *vpages_dev, long long n_pages,
