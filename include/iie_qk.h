@@ -221,8 +221,9 @@ int iie_attn_decode_batch_rows_dev(const int64_t *q_dev, const int64_t *k_dev, c
  * table_dev [n_seqs][table_ld]: physical page of every logical page of a sequence, position t being row t % page_rows of logical page
  * t / page_rows.  Sequences may share pages that none of them appends to.  cos_dev / sin_dev [rope_rows][head_dim / 2]; rope as above.
  * Positions, lengths and page numbers are read on the device: what lies outside the pool, the table or the rotation rows raises bit 4 of the
- * flag word and is left out.  All entries: 0 ok, 1 bad argument or CUDA failure; asynchronous on `stream`; they allocate nothing and share
- * no scratch, so calls on different streams may overlap and captured calls stay valid as long as the caller's buffers.
+ * flag word and is left out.  All entries: 0 ok, 1 bad argument, CUDA failure or a current device other than that of the library's first use;
+ * asynchronous on `stream`; they allocate nothing and share no scratch, so calls on different streams may overlap and captured calls stay valid
+ * as long as the caller's buffers.
  *
  * Append: `tokens` rows of keys and values [n_kv * head_dim], int64 (narrow = 0) or int32 (1), k_ld / v_ld apart.  Sequence i takes rows
  * rows_dev[i] .. rows_dev[i + 1] - 1 (rows_dev NULL: row i, one each) as its positions start_dev[i], start_dev[i] + 1, ...; a negative start

@@ -68,6 +68,7 @@ int g_attn_parity = 0;                // which of the two attention digit-count 
 long long g_tc_min_tokens = 0;        // from this many rows on, products run on the tcgen05 tiles (0: by size, see linear_dev and moe_fused)
 constexpr long long TILES_FROM = 192; // rows from which every product takes the tiles
 int g_ready = -1;                     // -1 unknown, 0 usable, 1 unusable
+int g_home = -1;                      // device that was current then: where the flag word and the workspaces are
 int g_stage_mask = 0;                 // profiling: when non-zero, iie_moe_forward_dev runs only these stages
 enum Stage { ST_LIMBS = 1, ST_ROUTER = 2, ST_TOPK = 4, ST_GATEUP = 8, ST_DOWN = 16 };
 inline bool stage_on(int st) { return g_stage_mask == 0 || (g_stage_mask & st); }
@@ -85,7 +86,7 @@ unsigned long long g_ws_generation = 0;
 bool init() {
     if (g_ready >= 0) return g_ready == 0;
     int n = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess || n <= 0) { cudaGetLastError(); g_ready = 1; return false; }
+    if (cudaGetDeviceCount(&n) != cudaSuccess || n <= 0 || cudaGetDevice(&g_home) != cudaSuccess) { cudaGetLastError(); g_ready = 1; return false; }
     if (cudaStreamCreateWithFlags(&g_stream, cudaStreamNonBlocking) != cudaSuccess ||
         cudaMalloc(&g_flags, sizeof(int)) != cudaSuccess || cudaMemset(g_flags, 0, sizeof(int)) != cudaSuccess ||
         cudaMalloc(&g_cells, 2048) != cudaSuccess || cudaMemset(g_cells, 0, 2048) != cudaSuccess ||
@@ -604,6 +605,10 @@ namespace iie {
 int *shared_flag_word() {
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     return init() ? flag_word() : nullptr;
+}
+bool library_is_here() {
+    int device = -1;
+    return cudaGetDevice(&device) == cudaSuccess && device == g_home;
 }
 int *set_flag_word(int *word) { return std::exchange(t_flags, word); }
 void restore_flag_bits(int bits) {

@@ -439,6 +439,7 @@ cudaError_t launch_rmsnorm_pair(const int64_t *x, long long rows_a, long long ro
                                 const int64_t *gain_b, int fa, unsigned long long eps, int64_t *out, int *flags, cudaStream_t s);
 bool attn_shape_ok(int n_heads, int n_kv, int head_dim);      // shapes launch_attn_decode accepts
 int *shared_flag_word();           // the library's device flag word (or the thread's own, see below), NULL without a device
+bool library_is_here();            // whether the current device is the one where that word is
 // Until the next call kernels that this thread launches through the attention and 1-bit entries raise their flags in `word` (null: in the
 // shared one); returns the word before.
 int *set_flag_word(int *word);

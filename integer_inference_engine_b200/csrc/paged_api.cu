@@ -55,7 +55,7 @@ extern "C" int iie_paged_append_dev(const void *k_dev, const void *v_dev, int na
         k_ld < (long long)n_kv * head_dim || v_ld < (long long)n_kv * head_dim || (!rows_dev && tokens < n_seqs)) return 1;
     if (n_seqs == 0 || tokens == 0) return 0;
     int *flags = shared_flag_word();
-    if (!flags || !k_dev || !v_dev || !kpages_dev || !vpages_dev || !table_dev || !start_dev) return 1;
+    if (!flags || !library_is_here() || !k_dev || !v_dev || !kpages_dev || !vpages_dev || !table_dev || !start_dev) return 1;
     PagedAppendArgs a = {};
     a.k = k_dev; a.v = v_dev; a.narrow = narrow != 0; a.k_ld = k_ld; a.v_ld = v_ld; a.kpages = kpages_dev; a.vpages = vpages_dev;
     a.n_pages = (int)n_pages; a.P = (int)page_rows; a.table = table_dev; a.table_ld = table_ld; a.start = start_dev; a.rows = rows_dev; a.T = tokens; a.B = (int)n_seqs;
@@ -83,7 +83,7 @@ extern "C" int iie_paged_attn_dev(const int64_t *q_dev, long long q_ld, const in
     if (n_seqs == 0) return 0;
     int *flags = shared_flag_word();
     const long long need = iie_paged_attn_bytes(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim, fa);
-    if (!flags || !q_dev || !kpages_dev || !vpages_dev || !table_dev || !lengths_dev || !out_dev || need < 0 || work_bytes < need || (need > 0 && !work_dev)) return 1;
+    if (!flags || !library_is_here() || !q_dev || !kpages_dev || !vpages_dev || !table_dev || !lengths_dev || !out_dev || need < 0 || work_bytes < need || (need > 0 && !work_dev)) return 1;
     PagedAttnArgs a = attn_shape(n_seqs, max_length, window, n_selected, page_rows, n_heads, n_kv, head_dim, fa);
     a.q_ld = q_ld; a.kpages = kpages_dev; a.vpages = vpages_dev; a.n_pages = (int)n_pages; a.table_ld = table_ld;
     a.cos = cos_dev; a.sin = sin_dev; a.rope_rows = rope_rows; a.rope = rope; a.inv_sqrt = inv_sqrt; a.log2e = sigmoid_log2e(fa);
@@ -108,7 +108,7 @@ extern "C" int iie_paged_select_dev(const int64_t *q_dev, long long q_ld, const 
         (long long)(n_heads / n_kv) * head_dim * 8 > 200 * 1024) return 1;
     if (n_seqs == 0) return 0;
     int *flags = shared_flag_word();
-    if (!flags || !q_dev || !bounds_dev || !table_dev || !lengths_dev || !score_dev || !selected_dev) return 1;
+    if (!flags || !library_is_here() || !q_dev || !bounds_dev || !table_dev || !lengths_dev || !score_dev || !selected_dev) return 1;
     PagedSelectArgs a = {};
     a.q = q_dev; a.q_ld = q_ld; a.bounds = bounds_dev; a.n_pages = (int)n_pages; a.P = (int)page_rows; a.table = table_dev; a.table_ld = table_ld; a.lengths = lengths_dev;
     a.max_len = table_ld * page_rows; a.window = window; a.cos = cos_dev; a.sin = sin_dev; a.rope_rows = rope_rows; a.rope = rope; a.H = n_heads; a.Hkv = n_kv; a.hd = head_dim; a.fa = fa; a.B = (int)n_seqs;
