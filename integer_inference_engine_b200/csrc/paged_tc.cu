@@ -121,8 +121,9 @@ struct TcWalk {
 };
 
 // One warp: the CTA's share of the list, as up to three runs: two pairs that it has in common with other CTAs, and whole pairs.  A pair that is cut costs its
-// CTAs an exchange, some six microseconds or four tiles; a second pair costs other query columns.
-//  * Whole pairs, dealt out in order, where the longest pairs so dealt make a CTA no more than four tiles above the average.
+// CTAs an exchange, some five microseconds; a second pair costs other query columns.
+//  * Whole pairs, dealt out in order, where the launch says so (`alone`) or the longest pairs so dealt make a CTA no more than one tile above the average: a
+//    tile is keys and values, one behind the other, some 2.6 us (1 x 600 keys, five tiles a pair: 25.0 us whole, 18.2 cut; 12 x 900 33.8 and 31.5; 16 x 600 25.8 either way).
 //  * Else each pair has CTAs of its own in proportion to its tiles, where there are enough CTAs and no part is more than two tiles above it.
 //  * Else the list is cut evenly: a CTA has the end of a pair, whole ones, the beginning of another.  (Cut pairs in an order that has two neighbours at
 //    the same one first, normalised between tiles as soon as the maxima are in, were no faster: the registers and the code that this takes cost the
@@ -135,7 +136,7 @@ __device__ __noinline__ int tc_count(const PagedAttnArgs &a, int b) {
     if (!paged_span(a, b, s) && blockIdx.x == 0) atomicOr(a.flags, 16);
     return tc_tiles(a, s);
 }
-__device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[RUNS]) {
+__device__ __forceinline__ void tc_share(const PagedAttnArgs &a, bool alone, TcWalk (&run)[RUNS]) {
     const int lane = threadIdx.x & 31, per_seq = a.Hkv * tc_head_groups(a), ctas = gridDim.x, me = blockIdx.x;
     const int own = tc_count(a, lane);             // (32 sequences at a time; the first ones kept)
     auto count = [&](int b) { return b < 32 ? own : tc_count(a, b); };
@@ -149,7 +150,7 @@ __device__ __forceinline__ void tc_share(const PagedAttnArgs &a, TcWalk (&run)[R
     auto parts = [&](int c) { return c == 0 ? 0 : max(1, min(c, (int)((uint32_t)c * ctas / total))); };
     auto part = [&](int c) { return c == 0 ? 0 : (c + parts(c) - 1) / parts(c); };
     enum { WHOLE_PAIRS, OWN_CTAS, EVEN } way = EVEN;
-    if ((pairs + ctas - 1) / ctas * most <= average + 4) way = WHOLE_PAIRS;
+    if (alone || (pairs + ctas - 1) / ctas * most <= average + 1) way = WHOLE_PAIRS;
     else if (pairs <= ctas) {
         int ps = 0, pl = 0;
 #pragma unroll 1
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     }
     if (warp == 3) {
         if (sh.alone) asm volatile("griddepcontrol.wait;" ::: "memory");       // (else what lies in front has ended: the clearing kernel waited for it)
-        tc_share(a, s.run);
+        tc_share(a, sh.alone, s.run);
     }
     tc_before();
     __syncthreads();
@@ -985,9 +986,12 @@ cudaError_t launch_tc(const PagedAttnArgs &a, cudaStream_t s) {
     }
     const long long most = (long long)a.B * a.Hkv * tc_head_groups(a) * tc_tiles_most(a);
     const unsigned ctas = (unsigned)std::min<long long>(std::min(sms, PT_MOST_CTAS), std::max<long long>(1, most));
-    // few tiles a CTA, and tc_share deals out whole pairs whatever the lengths: nothing to clear (1 x 300 keys 18.8 us; with the launch in front 19.8)
+    // Whole pairs whatever the lengths, where that is at most eight tiles a CTA and two above an even share of the longest lists: nothing to exchange or to clear, one launch that is
+    // not cooperative (1 x 300 keys 18.8 us replayed; with the launch in front 19.8; 32 sequences over 416 selected keys each 44.8 in place of 46.8 replayed, 45.6 of 51.5 called; 16 x 600
+    // 24.2 of 25.8 and 24.6 of 28.9).
     const long long pairs = (long long)a.B * a.Hkv * tc_head_groups(a);
-    const bool alone = (pairs + ctas - 1) / ctas * tc_tiles_most(a) <= 4;
+    const long long longest = (pairs + ctas - 1) / ctas * tc_tiles_most(a);
+    const bool alone = longest <= 8 && longest * ctas <= pairs * tc_tiles_most(a) + 2 * (long long)ctas;
     // outputs: two buffers of 64 columns a chunk; scores: two of 64, behind them or, at four chunks, over the end of the second
     const TcShape sh = {chunks, slots, chunks == 1 ? 256 : 512, chunks == 4 ? 384 : 128 * chunks, alone};
     if (!alone) {
