@@ -75,10 +75,12 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
     __syncthreads();
     if (s_seq < 0) return;
     const long long logical = s_page;
-    int page = -1;
-    if (logical < a.table_ld && !(a.rope && logical * P + s_first + s_count > a.rope_rows)) page = a.table[(long long)s_seq * a.table_ld + logical];
-    if (page < 0 || page >= a.n_pages) { if (tid == 0) atomicOr(a.flags, 16); return; }
-    const int half = a.hd / 2, first = s_first, count = s_count;
+    const int half = a.hd / 2, first = s_first;
+    // rows that the rotation table reaches; the others are left out
+    const int count = a.rope ? (int)max(0LL, min((long long)s_count, a.rope_rows - (logical * P + first))) : s_count;
+    const int page = logical < a.table_ld && count > 0 ? a.table[(long long)s_seq * a.table_ld + logical] : -1;
+    if (tid == 0 && (count < s_count || page < 0 || page >= a.n_pages)) atomicOr(a.flags, 16);
+    if (page < 0 || page >= a.n_pages) return;
     const long long cell = ((long long)page * a.Hkv + kv) * P * a.hd;
     int32_t *kp = a.kpages + cell, *vp = a.vpages + cell;
     const T *k = static_cast<const T *>(a.k) + s_row * a.k_ld + (long long)kv * a.hd, *v = static_cast<const T *>(a.v) + s_row * a.v_ld + (long long)kv * a.hd;

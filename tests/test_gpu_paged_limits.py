@@ -1,0 +1,43 @@
+"""The paged key/value cache at the ends of what its entries accept: the largest head dimensions, tables, lists, what lies half outside the cache.
+Every result is equal, bit for bit, to the restatement in NumPy's 64-bit integers."""
+import numpy as np
+import pytest
+
+from oracle import paged_oracle as po
+from test_gpu_paged import attend, dev, pool, tables
+
+pytestmark = pytest.mark.gpu
+
+
+def appended(rng, P, Hkv, hd, k, v, table, start, rows, rope_rows, counts):
+    """What an append leaves (keys, values, bounds, flags), and what it should where sequence i takes counts[i] rows from rows[i] on."""
+    from integer_inference_engine_b200 import device
+    kp, vp = (rng.integers(-(1 << 18), 1 << 18, size=(int(table.max()) + 3, Hkv, P, hd)).astype(np.int32) for _ in range(2))
+    bounds = rng.integers(-9, 9, size=(kp.shape[0], Hkv, 2, hd)).astype(np.int32)
+    cos, sin = tables(rope_rows, hd, 16)
+    dkp, dvp, db = dev(kp), dev(vp), dev(bounds)
+    device.read_flags()
+    device.paged_append(dev(k), dev(v), dkp, dvp, dev(table), dev(np.array(start, np.int32)), rows=None if rows is None else dev(np.array(rows, np.int32)), cos=dev(cos), sin=dev(sin), rope=1, bounds=db)
+    flags = device.read_flags()
+    for b, n in enumerate(counts):                 # (each by itself: the restatement knows no rows that are left out)
+        at = b if rows is None else rows[b]
+        if n > 0:
+            po.append(k[at:at + n], v[at:at + n], kp, vp, bounds, table[b:b + 1], start[b:b + 1], [0, n], 16, cos, sin, 1)
+    return [t.cpu().numpy() for t in (dkp, dvp, db)], [kp, vp, bounds], flags
+
+
+@pytest.mark.parametrize(("P", "start", "counts", "inside"), [
+    (16, [16, 2], [7, 3], [4, 3]),                 # positions 20, 21 and 22 lie behind the table of rotations, within a page that begins in front of them
+    (16, [3, 0], [30, 5], [17, 5]),                # ... and in the next pages
+    (32, [19, 20], [2, 1], [1, 0]),
+    (5, [18, 25], [4, 2], [2, 0]),
+])
+def test_rows_in_front_of_the_rotation_tables_end_are_appended(P, start, counts, inside):
+    rng = np.random.default_rng(P + start[0])
+    Hkv, hd, rows = 2, 32, [0] + list(np.cumsum(counts))
+    per = 40 // P + 2
+    table = rng.permutation(2 * per).reshape(2, per).astype(np.int32)
+    k, v = (rng.integers(-(1 << 18), 1 << 18, size=(sum(counts), Hkv * hd), dtype=np.int64) for _ in range(2))
+    got, want, flags = appended(rng, P, Hkv, hd, k, v, table, start, rows, 20, inside)
+    assert flags == 16
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
