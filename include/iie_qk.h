@@ -227,7 +227,9 @@ int iie_attn_decode_batch_rows_dev(const int64_t *q_dev, const int64_t *k_dev, c
  *
  * Append: `tokens` rows of keys and values [n_kv * head_dim], int64 (narrow = 0) or int32 (1), k_ld / v_ld apart.  Sequence i takes rows
  * rows_dev[i] .. rows_dev[i + 1] - 1 (rows_dev NULL: row i, one each) as its positions start_dev[i], start_dev[i] + 1, ...; a negative start
- * leaves the sequence out, rows behind the last sequence's are not read.  No two sequences append to the same page.  bounds_dev (nullable)
+ * leaves the sequence out, rows behind the last sequence's are not read.  rows_dev ascends and stays within 0 .. tokens: a sequence whose entries
+ * do not gets no rows and raises bit 4, and sequences behind one that descends may lack some of theirs; with tokens = 0 nothing is looked at.
+ * No two sequences append to the same page, no sequence to one twice.  bounds_dev (nullable)
  * [n_pages][n_kv][2][head_dim] receives, for every page that was met, the largest and the smallest value of each key dimension over its rows
  * up to the last one written.  A value beyond int32 raises bit 2. */
 int iie_paged_append_dev(const void *k_dev, const void *v_dev, int narrow, long long k_ld, long long v_ld, long long tokens, int32_t *kpages_dev,

@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
     pdl_enter();
     __shared__ int s_seq, s_first, s_count;
     __shared__ long long s_page, s_row;
-    __shared__ int s_scan[PA_THREADS / 32];
+    __shared__ long long s_scan[PA_THREADS / 32];
     __shared__ int s_lim[4][PA_THREADS];
     const int tid = threadIdx.x, kv = blockIdx.y, P = a.P;
     if (tid == 0) s_seq = -1;
@@ -45,31 +45,33 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
             if (at >= 0) { s_seq = b; s_page = at / P; s_first = at % P; s_count = 1; s_row = b; }
         }
     } else {
-        int before = 0;                                            // units of the sequences in front
+        // (the last CTA looks at every sequence's rows; entries that descend may name a row more than once: units are counted in 64 bits)
+        const bool checks = blockIdx.x == gridDim.x - 1 && kv == 0;
+        long long before = 0;                                      // units of the sequences in front
         for (int b0 = 0; b0 < a.B; b0 += PA_THREADS) {
             const int b = b0 + tid;
             long long at = -1, from = 0, n = 0;
             if (b < a.B) {
                 at = a.start[b]; from = a.rows[b]; n = (long long)a.rows[b + 1] - from;
-                if (n < 0 || from < 0 || from + n > a.T) { if (blockIdx.x == 0 && kv == 0) atomicOr(a.flags, 16); n = 0; }
+                if (n < 0 || from < 0 || from + n > a.T) { if (checks) atomicOr(a.flags, 16); n = 0; }
                 if (at < 0) n = 0;
             }
-            const int units = n > 0 ? (int)((at + n - 1) / P - at / P + 1) : 0;
-            int upto = units;
+            const long long units = n > 0 ? (at + n - 1) / P - at / P + 1 : 0;
+            long long upto = units;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if ((tid & 31) >= d) upto += o; }
+            for (int d = 1; d < 32; d <<= 1) { const long long o = __shfl_up_sync(0xffffffffu, upto, d); if ((tid & 31) >= d) upto += o; }
             if ((tid & 31) == 31) s_scan[tid >> 5] = upto;
             __syncthreads();
-            int base = before, all = 0;
+            long long base = before, all = 0;
             for (int w = 0; w < PA_THREADS / 32; w++) { if (w < (tid >> 5)) base += s_scan[w]; all += s_scan[w]; }
-            const int mine = (int)blockIdx.x - (base + upto - units);
+            const long long mine = blockIdx.x - (base + upto - units);
             if (mine >= 0 && mine < units) {
                 const long long p0 = (at / P + mine) * P, lo = max(at, p0), hi = min(at + n, p0 + P);
                 s_seq = b; s_page = p0 / P; s_first = (int)(lo - p0); s_count = (int)(hi - lo); s_row = from + (lo - at);
             }
             before += all;
             __syncthreads();
-            if (s_seq >= 0 || before > (int)blockIdx.x) break;
+            if (!checks && (s_seq >= 0 || before > blockIdx.x)) break;
         }
     }
     __syncthreads();

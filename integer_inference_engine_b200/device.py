@@ -251,7 +251,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, kpages: torch.Tensor, vpages:
     sequence] has the physical page of every logical page (position ``t`` is row ``t % page rows`` of logical page ``t // page rows``).
     ``k`` / ``v`` [T, n_kv * head_dim], int64 or int32, before rotation; rows may be column slices of one matrix.  Sequence ``i`` takes rows
     ``rows[i] .. rows[i + 1] - 1`` (``rows`` int32 [B + 1]; None: row ``i``, one each) as positions ``start[i]``, ``start[i] + 1``, ...
-    (int32 [B]); a negative start leaves it out, rows behind the last sequence's are not read.  No two sequences append to one page.
+    (int32 [B]); a negative start leaves it out, rows behind the last sequence's are not read.  ``rows`` ascends within 0 .. T: a sequence whose
+    entries do not gets no rows and raises bit 4, and sequences behind one that descends may lack some of theirs.  No two sequences append to one
+    page, no sequence to one twice.
     ``bounds`` int32 [pages, n_kv, 2, head_dim] receives the largest and smallest value of every key dimension over the rows of each page
     met, up to the last one written: what :func:`paged_select` ranks pages by.  A value beyond int32 raises bit 2, a position or page
     outside the cache (it is left out) bit 4 of :func:`read_flags`."""

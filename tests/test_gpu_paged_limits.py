@@ -41,3 +41,33 @@ def test_rows_in_front_of_the_rotation_tables_end_are_appended(P, start, counts,
     got, want, flags = appended(rng, P, Hkv, hd, k, v, table, start, rows, 20, inside)
     assert flags == 16
     assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("P", [1, 4])
+@pytest.mark.parametrize("wrong", [1, 127, 128, 200, 299])
+@pytest.mark.parametrize("how", ["descends", "passes the end"])
+def test_wrong_rows_of_any_sequence_are_flagged(P, wrong, how):
+    """More sequences than a scan takes at once: the wrong one gets no rows, the others theirs (as long as there are no more of
+    these than rows: eight lie behind the last sequence's)."""
+    rng = np.random.default_rng(wrong + P)
+    B, Hkv, hd, each = 300, 1, 16, 2
+    rows = [i * each for i in range(B + 1)]
+    counts = [each] * B
+    if how == "descends":
+        if wrong == B - 1:
+            rows[B] = rows[B - 1] - 1
+        else:
+            rows[wrong + 1] = rows[wrong] - 1      # the one behind begins in front of it
+            counts[wrong + 1] = rows[wrong + 2] - rows[wrong + 1]
+        counts[wrong] = 0
+    elif wrong == B - 1:
+        rows[B] += 9
+        counts[wrong] = 0
+    else:
+        rows[wrong + 1] = B * each + 9             # beyond all rows: the one behind descends
+        counts[wrong] = counts[wrong + 1] = 0
+    table = rng.permutation(B * 6).reshape(B, 6).astype(np.int32)
+    k, v = (rng.integers(-(1 << 18), 1 << 18, size=(B * each + 8, Hkv * hd), dtype=np.int64) for _ in range(2))
+    got, want, flags = appended(rng, P, Hkv, hd, k, v, table, [0] * B, rows, 40, counts)
+    assert flags == 16
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
