@@ -758,13 +758,14 @@ cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s) {
     const unsigned flat = (unsigned)std::min<long long>(1184, ((long long)a.B * a.H * a.hd + 255) / 256);
     const long long slots = a.max_slots;
     launch_behind(paged_general_init_kernel, flat, 256, 0, s, a);
+    // (with room for no key, too: it is the scores' kernel that flags lengths beyond their bound)
+    launch_behind(paged_general_scores_kernel, dim3((unsigned)std::max(1LL, (slots + PG_KEYS - 1) / PG_KEYS), pairs, a.B), 256, (size_t)PG_HEADS * a.hd * 8, s, a);
     if (slots > 0) {
-        launch_behind(paged_general_scores_kernel, dim3((unsigned)((slots + PG_KEYS - 1) / PG_KEYS), pairs, a.B), 256, (size_t)PG_HEADS * a.hd * 8, s, a);
         launch_behind(paged_general_exp_kernel, dim3((unsigned)((slots + 1023) / 1024), a.H, a.B), 256, 0, s, a);
         launch_behind(paged_general_values_kernel, dim3((unsigned)((slots + 127) / 128), pairs, a.B), 256, 0, s, a);
     }
     const cudaError_t e = launch_behind(paged_general_out_kernel, flat, 256, 0, s, a);
-    note_launch(5);
+    note_launch(slots > 0 ? 5 : 3);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -71,3 +71,18 @@ def test_wrong_rows_of_any_sequence_are_flagged(P, wrong, how):
     got, want, flags = appended(rng, P, Hkv, hd, k, v, table, [0] * B, rows, 40, counts)
     assert flags == 16
     assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize(("hd", "P"), [(128, 16), (80, 16), (64, 5)])
+@pytest.mark.parametrize("window", [0, 4])
+def test_lengths_beyond_a_bound_of_zero_are_flagged(hd, P, window):
+    """max_length = 0: no sequence has a key, one that says otherwise is left out."""
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(hd)
+    H, Hkv = 4, 2
+    kp, vp, table = pool(rng, [30, 20], P, Hkv, hd, 18)
+    q = rng.integers(-(1 << 18), 1 << 18, size=(2, H * hd), dtype=np.int64)
+    for lengths, flags in (([0, 0], 0), ([0, 3], 16), ([-1, 0], 16)):
+        device.read_flags()
+        got = attend(q, kp, vp, table, lengths, max_length=0, window=window)
+        assert device.read_flags() == flags and not got.any()
