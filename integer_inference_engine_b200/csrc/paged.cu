@@ -757,15 +757,26 @@ cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s) {
     const int rep = a.H / a.Hkv, pairs = a.Hkv * ((rep + PG_HEADS - 1) / PG_HEADS);
     const unsigned flat = (unsigned)std::min<long long>(1184, ((long long)a.B * a.H * a.hd + 255) / 256);
     const long long slots = a.max_slots;
-    launch_behind(paged_general_init_kernel, flat, 256, 0, s, a);
+    static std::atomic<unsigned long long> configured;
+    cudaError_t e = paged_once(configured, [] {
+        return cudaFuncSetAttribute(paged_general_scores_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PG_HEADS * PAGED_MAX_HEAD * 8);
+    });
+    if (e != cudaSuccess) return e;
+    int launches = 0;
+    auto behind = [&](auto kernel, dim3 grid, size_t smem) {       // (none behind one that failed)
+        if (e != cudaSuccess) return;
+        e = launch_behind(kernel, grid, 256, smem, s, a);
+        launches += e == cudaSuccess;
+    };
+    behind(paged_general_init_kernel, flat, 0);
     // (with room for no key, too: it is the scores' kernel that flags lengths beyond their bound)
-    launch_behind(paged_general_scores_kernel, dim3((unsigned)std::max(1LL, (slots + PG_KEYS - 1) / PG_KEYS), pairs, a.B), 256, (size_t)PG_HEADS * a.hd * 8, s, a);
+    behind(paged_general_scores_kernel, dim3((unsigned)std::max(1LL, (slots + PG_KEYS - 1) / PG_KEYS), pairs, a.B), (size_t)PG_HEADS * a.hd * 8);
     if (slots > 0) {
-        launch_behind(paged_general_exp_kernel, dim3((unsigned)((slots + 1023) / 1024), a.H, a.B), 256, 0, s, a);
-        launch_behind(paged_general_values_kernel, dim3((unsigned)((slots + 127) / 128), pairs, a.B), 256, 0, s, a);
+        behind(paged_general_exp_kernel, dim3((unsigned)((slots + 1023) / 1024), a.H, a.B), 0);
+        behind(paged_general_values_kernel, dim3((unsigned)((slots + 127) / 128), pairs, a.B), 0);
     }
-    const cudaError_t e = launch_behind(paged_general_out_kernel, flat, 256, 0, s, a);
-    note_launch(slots > 0 ? 5 : 3);
+    behind(paged_general_out_kernel, flat, 0);
+    note_launch(launches);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

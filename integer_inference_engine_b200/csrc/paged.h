@@ -8,6 +8,8 @@
 
 namespace iie {
 
+constexpr int PAGED_MAX_HEAD = 1024;               // head dimension: eight query heads of it as int64 are 64 KB of shared memory
+
 struct PagedAppendArgs {
     const void *k, *v;             // new rows [T][Hkv * hd], int64 or (narrow) int32, keys before rotation
     bool narrow;

@@ -14,7 +14,6 @@ using namespace iie;
 
 namespace {
 
-constexpr int PAGED_MAX_HEAD = 1024;               // head dimension; eight query heads of it as int64 fit shared memory
 constexpr long long PAGED_SLAB = 2LL << 30;        // scratch of a call: sequences beyond it go one part behind the other
 
 bool shape_ok(int n_heads, int n_kv, int hd, int fa, int rope, const void *cos, const void *sin, long long rope_rows) {

@@ -86,3 +86,20 @@ def test_lengths_beyond_a_bound_of_zero_are_flagged(hd, P, window):
         device.read_flags()
         got = attend(q, kp, vp, table, lengths, max_length=0, window=window)
         assert device.read_flags() == flags and not got.any()
+
+
+@pytest.mark.parametrize("hd", [768, 770, 1024])
+@pytest.mark.parametrize("chosen", [False, True])
+def test_attention_of_large_heads(hd, chosen):
+    """Eight query heads of these are 48 KB as 64 bits, the first size beyond it, and the largest that is accepted; more than eight heads a KV head."""
+    from integer_inference_engine_b200 import device
+    H, Hkv, P, lengths = 9, 1, 16, [40, 0, 3]
+    rng = np.random.default_rng(hd)
+    kp, vp, table = pool(rng, lengths, P, Hkv, hd, 18)
+    q = rng.integers(-(1 << 18), 1 << 18, size=(len(lengths), H * hd), dtype=np.int64)
+    cos, sin = tables(max(lengths), hd, 16)
+    pages = np.array([[[2, 0]], [[0, 1]], [[-1, 0]]], np.int32) if chosen else None
+    device.read_flags()
+    got = attend(q, kp, vp, table, lengths, cos=cos, sin=sin, rope=2, pages=pages)
+    assert device.read_flags() == 0
+    assert np.array_equal(got, po.attention(q, kp, vp, table, lengths, 16, 0, cos, sin, 2, pages))
