@@ -490,6 +490,7 @@ __global__ void __launch_bounds__(PS_THREADS) paged_pick_kernel(const PagedSelec
 // 64-bit products.
 constexpr int PR_PAGES = 8;                        // pages of a warp at a time
 constexpr int PR_GAP = 64;
+constexpr size_t PR_SHARED = 220 * 1024;           // of a CTA at most: queries and the warps' pages, beside them (in the one-launch form) the scores
 constexpr int PR_CLUSTER = 8, PR_TURN = PR_PAGES * (PS_THREADS / 32), PR_MOST = 2 * PR_CLUSTER * PR_TURN;     // CTAs of a cluster; pages of one at a time; of a list for this form
 __host__ __device__ inline int rank_heads(int rep) { return rep <= 4 ? 4 : (rep + 7) / 8 * 8; }
 __host__ __device__ inline size_t rank_stage(int hd) { return (size_t)PR_PAGES * (8 * hd + PR_GAP); }       // of a warp
@@ -783,14 +784,14 @@ cudaError_t launch_paged_attn(const PagedAttnArgs &a, cudaStream_t s) {
 cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
     const int rep = a.H / a.Hkv;
     const size_t rank = (size_t)rank_heads(rep) * a.hd * 12 + PS_THREADS / 32 * rank_stage(a.hd), fused = rank + (size_t)a.table_ld * 8;
-    const bool staged = a.hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0 && rank <= 215 * 1024;
+    const bool staged = a.hd % 16 == 0 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0 && rank <= PR_SHARED;
     const int sms = paged_sms();
     if (sms <= 0) return cudaErrorInvalidDevice;
     const unsigned blocks = (unsigned)std::min<long long>(PR_CLUSTER, (a.table_ld + PR_TURN - 1) / PR_TURN);
-    if (staged && a.table_ld <= PR_MOST && (a.table_ld <= 2 * PR_TURN || (long long)blocks * a.Hkv * a.B <= 2 * sms)) {
+    if (staged && fused <= PR_SHARED && a.table_ld <= PR_MOST && (a.table_ld <= 2 * PR_TURN || (long long)blocks * a.Hkv * a.B <= 2 * sms)) {
         static std::atomic<unsigned long long> configured;
         cudaError_t e = paged_once(configured, [] {
-            const cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+            const cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PR_SHARED);
             return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         });
         if (e != cudaSuccess) return e;
@@ -807,7 +808,7 @@ cudaError_t launch_paged_select(const PagedSelectArgs &a, cudaStream_t s) {
     }
     static std::atomic<unsigned long long> configured;
     cudaError_t e = paged_once(configured, [] {
-        cudaError_t e = cudaFuncSetAttribute(paged_rank_even_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        cudaError_t e = cudaFuncSetAttribute(paged_rank_even_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PR_SHARED);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_rank_even_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PK_HELD * 8);

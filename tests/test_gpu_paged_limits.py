@@ -103,3 +103,21 @@ def test_attention_of_large_heads(hd, chosen):
     got = attend(q, kp, vp, table, lengths, cos=cos, sin=sin, rope=2, pages=pages)
     assert device.read_flags() == 0
     assert np.array_equal(got, po.attention(q, kp, vp, table, lengths, 16, 0, cos, sin, 2, pages))
+
+
+# head dimension, query heads of a KV head (as many as its queries are padded to), pages of the table: queries, pages on their way and scores together pass 220 KB of shared memory
+RANK = [(384, 4, 769), (384, 3, 1000), (352, 8, 1024), (304, 16, 1000), (240, 32, 1000), (48, 328, 1000), (384, 4, 768), (272, 24, 1000), (64, 240, 300)]
+
+
+@pytest.mark.parametrize(("hd", "rep", "per"), RANK)
+def test_select_of_large_heads_from_wide_tables(hd, rep, per):
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(hd + per)
+    lengths, n_pages = [per - 1, 37, 0], 50
+    bounds = np.sort(rng.integers(-(1 << 18), 1 << 18, size=(n_pages, 1, 2, hd)), axis=2)[:, :, ::-1].astype(np.int32)
+    table = rng.integers(0, n_pages, size=(3, per)).astype(np.int32)
+    q = rng.integers(-(1 << 18), 1 << 18, size=(3, rep * hd), dtype=np.int64)
+    device.read_flags()
+    got = device.paged_select(dev(q), dev(bounds), dev(table), dev(np.array(lengths, np.int32)), 1, 9)
+    assert device.read_flags() == 0
+    assert np.array_equal(got.cpu().numpy(), po.select(q, bounds, table, lengths, 1, 9, 1, 1, 16, 0, None, None, 0))
