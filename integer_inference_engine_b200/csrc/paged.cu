@@ -42,7 +42,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
     if (!a.rows) {
         if (tid == 0) {
             const int b = blockIdx.x, at = a.start[b];
-            if (at >= 0) { s_seq = b; s_page = at / P; s_first = at % P; s_count = 1; s_row = b; }
+            if (a.rope && at >= a.rope_rows) atomicOr(a.flags, 16);
+            else if (at >= 0) { s_seq = b; s_page = at / P; s_first = at % P; s_count = 1; s_row = b; }
         }
     } else {
         // (the last CTA looks at every sequence's rows; entries that descend may name a row more than once: units are counted in 64 bits)
@@ -66,8 +67,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
             for (int w = 0; w < PA_THREADS / 32; w++) { if (w < (tid >> 5)) base += s_scan[w]; all += s_scan[w]; }
             const long long mine = blockIdx.x - (base + upto - units);
             if (mine >= 0 && mine < units) {
-                const long long p0 = (at / P + mine) * P, lo = max(at, p0), hi = min(at + n, p0 + P);
-                s_seq = b; s_page = p0 / P; s_first = (int)(lo - p0); s_count = (int)(hi - lo); s_row = from + (lo - at);
+                const long long p0 = (at / P + mine) * P, lo = max(at, p0), end = min(at + n, p0 + P), hi = a.rope ? min(end, a.rope_rows) : end;
+                if (hi < end) atomicOr(a.flags, 16);               // positions behind the rotation table's end are left out
+                if (hi > lo) s_seq = b;
+                s_page = p0 / P; s_first = (int)(lo - p0); s_count = (int)(hi - lo); s_row = from + (lo - at);
             }
             before += all;
             __syncthreads();
@@ -77,12 +80,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
     __syncthreads();
     if (s_seq < 0) return;
     const long long logical = s_page;
-    const int half = a.hd / 2, first = s_first;
-    // rows that the rotation table reaches; the others are left out
-    const int count = a.rope ? (int)max(0LL, min((long long)s_count, a.rope_rows - (logical * P + first))) : s_count;
-    const int page = logical < a.table_ld && count > 0 ? a.table[(long long)s_seq * a.table_ld + logical] : -1;
-    if (tid == 0 && (count < s_count || page < 0 || page >= a.n_pages)) atomicOr(a.flags, 16);
-    if (page < 0 || page >= a.n_pages) return;
+    const int page = logical < a.table_ld ? a.table[(long long)s_seq * a.table_ld + logical] : -1;
+    if (page < 0 || page >= a.n_pages) { if (tid == 0) atomicOr(a.flags, 16); return; }
+    const int half = a.hd / 2, first = s_first, count = s_count;
     const long long cell = ((long long)page * a.Hkv + kv) * P * a.hd;
     int32_t *kp = a.kpages + cell, *vp = a.vpages + cell;
     const T *k = static_cast<const T *>(a.k) + s_row * a.k_ld + (long long)kv * a.hd, *v = static_cast<const T *>(a.v) + s_row * a.v_ld + (long long)kv * a.hd;
