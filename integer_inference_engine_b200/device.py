@@ -177,6 +177,7 @@ def attention_decode_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kc
 
 
 _I32, _I64 = torch.int32, torch.int64
+_MOST = 2 ** 31 - 1                                 # what the library counts in 31 bits
 
 
 def _on_current_device(names: str, *tensors) -> None:
@@ -298,6 +299,8 @@ def paged_attention(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor,
     n_heads, q_ld = _paged_query(q, B, n_kv, head_dim)
     if pages is not None and (pages.dtype != torch.int32 or pages.dim() != 3 or pages.shape[:2] != (B, n_kv) or pages.shape[2] == 0 or not pages.is_contiguous()):
         raise ValueError("pages must be a contiguous int32 [sequences, n_kv, n] with n > 0")
+    if pages is not None and pages.shape[2] * page_rows > _MOST:
+        raise ValueError("pages must name at most 2**31 - 1 rows of a sequence")
     if max_length is None:
         max_length = per_seq * page_rows
     if not 0 <= max_length <= per_seq * page_rows:
@@ -342,8 +345,8 @@ def paged_select(q: torch.Tensor, bounds: torch.Tensor, table: torch.Tensor, len
     n_pages, n_kv, _, head_dim = bounds.shape
     B, per_seq = _paged_table(table, "lengths", lengths)
     n_heads, q_ld = _paged_query(q, B, n_kv, head_dim)
-    if page_rows <= 0 or n_select <= 0 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > n_select:
-        raise ValueError("page_rows and n_select must be positive, keep_first + keep_last at most n_select")
+    if page_rows <= 0 or not 0 < n_select <= _MOST or keep_first < 0 or keep_last < 0 or keep_first + keep_last > n_select:
+        raise ValueError("page_rows and n_select must be positive (n_select below 2**31), keep_first + keep_last at most n_select")
     if window < 0:
         raise ValueError("window must not be negative (0: every key)")
     if out is None:

@@ -107,3 +107,12 @@ def test_c_entries_refuse(lib):
     for c in (dict(n=0), dict(first=4), dict(last=-1), dict(H=3), dict(q_ld=1), dict(hd=0)):
         assert select(**c) == 1, c
     assert select(B=0) == 0
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 4])
+def test_counts_beyond_31_bits_are_refused(n):
+    """... before they are cut to the 32 bits that the library takes, and before anything of that size is laid out."""
+    with pytest.raises(ValueError, match="n_select"):
+        call("select", good(), n_select=n)
+    with pytest.raises(ValueError, match="rows of a sequence"):
+        call("attention", {**good(), "pages": torch.empty((3, 2, n), dtype=I32, device="meta")})
