@@ -121,3 +121,124 @@ def test_select_of_large_heads_from_wide_tables(hd, rep, per):
     got = device.paged_select(dev(q), dev(bounds), dev(table), dev(np.array(lengths, np.int32)), 1, 9)
     assert device.read_flags() == 0
     assert np.array_equal(got.cpu().numpy(), po.select(q, bounds, table, lengths, 1, 9, 1, 1, 16, 0, None, None, 0))
+
+
+# heads, KV heads, lengths' bound, sequences (on 148 SMs: pairs dealt out whole, 305 tiles each; an even cut with whole pairs in it; pairs of 700 tiles cut into parts of some 300)
+@pytest.mark.parametrize(("H", "Hkv", "most", "B"), [(8, 4, 39000, 37), (8, 8, 39000, 40), (8, 4, 89600, 16)])
+def test_more_tiles_of_a_pair_than_one_accumulation_takes(H, Hkv, most, B):
+    """Output sums are read out every 256 tiles of 128 keys.  Few physical pages stand behind all tables."""
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(B)
+    hd, P, n_pages = 32, 16, 60
+    lengths = [most] + [int(n) for n in most - rng.integers(0, 100, size=B - 1)]
+    kp, vp = (rng.integers(-(1 << 18), 1 << 18, size=(n_pages, Hkv, P, hd)).astype(np.int32) for _ in range(2))
+    vp[:, 0] = rng.choice(np.array([-(1 << 31), (1 << 31) - 1, -1], np.int64), size=vp[:, 0].shape)       # the largest sums that there are
+    table = rng.integers(0, n_pages, size=(B, (most + P - 1) // P)).astype(np.int32)
+    q = rng.integers(-(1 << 14), 1 << 14, size=(B, H * hd), dtype=np.int64)
+    cos, sin = tables(most, hd, 16)
+    device.read_flags()
+    got = attend(q, kp, vp, table, lengths, cos=cos, sin=sin, rope=1)
+    assert device.read_flags() == 0
+    for b in (0, 1, B // 2, B - 1):
+        assert np.array_equal(got[b:b + 1], po.attention(q[b:b + 1], kp, vp, table[b:b + 1], lengths[b:b + 1], 16, 0, cos, sin, 1)), b
+
+
+@pytest.mark.parametrize(("H", "Hkv", "hd", "lengths"), [(12, 1, 128, [5000, 3000]), (20, 1, 64, [9000]), (32, 2, 96, [4000, 0, 7000, 100]), (9, 1, 32, [20000, 1])])
+def test_more_than_eight_heads_over_a_long_cache(H, Hkv, hd, lengths):
+    """Several groups of query heads per KV head, their pairs cut between CTAs."""
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(H)
+    kp, vp, table = pool(rng, lengths, 16, Hkv, hd, 18)
+    q = rng.integers(-(1 << 16), 1 << 16, size=(len(lengths), H * hd), dtype=np.int64)
+    cos, sin = tables(max(lengths), hd, 16)
+    device.read_flags()
+    got = attend(q, kp, vp, table, lengths, cos=cos, sin=sin, rope=2)
+    assert device.read_flags() == 0
+    assert np.array_equal(got, po.attention(q, kp, vp, table, lengths, 16, 0, cos, sin, 2))
+
+
+@pytest.mark.parametrize("hd", [64, 80])
+@pytest.mark.parametrize("chosen", [False, True])
+def test_scratch_in_parts(hd, chosen):
+    """Tables (or lists) so wide that the scratch of all sequences passes its limit: they go in parts, one behind the other, over the same scratch."""
+    import torch
+
+    from integer_inference_engine_b200 import device, qk_cuda
+    H, Hkv, P, per = 8, 2, 16, 2048
+    size = lambda n: qk_cuda.load_library().iie_paged_attn_bytes(n, per * P, 0, per if chosen else 0, P, H, Hkv, hd, 16)
+    part = (2 << 30) // size(1)
+    B = part + 37
+    assert size(B) == size(part) > 1 << 29
+    rng = np.random.default_rng(hd)
+    lengths = [int(n) for n in rng.integers(0, 41, size=B)]
+    lengths[part - 1:part + 1] = [600, 500]        # the last of a part, the first of the next
+    kp, vp, narrow = pool(rng, lengths, P, Hkv, hd, 18)
+    table = np.full((B, per), -7, np.int32)
+    table[:, :narrow.shape[1]] = narrow
+    pages = None
+    if chosen:
+        pages = np.full((B, Hkv, per), -1, np.int32)
+        for b, n in enumerate(lengths):
+            take = rng.permutation((n + P - 1) // P)[:20]
+            for g in range(Hkv):
+                pages[b, g, rng.permutation(per)[:len(take)]] = take
+    q = rng.integers(-(1 << 18), 1 << 18, size=(B, H * hd), dtype=np.int64)
+    cos, sin = tables(max(lengths), hd, 16)
+    device.read_flags()
+    got = attend(q, kp, vp, table, lengths, cos=cos, sin=sin, rope=1, pages=pages)
+    torch.cuda.empty_cache()
+    assert device.read_flags() == 0
+    assert np.array_equal(got, po.attention(q, kp, vp, table, lengths, 16, 0, cos, sin, 1, pages))
+
+
+@pytest.mark.parametrize(("H", "Hkv", "hd", "lengths"), [(32, 4, 128, [300]), (32, 8, 128, [1500, 0, 700, 1100]), (8, 2, 64, [40] * 30), (4, 2, 80, [90, 3])])
+def test_a_table_with_room_for_much_more(H, Hkv, hd, lengths):
+    """2048 pages a sequence, whatever its length, entries behind its last page pointing nowhere: attention, selection, attention over what it selects."""
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(hd + len(lengths))
+    P, B = 16, len(lengths)
+    kp, vp, narrow = pool(rng, lengths, P, Hkv, hd, 18)
+    table = np.full((B, 2048), -7, np.int32)
+    table[:, :narrow.shape[1]] = narrow
+    bounds = np.stack([kp.max(2), kp.min(2)], 2)
+    q = rng.integers(-(1 << 17), 1 << 17, size=(B, H * hd), dtype=np.int64)
+    cos, sin = tables(max(lengths), hd, 16)
+    device.read_flags()
+    assert np.array_equal(attend(q, kp, vp, table, lengths, cos=cos, sin=sin, rope=1), po.attention(q, kp, vp, table, lengths, 16, 0, cos, sin, 1))
+    pages = device.paged_select(dev(q), dev(bounds), dev(table), dev(np.array(lengths, np.int32)), P, 6, cos=dev(cos), sin=dev(sin), rope=1).cpu().numpy()
+    assert np.array_equal(pages, po.select(q, bounds, table, lengths, P, 6, 1, 1, 16, 0, cos, sin, 1))
+    assert np.array_equal(attend(q, kp, vp, table, lengths, cos=cos, sin=sin, rope=1, pages=pages), po.attention(q, kp, vp, table, lengths, 16, 0, cos, sin, 1, pages))
+    assert device.read_flags() == 0
+
+
+def test_two_captured_steps_replayed_at_once():
+    """Selection, attention over it and over everything, captured twice and replayed on two streams: neither graph's scratch is the other's."""
+    import torch
+
+    from integer_inference_engine_b200 import device
+    rng = np.random.default_rng(3)
+    H, Hkv, hd, P, lengths = 8, 2, 128, 16, [900, 40, 3000]
+    graphs, outs, wants, streams = [], [], [], [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        kp, vp, table = pool(rng, lengths, P, Hkv, hd, 18)
+        bounds = np.stack([kp.max(2), kp.min(2)], 2)
+        q = rng.integers(-(1 << 17), 1 << 17, size=(3, H * hd), dtype=np.int64)
+        world = [dev(t) for t in (q, kp, vp, table, np.array(lengths, np.int32), bounds)]
+        pages = po.select(q, bounds, table, lengths, P, 8, 1, 1, 16, 0, None, None, 0)
+        wants.append([pages] + [po.attention(q, kp, vp, table, lengths, 16, 0, None, None, 0, p) for p in (pages, None)])
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            picked = device.paged_select(world[0], world[5], world[3], world[4], P, 8)
+            outs.append([picked, device.paged_attention(*world[:5], pages=picked), device.paged_attention(*world[:5])])
+        graphs.append((graph, world))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for got, want in zip(outs, wants):
+        assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(got, want))
+    assert device.read_flags() == 0
+
