@@ -221,7 +221,7 @@ int iie_attn_decode_batch_rows_dev(const int64_t *q_dev, const int64_t *k_dev, c
  * table_dev [n_seqs][table_ld]: physical page of every logical page of a sequence, position t being row t % page_rows of logical page
  * t / page_rows.  Sequences may share pages that none of them appends to.  cos_dev / sin_dev [rope_rows][head_dim / 2]; rope as above.
  * Positions, lengths and page numbers are read on the device: what lies outside the pool, the table or the rotation rows raises bit 4 of the
- * flag word and is left out.  All entries: 0 ok, 1 bad argument, CUDA failure or a current device other than that of the library's first use;
+ * flag word and is left out (by selection ranked lowest).  All entries: 0 ok, 1 bad argument, CUDA failure or a current device other than that of the library's first use;
  * asynchronous on `stream`; they allocate nothing and share no scratch, so calls on different streams may overlap and captured calls stay valid
  * as long as the caller's buffers.
  *
@@ -252,8 +252,9 @@ int iie_paged_attn_dev(const int64_t *q_dev, long long q_ld, const int32_t *kpag
 /* The pages a token attends to: per sequence and KV head the first keep_first and last keep_last visible pages, then those of the highest
  * score, the lowest page among equals, n_select in all (at most 2^31 - 1); selected_dev [n_seqs][n_kv][n_select] ascending, -1 behind them.  The score of a page
  * is an upper bound of its keys' products with the token: the largest, over the query heads of the KV head, of
- * sum_i max(q_i largest_i, q_i smallest_i), modulo 2^64, with the rotated query and the page's bounds_dev.  score_dev: scratch of
- * n_seqs * n_kv * table_ld values. */
+ * sum_i max(q_i largest_i, q_i smallest_i), modulo 2^64, with the rotated query and the page's bounds_dev.  A page number outside the pool
+ * ranks lowest and raises bit 4 (one of the kept pages stays in the list); of a sequence with n_select visible pages or fewer all are listed and
+ * no number is looked at.  score_dev: scratch of n_seqs * n_kv * table_ld values.  selected_dev overlaps none of the inputs. */
 int iie_paged_select_dev(const int64_t *q_dev, long long q_ld, const int32_t *bounds_dev, long long n_pages, long long page_rows,
                          const int *table_dev, long long table_ld, const int *lengths_dev, long long n_seqs, int n_select, int keep_first,
                          int keep_last, long long window, const int64_t *cos_dev, const int64_t *sin_dev, long long rope_rows, int rope,

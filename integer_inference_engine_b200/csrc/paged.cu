@@ -1,7 +1,7 @@
 // Paged key/value cache: append with rotation, ranking of pages by a bound of their scores, and the attention of one new token per
 // sequence in its general form (any head dimension, page size and number of query heads).  Arithmetic of the attention: attn.cu.
 //
-// The general form keeps scores and exponentials in memory and takes five launches: it carries the shapes that have no other.
+// The general form keeps scores and exponentials in memory and takes five launches (three where no key has room): it carries the shapes that have no other.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -23,7 +23,7 @@ namespace {
 // need no atomics.  They are formed again from the page's rows, old ones read back: a function of what the cache holds, whatever was
 // appended and given up before.
 //
-// What bounds it: memory for long prompts (2350 rows of 8 KV heads of 128, 58 MB, 11.3 us: 5.1 TB/s), for a token each the launch and four dependent loads
+// What bounds it: memory for long prompts (2350 rows of 8 KV heads of 128, 58 MB, 11.2 us: 5.2 TB/s), for a token each the launch and four dependent loads
 // (a token's row, the table's entry, the row, the page's older rows; 3.2 us for 64 sequences).  A thread has the loads of PA_ROWS rows on their way
 // at once; CTAs of 128 are all resident from the start (of 256, 16.3 us with four rows, 13.2 with two; 128: 14.3 with one, 12.2 with four).
 constexpr int PA_THREADS = 128, PA_ROWS = 2;
@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const PagedApp
 
 // ---- attention, general form ------------------------------------------------------------------------------------------------------
 // Any head dimension, page and scale, in five launches: a start, scores with their maxima by 64 keys a CTA, exponentials with their sums, probabilities times values, the last shift;
-// what lies between them is in memory as 64 bits.  Bound by its 64-bit multiply-adds: 8 sequences of 2000 keys, 2 KV heads of 256, 117 us, 0.56 TB/s (of 128, through the
-// tensor cores, 22); 64 of 4096 keys, 4 KV heads of 128 in pages of 12 rows, 2.13 ms.
+// what lies between them is in memory as 64 bits.  Bound by its 64-bit multiply-adds: 8 sequences of 2000 keys, 2 KV heads of 256, 116 us, 0.56 TB/s (of 128, through the
+// tensor cores, 22); 64 of 4096 keys, 4 KV heads of 128 in pages of 12 rows, 2.12 ms.
 constexpr int PG_HEADS = 8, PG_KEYS = 64;
 
 struct GeneralWork {
@@ -627,7 +627,8 @@ __global__ void __launch_bounds__(PS_THREADS, 2) paged_select_kernel(const Paged
 }
 
 // Longer lists, in a launch of their own: the pages of all sequences and KV heads shared evenly, each pair of them by CTAs in proportion to its pages
-// (whole groups of eight), two CTAs an SM.  For lists of more than 1024 pages, or of more than 128 where the clusters would not all be resident at once.  Both forms, a call alone,
+// (whole groups of eight), two CTAs an SM.  For tables of more than 1024 pages, or of more than 128 where the clusters would not all be resident at once, whatever the lengths
+// (a table of 2048 pages: 32 x 62 pages 17.9 in place of 11.2, 1 x 500 14.3 of 11.6, 8 x 500 23.2 of 18.1).  Both forms, a call alone,
 // us (clusters first): 1 x 1000 pages 12.5 and 13.5, 1 x 2000 19.6 and 15.9, 1 x 8000 60.6 and 33.5; 8 x 500 13.9 and 19.4, 16 x 500 24.0 and 21.6, 32 x 1000 70.5 and 64.4; 64 x 200 38.6 and
 // 32.2, 150 x 120 45.1 and 53.1, 300 x 60 41.7 and 65.4; 8 x up to 2000 29.7 and 27.1: plan 2, the part's place and query 2, ranking 11 to 15 (multiply-adds 8 of them), the launch
 // between 1, picking 5.

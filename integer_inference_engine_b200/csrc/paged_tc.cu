@@ -10,17 +10,20 @@
 // the others from the unsigned one.  Every sum stays below 2^31: 4 hd 255 128 for a score, 255^2 per key for an output (at most 256 tiles
 // of 128 keys before the sums are read out).
 //
-// Tiles of 128 keys of all sequences and KV heads form one list that one CTA per SM share evenly, whatever the lengths.  The softmax floors e
-// and p, which takes the maximum and then the normaliser of all of a pair's keys (pair: a sequence's KV head with up to eight query heads) in
+// Tiles of 128 keys of all sequences and KV heads form one list that one CTA per SM share (pair: a sequence's KV head with up to eight query heads): by whole pairs,
+// by CTAs of a pair's own or by an even cut (tc_share).  The softmax floors e and p, which takes the maximum and then the normaliser of all of a pair's keys in
 // front of its values: a CTA takes the scores of all its tiles (in memory, as 32-bit distances below the maximum of 32 keys; one beyond
 // `clip` has no weight, so nothing is lost), the normalisers, then the values.  Pairs that lie in one CTA need nobody else.  Of those cut between CTAs
 // (at most one begins in each) every CTA tells the others its maximum and its normaliser, and the output sums are added up in memory with a count of their
-// parts.  The launch is cooperative, every wait is bounded, and integers are added in any order.  A small kernel in front clears what is told.
+// parts: that launch is cooperative, every wait is bounded, integers are added in any order, and a small kernel in front clears what is told.  Where few tiles leave
+// every pair whole whatever the lengths (launch_tc: `alone`) there is one launch, and it is not cooperative.
 //
-// What bounds it: memory where there is much of it, 122 us for 64 sequences of up to 4096 keys (4 KV heads of 128, 8 query heads each; 640 MB: 5.2 TB/s), 63 us for
-// 278 MB of three of up to 30000.  Beside that a call pays 3 us until the share is planned, 3 us until the first query columns are written, 6 to 9 us
-// between keys and values (a microsecond or two for an exchange, twice, and the exponentials: 24 clocks for a warp's 32, 0.13 us for a tile of eight heads),
-// 2 us for the outputs: 19 us for one sequence of 300 keys, 24 for one of 4096.
+// What bounds it, replayed: memory where there is much of it, 118 us for 64 sequences of up to 4096 keys (4 KV heads of 128, 8 query heads each; 640 MB: 5.4 TB/s over the
+// launch), 185 with 4096 keys each (1.07 GB: 5.8), 62 for 278 MB of three of up to 30000.  Beside that a call pays 3 us until the share is planned, 3 us until the first query
+// columns are written, 6 to 9 us between keys and values (a microsecond or two for an exchange, twice, and the exponentials: 24 clocks for a warp's 32, 0.13 us for a tile of
+// eight heads), 2 us for the outputs: 18 us for one sequence of 300 keys, 23 for one of 4096 (the contiguous caches' kernels, whose CTAs of a head are a cluster or
+// know their place without a plan, 11 and 16 with the append in them).  A KV head with more than eight query heads is as many pairs as it has groups of eight, and
+// its rows are read for each: 64 sequences of 4096 keys over one KV head 60 us with 8 heads, 99 with 16, 178 with 32.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>

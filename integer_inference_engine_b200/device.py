@@ -337,7 +337,9 @@ def paged_select(q: torch.Tensor, bounds: torch.Tensor, table: torch.Tensor, len
                  out: torch.Tensor | None = None) -> torch.Tensor:
     """The ``n_select`` logical pages of every sequence and KV head that the new token attends to: the first ``keep_first`` and last
     ``keep_last`` visible ones, then those whose keys can score highest, judged by the page's ``bounds`` (:func:`paged_append`): the largest, over
-    the query heads of the KV head, of ``sum_i max(q_i largest_i, q_i smallest_i)``, modulo 2**64; the lowest page among equals.
+    the query heads of the KV head, of ``sum_i max(q_i largest_i, q_i smallest_i)``, modulo 2**64; the lowest page among equals.  A page number
+    outside the pool ranks lowest and raises bit 4 of :func:`read_flags`; where a sequence has ``n_select`` pages or fewer all are listed and no
+    number is looked at.
     ``q``, ``table``, ``lengths``, ``window`` and the rotation as for :func:`paged_attention`.  Returns int32 [B, n_kv, n_select], ascending, -1 behind
     the last: its ``pages``."""
     if bounds.dim() != 4 or bounds.shape[2] != 2 or bounds.dtype != torch.int32 or not bounds.is_contiguous() or bounds.numel() == 0:
